@@ -630,6 +630,76 @@ int mtpk_kv_write(const uint16_t* k, int64_t k_row_stride, const uint16_t* v, in
                   int64_t keep_s, int64_t batch, int64_t t, int64_t kv_heads, int64_t head_dim,
                   void* stream);
 
+/* ---------------------------------------------------------------- position rotation of heads
+ * Heads x (f32 or bf16; element d of head h of token i at i * x_strides[0] + h * x_strides[1] + d, two
+ * int64 strides) normed, when w is given (f32 or bf16 [dim]), by x * rsqrt(mean(x^2) + eps) * (1 + w),
+ * then rotated at pos[i] (int64 [tokens]): the first rot_dim channels are pairs, (i, i + rot_dim / 2) or,
+ * with interleaved, (2 i, 2 i + 1), and pair i is turned by pos * rates[i] radians (f64 [rot_dim / 2],
+ * the angle reduced in 64 bits) and multiplied by magnitude. out: x's type, strides like x's; it may be x
+ * itself. fp32 arithmetic, one rounding. dim a multiple of 8 up to 512, rot_dim even, 2 .. dim; 16-byte
+ * aligned rows. The rates of a scaled context are the caller's (rotary.frequencies). No reference
+ * counterpart in this form (`apply_rope`, model.py:631-635, takes fp32 tables: mtpk_rownorm). */
+int mtpk_rotate(const void* x, int dtype, const int64_t* x_strides, int64_t tokens, int64_t heads,
+                int64_t dim, const void* w, int w_dtype, float eps, const int64_t* pos,
+                const double* rates, int rot_dim, int interleaved, float magnitude, void* out,
+                const int64_t* out_strides, void* stream);
+
+/* The q and k heads of this round's rows normed and rotated as above, k and v into the paged caches, in
+ * one launch (mtpk_rownorm of q, of k, and mtpk_kv_write, for a rotation without tables). q, k, v and out
+ * bf16: element d of (lane b, head h, step s) at b * strides[0] + h * strides[1] + s * strides[2] + d
+ * (three int64 strides each, multiples of 8; 16-byte aligned). q_norm, k_norm (norm_dtype f32 | bf16
+ * [head_dim], each may be NULL: no norm). Step s of lane b is at base_pos[b] + s, rotated at
+ * positions[b * t + s] when positions is given (int64 [batch, t]); its k and v go where
+ * mtpk_kv_write puts them, with its keep (rows with 0, and positions outside the lane's table or the
+ * pool, are not written; their q rows are). out [batch, t, heads, head_dim]. head_dim as dim above. */
+int mtpk_rotate_to_cache(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
+                         const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
+                         const void* q_norm, const void* k_norm, int norm_dtype, float eps,
+                         const double* rates, int rot_dim, int interleaved, float magnitude,
+                         uint16_t* k_pool, uint16_t* v_pool, int64_t pool_rows,
+                         const int32_t* block_table, int64_t table_stride, const int64_t* base_pos,
+                         const int64_t* positions, const uint8_t* keep, int64_t keep_b, int64_t keep_s,
+                         int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                         uint16_t* out, const int64_t* out_strides, void* stream);
+
+/* ---------------------------------------------------------------- masked paged attention
+ * mtpk_paged_attention_gated's operands with scores that are capped or biased, and masks beyond the
+ * causal order. For the row at p = base_pos[b] + s of q head h and the key at j:
+ *   x = scale * q . k_j;  x = softcap * tanh(x / softcap) when softcap > 0;
+ *   x -= slopes[h] * |p - j| when slopes is given (f32 [heads]);
+ * seen iff j >= first[b * t + s] (int32 | int64 [batch, t], may be NULL: the row's document), p - j <
+ * window (0: none), and j <= p or both p and j below prefix[b] (int32 | int64 [batch], may be NULL); keys
+ * at or past base_pos[b] + t, or past the table, are never seen. out = the softmax's sum over the seen
+ * keys, 0 for a row that sees none, times sigmoid(gate) when gate is given, rounded once. Keys that no row
+ * sees may hold anything, and one row's keys do not touch another row. Query, gate and output strides
+ * multiples of 8, rows 16-byte aligned. Pools of any size; table_stride <= 2^26.
+ * n_split from mtpk_attention_masked_splits (0 for a shape that is not taken; max_ctx a bound on
+ * base_pos + t), at most 64; n_split > 1 needs mtpk_attention_masked_workspace_bytes of workspace
+ * (16-byte aligned). No reference counterpart. */
+int mtpk_attention_masked_splits(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                 int64_t max_ctx, int64_t window);
+int64_t mtpk_attention_masked_workspace_bytes(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads,
+                                              int64_t head_dim, int n_split);
+int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, const uint16_t* gate,
+                                const int64_t* gate_strides, int64_t batch, int64_t t, int64_t heads,
+                                int64_t kv_heads, int64_t head_dim, const uint16_t* k_pool,
+                                const uint16_t* v_pool, int64_t pool_rows, const int32_t* block_table,
+                                int64_t table_stride, const int64_t* base_pos, float scale, float softcap,
+                                int64_t window, const float* slopes, const void* prefix, int prefix_dtype,
+                                const void* first, int first_dtype, int n_split, void* workspace,
+                                int64_t workspace_bytes, uint16_t* out, const int64_t* out_strides,
+                                void* stream);
+
+/* ---------------------------------------------------------------- copies of cache blocks
+ * Block dst[i] = block src[i] (int32 | int64 [pairs], on the device) in each of n_pools pools, in one
+ * launch per 64 pools: forked lanes' last blocks, blocks that a compaction moves. pools and block_bytes
+ * are host arrays; pool p holds n_blocks blocks of block_bytes[p] bytes (a multiple of 16; pools 16-byte
+ * aligned). A pair with an id outside [0, n_blocks) is skipped. A block may be the source of several
+ * pairs; no block may be the destination of two, nor source of one and destination of another. No
+ * reference counterpart (`block_pool.py` hands out blocks and never moves them). */
+int mtpk_copy_blocks(void* const* pools, const int64_t* block_bytes, int n_pools, int64_t n_blocks,
+                     const void* src, const void* dst, int index_dtype, int64_t pairs, void* stream);
+
 /* Streaming-read probe (no reference counterpart: a measurement of the HBM read ceiling the MoE
  * weight streams are compared with). Reads bytes [0, bytes) of `base` with 16-byte loads,
  * `loads_in_flight` (4, 8 or 16) per thread per iteration, over `grid` workgroups of 256

@@ -6,6 +6,7 @@ missing or does not load, every device entry point raises: there is no silent fa
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_int, c_int64, c_void_p
@@ -221,6 +222,27 @@ _SIGNATURES: dict[str, tuple[object, list]] = {
          c_void_p],
     ),
     "mtpk_probe_mfma_16x16x32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mtpk_rotate": (
+        c_int,
+        [c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, ctypes.c_float, c_void_p,
+         c_void_p, c_int, c_int, ctypes.c_float, c_void_p, c_void_p, c_void_p],
+    ),
+    "mtpk_rotate_to_cache": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+         ctypes.c_float, c_void_p, c_int, c_int, ctypes.c_float, c_void_p, c_void_p, c_int64, c_void_p,
+         c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_int64, c_void_p, c_void_p, c_void_p],
+    ),
+    "mtpk_attention_masked_splits": (c_int, [c_int64] * 7),
+    "mtpk_attention_masked_workspace_bytes": (c_int64, [c_int64] * 5 + [c_int]),
+    "mtpk_paged_attention_masked": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+         c_void_p, c_int64, c_void_p, c_int64, c_void_p, ctypes.c_float, ctypes.c_float, c_int64, c_void_p,
+         c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
+    ),
+    "mtpk_copy_blocks": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
     "mtpk_probe_stream": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),
     "mtpk_delta_rule": (
         c_int,
@@ -303,6 +325,27 @@ def row_stride(x: torch.Tensor) -> int | None:
 def stream_of(device: torch.device) -> int:
     """Handle of torch's current stream on `device` (what the kernels launch on)."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """A context in which `device` is the current one: launches and workgroup counts go by it, also
+    where the tensors are not on the device that the caller has selected."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def strides(x: torch.Tensor, *dims: int) -> ctypes.Array:
+    """Element strides of the named dims as an int64 array (a host pointer for the C entry points)."""
+    return (c_int64 * len(dims))(*[x.stride(d) for d in dims])
+
+
+def rows16(x: torch.Tensor, *dims: int) -> bool:
+    """Whether every row of `x` (unit stride over the last dim, rows along `dims`) starts on 16 bytes;
+    a size-1 dim's stride is arbitrary but is multiplied by 0 alone, so it may be anything divisible."""
+    unit = 16 // x.element_size()
+    return x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(x.stride(d) % unit == 0 for d in dims)
 
 
 def float_code(dtype: torch.dtype) -> int:

@@ -13,6 +13,7 @@ bf16 `[B, heads, t, hd]`.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -178,3 +179,162 @@ def kv_write(k_pool: torch.Tensor, v_pool: torch.Tensor, k: torch.Tensor, v: tor
         k.data_ptr(), _mtpk.row_stride(k), v.data_ptr(), _mtpk.row_stride(v), k_pool.data_ptr(), v_pool.data_ptr(),
         k_pool.shape[0], table.data_ptr(), table.shape[1], pos.data_ptr(), _mtpk.ptr(kp), kb, ks, b, t,
         kvh, hd, _mtpk.stream_of(device)), "mtpk_kv_write")  # fmt: skip
+
+
+def check_cache(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, base_pos: torch.Tensor,
+                batch: int, head_dim: int) -> None:
+    """Raise unless the pools are a K and a V cache of `head_dim`, contiguous bf16, with an integer table
+    and base position for each of `batch` lanes."""
+    rows, kvh = k_pool.shape[0], k_pool.shape[1] if k_pool.dim() == 3 else 0
+    if k_pool.dim() != 3 or k_pool.shape[2] != head_dim or rows % BLOCK or rows == 0:
+        raise ValueError(f"k_pool must be [rows, kv_heads, {head_dim}] of {BLOCK}-row blocks, got {tuple(k_pool.shape)}")
+    if tuple(v_pool.shape) != (rows // BLOCK, kvh, head_dim, BLOCK):
+        raise ValueError(f"v_pool must be [{rows // BLOCK}, {kvh}, {head_dim}, {BLOCK}] "
+                         f"(V transposed per block), got {tuple(v_pool.shape)}")
+    if k_pool.dtype != torch.bfloat16 or v_pool.dtype != torch.bfloat16 or not (
+            k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError("pools must be contiguous bf16")
+    if block_table.dim() != 2 or block_table.shape[0] != batch or tuple(base_pos.shape) != (batch,):
+        raise ValueError(f"block_table must be [{batch}, blocks] and base_pos [{batch}], got "
+                         f"{tuple(block_table.shape)} and {tuple(base_pos.shape)}")
+    if block_table.dtype not in (torch.int32, torch.int64) or base_pos.dtype not in (torch.int32, torch.int64):
+        raise ValueError("block_table and base_pos must be int32 or int64")
+
+
+def table_and_base(block_table: torch.Tensor, base_pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The types that the kernels read: int32 table, int64 positions, contiguous."""
+    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
+    pos = base_pos if base_pos.dtype == torch.int64 else base_pos.to(torch.int64)
+    return table.contiguous(), pos.contiguous()
+
+
+def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                           base_pos: torch.Tensor, ctx_len: int, scale: float, *, softcap: float = 0.0,
+                           window: int = 0, slopes: torch.Tensor | None = None,
+                           prefix: torch.Tensor | None = None, first: torch.Tensor | None = None,
+                           gate: torch.Tensor | None = None) -> torch.Tensor:
+    """`paged_attention_gated` with scores that are capped or biased and masks beyond the causal order
+    (`mtpk_paged_attention_masked`). q `[B, t, heads, hd]`, any strides; returns `[B, t, heads, hd]`
+    contiguous. For the row at position p and the key at j:
+
+    `softcap` c > 0: the scaled score x becomes `c * tanh(x / c)`. `slopes` fp32 `[heads]`: minus
+    `slopes[h] * |p - j|`. The row sees j iff `j <= p`, or p and j are both below `prefix[b]` (integers
+    `[B]`; at most `base_pos[b] + t` counts); and `p - j < window` (0: no window); and `j >= first[b, s]`
+    (integers `[B, t]`: the first position of the row's document). A row that sees nothing is zeros.
+    `gate` of q's shape multiplies the output by its sigmoid. Keys that a row does not see never reach its
+    output, whatever they hold. `ctx_len` is a host bound on `max(base_pos) + t`; it sizes the key splits
+    alone. bf16 with fp32 scores, statistics and sums; the output is rounded once."""
+    device = _mtpk.require_device(q, k_pool, v_pool, block_table, base_pos)
+    if q.dim() != 4 or q.dtype != torch.bfloat16:
+        raise ValueError(f"q must be bf16 [B, t, heads, hd], got {q.dtype} {tuple(q.shape)}")
+    b, t, heads, hd = q.shape
+    if hd not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {hd}")
+    check_cache(k_pool, v_pool, block_table, base_pos, b, hd)
+    kvh = k_pool.shape[1]
+    if heads == 0 or kvh == 0 or heads % kvh:
+        raise ValueError(f"{heads} q heads are not a multiple of {kvh} kv heads")
+    if not 0 <= int(ctx_len) <= block_table.shape[1] * BLOCK:
+        raise ValueError(f"context bound {ctx_len} exceeds the table's {block_table.shape[1]} blocks")
+    if not 0 < scale < math.inf or not 0 <= softcap < math.inf or window < 0:
+        raise ValueError(f"scale must be positive, softcap and window not negative, got {scale}, {softcap} and {window}")
+    if gate is not None and (gate.shape != q.shape or gate.dtype != torch.bfloat16 or gate.device != device):
+        raise ValueError("gate must be bf16 of q's shape on its device")
+    if slopes is not None:
+        if slopes.shape != (heads,) or slopes.dtype != torch.float32 or slopes.device != device:
+            raise ValueError(f"slopes must be float32 [{heads}] on {device}")
+        slopes = slopes.contiguous()
+    prefix = _integers(prefix, "prefix", (b,), device)
+    first = _integers(first, "first", (b, t), device)
+    out = torch.empty(b, t, heads, hd, dtype=torch.bfloat16, device=device)
+    if out.numel() == 0:
+        return out
+    if not _mtpk.rows16(q, 0, 1, 2):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if gate is not None and not _mtpk.rows16(gate, 0, 1, 2):
+        gate = gate.clone(memory_format=torch.contiguous_format)
+    table, pos = table_and_base(block_table, base_pos)
+    lib = _mtpk.lib()
+    with _mtpk.on(device):
+        n_split = lib.mtpk_attention_masked_splits(b, t, heads, kvh, hd, int(ctx_len), int(window))
+        ws, ws_bytes = None, 0
+        if n_split > 1:
+            ws_bytes = lib.mtpk_attention_masked_workspace_bytes(b, t, heads, kvh, hd, n_split)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        qs, os_ = _strides(q), _strides(out)
+        gs = _strides(gate) if gate is not None else None
+        _mtpk.check(lib.mtpk_paged_attention_masked(
+            q.data_ptr(), ctypes.addressof(qs), _mtpk.ptr(gate), ctypes.addressof(gs) if gs else None, b, t, heads,
+            kvh, hd, k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], table.data_ptr(), table.shape[1],
+            pos.data_ptr(), scale, softcap, int(window), _mtpk.ptr(slopes), _mtpk.ptr(prefix), _code(prefix),
+            _mtpk.ptr(first), _code(first), n_split, _mtpk.ptr(ws), ws_bytes, out.data_ptr(),
+            ctypes.addressof(os_), _mtpk.stream_of(device)), "mtpk_paged_attention_masked")  # fmt: skip
+    return out
+
+
+def _integers(x: torch.Tensor | None, name: str, shape: tuple, device: torch.device) -> torch.Tensor | None:
+    if x is None:
+        return None
+    if tuple(x.shape) != shape or x.dtype not in (torch.int32, torch.int64) or x.device != device:
+        raise ValueError(f"{name} must be int32 or int64 {list(shape)} on {device}, got {x.dtype} {tuple(x.shape)}")
+    return x.contiguous()
+
+
+def _code(x: torch.Tensor | None) -> int:
+    return 0 if x is None else _mtpk.index_code(x.dtype)
+
+
+def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None:
+    """Block `dst[i]` of every pool becomes block `src[i]` of it, in one launch (`mtpk_copy_blocks`): K pools
+    `[rows, kv_heads, hd]` and V pools `[rows / block, kv_heads, hd, block]` of one cache's layers.
+
+    `src` and `dst` are block ids of equal length: lists or CPU tensors, which are checked (each id inside
+    the pools, no block the destination of two pairs, nor source of one and destination of another;
+    `ValueError`) and copied to the device, or int32 / int64 device tensors, which are taken as they are:
+    a pair with an id outside the pools is skipped, and the rest of the rule is the caller's. CPU pools
+    take the torch spelling."""
+    if not pools:
+        raise ValueError("copy_blocks takes at least one pool")
+    device, n_blocks = pools[0].device, 0
+    for p in pools:
+        n = p.shape[0] if p.dim() == 4 else p.shape[0] // block if p.dim() == 3 and p.shape[0] % block == 0 else 0
+        n_blocks = n_blocks or n
+        if n != n_blocks or p.numel() == 0 or not p.is_contiguous() or p.device != device:
+            raise ValueError("pools must be contiguous K caches [rows, kv_heads, hd] and V caches [blocks, kv_heads, hd, "
+                             f"{block}] of one number of blocks on one device, got {tuple(p.shape)} on {p.device}")
+    checked = not (torch.is_tensor(src) and src.is_cuda)
+    if checked != (not (torch.is_tensor(dst) and dst.is_cuda)):
+        raise ValueError("src and dst must both be on the host or both on the device")
+    if checked:
+        src, dst = (torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in (src, dst))
+    if src.shape != dst.shape or src.dim() != 1 or src.dtype not in (torch.int32, torch.int64) or src.dtype != dst.dtype:
+        raise ValueError("src and dst must be int32 or int64 vectors of one length and type")
+    pairs = src.shape[0]
+    if pairs == 0:
+        return
+    if checked:
+        if int(min(src.min(), dst.min())) < 0 or int(max(src.max(), dst.max())) >= n_blocks:
+            raise ValueError(f"block ids must lie in [0, {n_blocks})")
+        kinds = torch.zeros(n_blocks, dtype=torch.int32)
+        kinds.index_add_(0, dst, torch.ones(pairs, dtype=torch.int32))
+        if int(kinds.max()) > 1 or int(kinds[src].max()) > 0:
+            raise ValueError("a block is the destination of two pairs, or source and destination")
+    if device.type == "cpu":
+        for p in pools:
+            blocks = p.view(n_blocks, -1)
+            blocks[dst] = blocks[src]
+        return
+    if checked:
+        src, dst = torch.stack((src, dst)).pin_memory().to(device, non_blocking=True).unbind(0)
+    elif src.device != device or dst.device != device:
+        raise ValueError(f"src and dst must be on {device}")
+    sizes = [p.numel() // n_blocks * p.element_size() for p in pools]
+    if any(s % 16 or p.data_ptr() % 16 for s, p in zip(sizes, pools)):
+        raise ValueError("blocks must be multiples of 16 bytes and lie on 16 bytes")
+    src, dst = src.contiguous(), dst.contiguous()
+    ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
+    bytes_ = (ctypes.c_int64 * len(pools))(*sizes)
+    with _mtpk.on(device):
+        _mtpk.check(_mtpk.lib().mtpk_copy_blocks(
+            ctypes.addressof(ptrs), ctypes.addressof(bytes_), len(pools), n_blocks, src.data_ptr(), dst.data_ptr(),
+            _mtpk.index_code(src.dtype), pairs, _mtpk.stream_of(device)), "mtpk_copy_blocks")  # fmt: skip

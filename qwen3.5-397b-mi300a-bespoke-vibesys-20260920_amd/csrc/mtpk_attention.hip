@@ -21,6 +21,7 @@
 
 #include <algorithm>
 
+#include "mtpk_attention_common.h"
 #include "mtpk_device.h"
 #include "mtpk_host.h"
 
@@ -30,7 +31,6 @@ constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = kAttnWaves * kWave;
 constexpr int kAttnRows = 16 * kAttnWaves;  // query rows per workgroup
 constexpr int kAttnKeys = 32;               // keys per staged tile
-constexpr int kAttnBlock = 16;              // KV cache block size
 
 template <int HD>
 struct AttnGeom {
@@ -80,14 +80,9 @@ __device__ inline float row16_sum(float v) {
   return v;
 }
 
-// Where the query rows come from and the output rows go: element d of (lane b, q head h, step s)
-// is at b * sb + h * sh + s * st + d of each tensor (unit stride over d). With `gate`, the stored
+// Where the query rows come from and the output rows go. With `gate`, the stored
 // output is bf16(bf16(o) * bf16(sigmoid(gate))), the rounding of the torch chain
 // `out * torch.sigmoid(gate)` on bf16 tensors (`model.py:2158-2290`).
-struct AttnRows {
-  int64_t sb, sh, st;
-  __device__ inline int64_t at(int b, int h, int s) const { return b * sb + h * sh + s * st; }
-};
 struct AttnIO {
   const uint16_t* q;
   AttnRows qr;

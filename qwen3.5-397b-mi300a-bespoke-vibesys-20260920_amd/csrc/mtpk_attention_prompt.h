@@ -25,12 +25,9 @@
 // that chain but run in lockstep, matrix unit and softmax taking turns: slower by a quarter.
 #pragma once
 
-#include "mtpk_device.h"
+#include "mtpk_attention_common.h"
 
 namespace mtpk {
-
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kPromptRows = 128;  // query rows per workgroup
 constexpr int kPromptKeys = 32;   // keys per tile
@@ -47,13 +44,6 @@ __device__ __host__ inline int prompt_keys_end(int bp, int rg, int rows, int gro
   const int last = rg * kPromptRows + kPromptRows - 1;
   return bp + (last < rows ? last : rows - 1) / group + 1;
 }
-
-// Bits 2 and 3 of a tile's key or row index swapped.
-__device__ inline int prompt_swap(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
-
-// The change of place of a K row's pieces: the rows 0..3 and 0..7 that one LDS cycle reads, of either
-// half of the wave, then lie in different bank groups.
-__device__ inline int prompt_flip(int row) { return ((row & 3) << 1) | (row >> 2 & 1); }
 
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_prompt_attention(

@@ -377,6 +377,11 @@ class BlockTables:
     Block 0 is never handed out: unused table entries point at it, so a padded read stays in
     bounds and reads rows no lane owns (`block_pool.py:38`). Blocks are handed out in a seeded
     shuffled order so that a lane's physical rows are not contiguous.
+
+    A block may be held by several lanes (`fork`): it goes back to the free ones when the last of them
+    lets go of it. `fork` and `compact` return the block copies that they ask for, as `(src, dst)` lists
+    for `attention.copy_blocks` over every pool that is read through these tables; the tables themselves
+    are written at once, so the copies come before the next read or write through them.
     """
 
     def __init__(self, lanes: int, max_seq: int, block_size: int, device: torch.device,
@@ -388,6 +393,7 @@ class BlockTables:
         self._free = (torch.randperm(self.n_blocks - 1, generator=gen) + 1).tolist()
         self.host = [[] for _ in range(lanes)]
         self.held_positions = [0] * lanes  # len(host[lane]) * block_size
+        self._holders: dict[int, int] = {}  # of the blocks that more than one lane holds
         self.table = torch.zeros(lanes, self.max_blocks, dtype=torch.int32, device=device)
         self.device = device
 
@@ -437,10 +443,78 @@ class BlockTables:
         self.table[u[:, 0], u[:, 1]] = u[:, 2].to(torch.int32)
 
     def release(self, lane: int) -> None:
-        self._free.extend(reversed(self.host[lane]))
+        self._let_go(self.host[lane])
         self.host[lane] = []
         self.held_positions[lane] = 0
         self.table[lane].zero_()
+
+    def _let_go(self, blocks: list[int]) -> None:
+        for block in reversed(blocks):
+            left = self._holders.pop(block, 1) - 1
+            if left > 1:
+                self._holders[block] = left
+            elif left == 0:
+                self._free.append(block)
+
+    def trim(self, lane: int, length: int) -> None:
+        """Let go of the blocks of lane `lane` past its first `length` positions."""
+        if length < 0:
+            raise ValueError(f"lane {lane}: cannot keep {length} positions")
+        need = (length + self.block_size - 1) // self.block_size
+        have = self.host[lane]
+        if need >= len(have):
+            return
+        self._let_go(have[need:])
+        self.table[lane, need : len(have)] = 0
+        del have[need:]
+        self.held_positions[lane] = need * self.block_size
+
+    def fork(self, src: int, dst: int, length: int) -> tuple[list[int], list[int]]:
+        """Lane `dst`, which holds nothing, continues after the first `length` positions of lane `src`: it
+        shares the whole blocks below `length`, and takes a block of its own for a last partly filled one.
+        Returns that block's copy, at most one `(src, dst)` pair. Either lane then writes at or past
+        `length` without the other's notice; a write below it into a shared block is seen by both."""
+        whole, part = divmod(length, self.block_size)
+        need = whole + (part > 0)
+        if src == dst or self.host[dst]:
+            raise ValueError(f"lane {dst} holds blocks: release it before it becomes a fork")
+        if not 0 <= length <= self.held_positions[src]:
+            raise ValueError(f"lane {src} holds {self.held_positions[src]} positions, not {length}")
+        if part and not self._free:
+            raise ValueError("no free block for the fork's last one")
+        mine = self.host[src][:whole]
+        pairs: tuple[list[int], list[int]] = ([], [])
+        for block in mine:
+            self._holders[block] = self._holders.get(block, 1) + 1
+        if part:
+            pairs[0].append(self.host[src][whole])
+            pairs[1].append(self._free.pop())
+            mine.append(pairs[1][0])
+        self.host[dst] = mine
+        self.held_positions[dst] = need * self.block_size
+        if whole:
+            self.table[dst, :whole] = self.table[src, :whole]
+        if part:
+            self.table[dst, whole] = pairs[1][0]
+        return pairs
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Move every held block to the lowest ids, `1 ..` their count, so that the free ones are the pools'
+        tail: returns the moves as `(src, dst)` lists (no block is in both) and writes the tables."""
+        held = sorted({block for have in self.host for block in have})
+        low = set(range(1, len(held) + 1))
+        src = [block for block in held if block not in low]
+        dst = sorted(low.difference(held))
+        to = dict(zip(src, dst, strict=True))
+        self.host = [[to.get(block, block) for block in have] for have in self.host]
+        self._holders = {to.get(block, block): n for block, n in self._holders.items()}
+        self._free = list(range(self.n_blocks - 1, len(held), -1))  # the lowest is handed out first
+        if src:
+            table = torch.zeros(self.lanes, self.max_blocks, dtype=torch.int32)
+            for lane, have in enumerate(self.host):
+                table[lane, : len(have)] = torch.tensor(have, dtype=torch.int32)
+            self.table.copy_(table)
+        return src, dst
 
     def physical_rows(self, lanes: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         """Physical pool rows of positions `pos` `[B, t]` of lanes `lanes` `[B]` (device)."""
@@ -617,6 +691,31 @@ class Model:
                 p["conv"][lane].zero_()
                 p["rec"][lane].zero_()
         self.hidden_cache[lane].zero_()
+
+    def caches(self, *more: dict) -> list[torch.Tensor]:
+        """The K and V pools of the attention layers, and of `more` (an MTP head's `pool`)."""
+        own = [p for ty, p in zip(self.cfg.layer_types, self.pool) if ty == ATTN]
+        return [p[name] for p in (*own, *more) for name in ("k", "v")]
+
+    def fork(self, src: int, dst: int, length: int, *more: dict) -> None:
+        """Slot `dst`, which is reset, becomes a second continuation of slot `src` after its `length`
+        committed positions: blocks shared (`BlockTables.fork`), its last block, DeltaNet state and cached
+        hidden copied. `more`: pools beside the layers' that are read through the same tables."""
+        pairs = self.blocks.fork(src, dst, length)
+        if pairs[0]:
+            attention.copy_blocks(self.caches(*more), *pairs, self.cfg.block_size)
+        for ty, p in zip(self.cfg.layer_types, self.pool):
+            if ty != ATTN:
+                p["conv"][dst].copy_(p["conv"][src])
+                p["rec"][dst].copy_(p["rec"][src])
+        self.hidden_cache[dst].copy_(self.hidden_cache[src])
+
+    def compact(self, *more: dict) -> int:
+        """Move the held cache blocks to the pools' front (`BlockTables.compact`); returns how many moved."""
+        src, dst = self.blocks.compact()
+        if src:
+            attention.copy_blocks(self.caches(*more), src, dst, self.cfg.block_size)
+        return len(src)
 
     # ------------------------------------------------------------ sublayers
 
