@@ -323,8 +323,9 @@ def row_stride(x: torch.Tensor) -> int | None:
 
 
 def stream_of(device: torch.device) -> int:
-    """Handle of torch's current stream on `device` (what the kernels launch on)."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of torch's current stream on `device` (what the kernels launch on): the handle alone, without
+    the Stream object around it (0.1 against 2.1 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 _HERE = contextlib.nullcontext()
@@ -336,16 +337,15 @@ def on(device: torch.device):
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
-def strides(x: torch.Tensor, *dims: int) -> ctypes.Array:
-    """Element strides of the named dims as an int64 array (a host pointer for the C entry points)."""
-    return (c_int64 * len(dims))(*[x.stride(d) for d in dims])
-
-
-def rows16(x: torch.Tensor, *dims: int) -> bool:
-    """Whether every row of `x` (unit stride over the last dim, rows along `dims`) starts on 16 bytes;
-    a size-1 dim's stride is arbitrary but is multiplied by 0 alone, so it may be anything divisible."""
-    unit = 16 // x.element_size()
-    return x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(x.stride(d) % unit == 0 for d in dims)
+def rows16(x: torch.Tensor) -> bool:
+    """Whether every row of `x` along its last dim is contiguous and starts on 16 bytes."""
+    unit, strides = 16 // x.element_size(), x.stride()
+    if strides[-1] != 1 or x.data_ptr() % 16:
+        return False
+    for s in strides[:-1]:
+        if s % unit:
+            return False
+    return True
 
 
 def float_code(dtype: torch.dtype) -> int:

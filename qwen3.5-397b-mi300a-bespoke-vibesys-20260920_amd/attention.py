@@ -181,31 +181,30 @@ def kv_write(k_pool: torch.Tensor, v_pool: torch.Tensor, k: torch.Tensor, v: tor
         kvh, hd, _mtpk.stream_of(device)), "mtpk_kv_write")  # fmt: skip
 
 
-def check_cache(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, base_pos: torch.Tensor,
-                batch: int, head_dim: int) -> None:
-    """Raise unless the pools are a K and a V cache of `head_dim`, contiguous bf16, with an integer table
-    and base position for each of `batch` lanes."""
-    rows, kvh = k_pool.shape[0], k_pool.shape[1] if k_pool.dim() == 3 else 0
-    if k_pool.dim() != 3 or k_pool.shape[2] != head_dim or rows % BLOCK or rows == 0:
-        raise ValueError(f"k_pool must be [rows, kv_heads, {head_dim}] of {BLOCK}-row blocks, got {tuple(k_pool.shape)}")
-    if tuple(v_pool.shape) != (rows // BLOCK, kvh, head_dim, BLOCK):
-        raise ValueError(f"v_pool must be [{rows // BLOCK}, {kvh}, {head_dim}, {BLOCK}] "
-                         f"(V transposed per block), got {tuple(v_pool.shape)}")
-    if k_pool.dtype != torch.bfloat16 or v_pool.dtype != torch.bfloat16 or not (
-            k_pool.is_contiguous() and v_pool.is_contiguous()):
+def cache_operands(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, base_pos: torch.Tensor,
+                   batch: int, kv_heads: int, head_dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """`(table, base)` as the kernels read them, contiguous int32 and int64; raises unless the pools are a
+    K and a V cache of these heads, contiguous bf16, with a table and a base position for each lane."""
+    rows = k_pool.shape[0]
+    if k_pool.shape != (rows, kv_heads, head_dim) or rows % BLOCK or rows == 0:
+        raise ValueError(f"k_pool must be [rows, {kv_heads}, {head_dim}] of {BLOCK}-row blocks, got {list(k_pool.shape)}")
+    if v_pool.shape != (rows // BLOCK, kv_heads, head_dim, BLOCK):
+        raise ValueError(f"v_pool must be {[rows // BLOCK, kv_heads, head_dim, BLOCK]} (V transposed per block), "
+                         f"got {list(v_pool.shape)}")
+    if not k_pool.dtype == v_pool.dtype == torch.bfloat16 or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("pools must be contiguous bf16")
-    if block_table.dim() != 2 or block_table.shape[0] != batch or tuple(base_pos.shape) != (batch,):
+    if block_table.dim() != 2 or block_table.shape[0] != batch or base_pos.shape != (batch,):
         raise ValueError(f"block_table must be [{batch}, blocks] and base_pos [{batch}], got "
-                         f"{tuple(block_table.shape)} and {tuple(base_pos.shape)}")
-    if block_table.dtype not in (torch.int32, torch.int64) or base_pos.dtype not in (torch.int32, torch.int64):
-        raise ValueError("block_table and base_pos must be int32 or int64")
-
-
-def table_and_base(block_table: torch.Tensor, base_pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """The types that the kernels read: int32 table, int64 positions, contiguous."""
-    table = block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)
-    pos = base_pos if base_pos.dtype == torch.int64 else base_pos.to(torch.int64)
-    return table.contiguous(), pos.contiguous()
+                         f"{list(block_table.shape)} and {list(base_pos.shape)}")
+    if block_table.dtype != torch.int32:
+        if block_table.dtype != torch.int64:
+            raise ValueError(f"block_table must be int32 or int64, got {block_table.dtype}")
+        block_table = block_table.to(torch.int32)
+    if base_pos.dtype != torch.int64:
+        if base_pos.dtype != torch.int32:
+            raise ValueError(f"base_pos must be int32 or int64, got {base_pos.dtype}")
+        base_pos = base_pos.to(torch.int64)
+    return block_table.contiguous(), base_pos.contiguous()
 
 
 def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -230,58 +229,64 @@ def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     b, t, heads, hd = q.shape
     if hd not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {hd}")
-    check_cache(k_pool, v_pool, block_table, base_pos, b, hd)
+    if k_pool.dim() != 3:
+        raise ValueError(f"k_pool must be [rows, kv_heads, {hd}], got {list(k_pool.shape)}")
     kvh = k_pool.shape[1]
+    table, pos = cache_operands(k_pool, v_pool, block_table, base_pos, b, kvh, hd)
     if heads == 0 or kvh == 0 or heads % kvh:
         raise ValueError(f"{heads} q heads are not a multiple of {kvh} kv heads")
-    if not 0 <= int(ctx_len) <= block_table.shape[1] * BLOCK:
-        raise ValueError(f"context bound {ctx_len} exceeds the table's {block_table.shape[1]} blocks")
+    if not 0 <= ctx_len <= table.shape[1] * BLOCK:
+        raise ValueError(f"context bound {ctx_len} exceeds the table's {table.shape[1]} blocks")
     if not 0 < scale < math.inf or not 0 <= softcap < math.inf or window < 0:
         raise ValueError(f"scale must be positive, softcap and window not negative, got {scale}, {softcap} and {window}")
-    if gate is not None and (gate.shape != q.shape or gate.dtype != torch.bfloat16 or gate.device != device):
-        raise ValueError("gate must be bf16 of q's shape on its device")
+    gs = prefix_dt = first_dt = 0
+    if gate is not None:
+        if gate.shape != q.shape or gate.dtype != torch.bfloat16 or gate.device != device:
+            raise ValueError("gate must be bf16 of q's shape on its device")
+        if not _mtpk.rows16(gate):
+            gate = gate.clone(memory_format=torch.contiguous_format)
+        s = gate.stride()
+        gate_strides = _Three(s[0], s[2], s[1])
+        gs = ctypes.addressof(gate_strides)
     if slopes is not None:
         if slopes.shape != (heads,) or slopes.dtype != torch.float32 or slopes.device != device:
             raise ValueError(f"slopes must be float32 [{heads}] on {device}")
         slopes = slopes.contiguous()
-    prefix = _integers(prefix, "prefix", (b,), device)
-    first = _integers(first, "first", (b, t), device)
-    out = torch.empty(b, t, heads, hd, dtype=torch.bfloat16, device=device)
+    if prefix is not None:
+        prefix, prefix_dt = _integers(prefix, "prefix", (b,), device)
+    if first is not None:
+        first, first_dt = _integers(first, "first", (b, t), device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.numel() == 0:
         return out
-    if not _mtpk.rows16(q, 0, 1, 2):
+    if not _mtpk.rows16(q):
         q = q.clone(memory_format=torch.contiguous_format)
-    if gate is not None and not _mtpk.rows16(gate, 0, 1, 2):
-        gate = gate.clone(memory_format=torch.contiguous_format)
-    table, pos = table_and_base(block_table, base_pos)
+    s, z = q.stride(), out.stride()
+    qs, os_ = _Three(s[0], s[2], s[1]), _Three(z[0], z[2], z[1])
     lib = _mtpk.lib()
     with _mtpk.on(device):
-        n_split = lib.mtpk_attention_masked_splits(b, t, heads, kvh, hd, int(ctx_len), int(window))
+        n_split = lib.mtpk_attention_masked_splits(b, t, heads, kvh, hd, ctx_len, window)
         ws, ws_bytes = None, 0
         if n_split > 1:
             ws_bytes = lib.mtpk_attention_masked_workspace_bytes(b, t, heads, kvh, hd, n_split)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-        qs, os_ = _strides(q), _strides(out)
-        gs = _strides(gate) if gate is not None else None
-        _mtpk.check(lib.mtpk_paged_attention_masked(
-            q.data_ptr(), ctypes.addressof(qs), _mtpk.ptr(gate), ctypes.addressof(gs) if gs else None, b, t, heads,
-            kvh, hd, k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], table.data_ptr(), table.shape[1],
-            pos.data_ptr(), scale, softcap, int(window), _mtpk.ptr(slopes), _mtpk.ptr(prefix), _code(prefix),
-            _mtpk.ptr(first), _code(first), n_split, _mtpk.ptr(ws), ws_bytes, out.data_ptr(),
-            ctypes.addressof(os_), _mtpk.stream_of(device)), "mtpk_paged_attention_masked")  # fmt: skip
+        status = lib.mtpk_paged_attention_masked(
+            q.data_ptr(), ctypes.addressof(qs), _mtpk.ptr(gate), gs, b, t, heads, kvh, hd, k_pool.data_ptr(),
+            v_pool.data_ptr(), k_pool.shape[0], table.data_ptr(), table.shape[1], pos.data_ptr(), scale, softcap, window,
+            _mtpk.ptr(slopes), _mtpk.ptr(prefix), prefix_dt, _mtpk.ptr(first), first_dt, n_split, _mtpk.ptr(ws), ws_bytes,
+            out.data_ptr(), ctypes.addressof(os_), _mtpk.stream_of(device))
+    if status:
+        _mtpk.check(status, "mtpk_paged_attention_masked")
     return out
 
 
-def _integers(x: torch.Tensor | None, name: str, shape: tuple, device: torch.device) -> torch.Tensor | None:
-    if x is None:
-        return None
-    if tuple(x.shape) != shape or x.dtype not in (torch.int32, torch.int64) or x.device != device:
-        raise ValueError(f"{name} must be int32 or int64 {list(shape)} on {device}, got {x.dtype} {tuple(x.shape)}")
-    return x.contiguous()
+_Three = ctypes.c_int64 * 3
 
 
-def _code(x: torch.Tensor | None) -> int:
-    return 0 if x is None else _mtpk.index_code(x.dtype)
+def _integers(x: torch.Tensor, name: str, shape: tuple, device: torch.device) -> tuple[torch.Tensor, int]:
+    if x.shape != shape or x.dtype not in (torch.int32, torch.int64) or x.device != device:
+        raise ValueError(f"{name} must be int32 or int64 {list(shape)} on {device}, got {x.dtype} {list(x.shape)}")
+    return x.contiguous(), _mtpk.index_code(x.dtype)
 
 
 def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None:

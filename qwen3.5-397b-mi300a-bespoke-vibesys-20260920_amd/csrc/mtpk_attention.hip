@@ -59,11 +59,6 @@ __device__ __host__ inline void attn_split_range(int ctx, int n_split, int sp, i
 // result: quad_perm swaps (xor 1, xor 2) combine each quad, row_half_mirror (lane i with 7 - i
 // inside each 8) the two quads of a half, row_mirror (i with 15 - i) the two halves. Register
 // moves, no LDS round trip.
-template <int CTRL>
-__device__ inline float dpp_mov(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
-}
-
 __device__ inline float row16_max(float v) {
   v = fmaxf(v, dpp_mov<0xB1>(v));   // quad_perm [1, 0, 3, 2]
   v = fmaxf(v, dpp_mov<0x4E>(v));   // quad_perm [2, 3, 0, 1]

@@ -176,6 +176,14 @@ __device__ inline void store_index(void* p, int dtype, int64_t i, int64_t v) {
     reinterpret_cast<int32_t*>(p)[i] = (int32_t)v;
 }
 
+// A value from another lane of the 16-lane row, by a DPP control: quad_perm [1, 0, 3, 2] is 0xB1 and
+// [2, 3, 0, 1] is 0x4E, row_half_mirror (lane i with 7 - i inside each 8) 0x141, row_mirror (i with
+// 15 - i) 0x140.
+template <int CTRL>
+__device__ inline float dpp_mov(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+
 // Wave-wide reductions over 64 lanes (butterfly: every lane ends with the result).
 __device__ inline float wave_max(float v) {
 #pragma unroll

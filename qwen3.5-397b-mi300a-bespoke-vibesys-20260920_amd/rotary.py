@@ -61,6 +61,9 @@ def frequencies(dim: int, theta: float, *, scaling: str = "none", factor: float 
     return (rates / factor * ramp + rates * (1 - ramp)).to(device), 0.1 * math.log(factor) + 1.0
 
 
+_Two, _Three = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+
+
 def _check_rates(rates: torch.Tensor, dim: int) -> int:
     if rates.dtype != torch.float64 or rates.dim() != 1 or not rates.is_contiguous():
         raise ValueError("rates must be a contiguous float64 [pairs] tensor")
@@ -72,14 +75,10 @@ def _check_rates(rates: torch.Tensor, dim: int) -> int:
     return rot
 
 
-def _check_norm(w: torch.Tensor | None, dim: int, device: torch.device) -> None:
-    if w is not None and (w.shape != (dim,) or w.stride(0) != 1 or w.device != device):
-        raise ValueError(f"a norm's weight must be a contiguous [{dim}] tensor on {device}")
-
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """`x` itself where its rows lie on 16 bytes, else a contiguous copy."""
-    return x if _mtpk.rows16(x, *range(x.dim() - 1)) else x.clone(memory_format=torch.contiguous_format)
+def _check_norm(w: torch.Tensor, dim: int, device: torch.device) -> tuple[torch.Tensor, int]:
+    if w.shape != (dim,) or w.device != device:
+        raise ValueError(f"a norm's weight must be a [{dim}] tensor on {device}")
+    return w if _mtpk.rows16(w) else w.clone(memory_format=torch.contiguous_format), _mtpk.float_code(w.dtype)
 
 
 def rotate(x: torch.Tensor, positions: torch.Tensor, rates: torch.Tensor, *, magnitude: float = 1.0,
@@ -90,47 +89,52 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, rates: torch.Tensor, *, mag
     x's shape and type, or `out` (which may be `x`, but overlap it in no other way). Any strides of x;
     rows that do not lie on 16 bytes are copied first."""
     device = _mtpk.require_device(x, positions, rates)
-    if x.dim() < 2 or tuple(positions.shape) != tuple(x.shape[:-2]):
-        raise ValueError(f"positions must be {tuple(x.shape[:-2])} for heads {tuple(x.shape)}, got {tuple(positions.shape)}")
+    if x.dim() < 2 or positions.shape != x.shape[:-2]:
+        raise ValueError(f"positions must be {list(x.shape[:-2])} for heads {list(x.shape)}, got {list(positions.shape)}")
     heads, dim = x.shape[-2:]
     rot = _check_rates(rates, dim)
-    _check_norm(w, dim, device)
+    dtype = _mtpk.float_code(x.dtype)
+    w_dtype = 0
+    if w is not None:
+        w, w_dtype = _check_norm(w, dim, device)
     if positions.dtype != torch.int64:
-        if positions.dtype.is_floating_point or positions.dtype == torch.bool:
+        if positions.dtype.is_floating_point or positions.dtype.is_complex or positions.dtype == torch.bool:
             raise ValueError("positions must be integers")
         positions = positions.to(torch.int64)
-    dtype = _mtpk.float_code(x.dtype)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != device:
-        raise ValueError(f"out must be {tuple(x.shape)} {x.dtype} on {device}")
-    flat = x if x.dim() == 3 else _tokens(x)
-    to = out if out.dim() == 3 else _tokens(out)
-    if flat is None or not _mtpk.rows16(flat, 0, 1):
-        flat = x.clone(memory_format=torch.contiguous_format).view(-1, heads, dim)
-    if to is None or not _mtpk.rows16(to, 0, 1):
+        raise ValueError(f"out must be {list(x.shape)} {x.dtype} on {device}")
+    src, dst = _tokens(x), _tokens(out)
+    if src is None:
+        src = x.clone(memory_format=torch.contiguous_format).view(-1, heads, dim)
+    if dst is None:
         raise ValueError("out's rows must lie on 16 bytes and its leading dims at one stride")
-    if flat.numel() == 0:
+    tokens = src.shape[0]
+    if tokens == 0 or heads == 0:
         return out
-    pos = positions.reshape(-1).contiguous()
-    xs, os_ = _mtpk.strides(flat, 0, 1), _mtpk.strides(to, 0, 1)
+    pos = positions if positions.is_contiguous() else positions.contiguous()
+    xs, os_ = _Two(*src.stride()[:2]), _Two(*dst.stride()[:2])
     with _mtpk.on(device):
-        _mtpk.check(_mtpk.lib().mtpk_rotate(
-            flat.data_ptr(), dtype, ctypes.addressof(xs), flat.shape[0], heads, dim, _mtpk.ptr(w),
-            _mtpk.float_code(w.dtype) if w is not None else 0, eps, pos.data_ptr(), rates.data_ptr(), rot,
-            int(interleaved), magnitude, to.data_ptr(), ctypes.addressof(os_), _mtpk.stream_of(device),
-        ), "mtpk_rotate")  # fmt: skip
+        status = _mtpk.lib().mtpk_rotate(
+            src.data_ptr(), dtype, ctypes.addressof(xs), tokens, heads, dim, None if w is None else w.data_ptr(),
+            w_dtype, eps, pos.data_ptr(), rates.data_ptr(), rot, interleaved, magnitude, dst.data_ptr(),
+            ctypes.addressof(os_), _mtpk.stream_of(device))
+    if status:
+        _mtpk.check(status, "mtpk_rotate")
     return out
 
 
 def _tokens(x: torch.Tensor) -> torch.Tensor | None:
     """`[..., heads, dim]` as a `[tokens, heads, dim]` view, or None where the leading dims have no one
-    stride."""
-    heads, dim = x.shape[-2:]
-    try:
-        return x.view(-1, heads, dim) if x.numel() else x.reshape(-1, heads, dim)
-    except RuntimeError:
-        return None
+    stride or the rows do not lie on 16 bytes."""
+    if x.dim() != 3:
+        heads, dim = x.shape[-2:]
+        try:
+            x = x.view(-1, heads, dim) if x.numel() else x.reshape(0, heads, dim)
+        except RuntimeError:
+            return None
+    return x if _mtpk.rows16(x) else None
 
 
 def rotate_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rates: torch.Tensor, k_pool: torch.Tensor,
@@ -145,45 +149,48 @@ def rotate_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rates: to
     16 bytes are copied first). Rows of a lane must not share a pool row with another lane's."""
     device = _mtpk.require_device(q, k, v, rates, k_pool, v_pool, block_table, base_pos)
     if q.dim() != 4 or k.dim() != 4:
-        raise ValueError(f"q and k must be [B, t, heads, hd], got {tuple(q.shape)} and {tuple(k.shape)}")
+        raise ValueError(f"q and k must be [B, t, heads, hd], got {list(q.shape)} and {list(k.shape)}")
     b, t, heads, hd = q.shape
     kvh = k.shape[2]
     if k.shape != (b, t, kvh, hd) or v.shape != k.shape:
-        raise ValueError(f"k and v must be [{b}, {t}, kv_heads, {hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if not q.dtype == k.dtype == v.dtype == k_pool.dtype == v_pool.dtype == torch.bfloat16:
-        raise ValueError("q, k, v and the pools must be bf16")
+        raise ValueError(f"k and v must be [{b}, {t}, kv_heads, {hd}], got {list(k.shape)} and {list(v.shape)}")
+    if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
+        raise ValueError("q, k and v must be bf16")
     rot = _check_rates(rates, hd)
-    attention.check_cache(k_pool, v_pool, block_table, base_pos, b, hd)
-    if k_pool.shape[1] != kvh:
-        raise ValueError(f"the pools hold {k_pool.shape[1]} kv heads, k has {kvh}")
-    for w in (q_norm, k_norm):
-        _check_norm(w, hd, device)
-    if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
-        raise ValueError("q_norm and k_norm must be of one type")
-    norm = q_norm if q_norm is not None else k_norm
+    table, pos = attention.cache_operands(k_pool, v_pool, block_table, base_pos, b, kvh, hd)
+    norm_dtype = 0
+    if q_norm is not None:
+        q_norm, norm_dtype = _check_norm(q_norm, hd, device)
+    if k_norm is not None:
+        k_norm, k_dtype = _check_norm(k_norm, hd, device)
+        if q_norm is not None and k_dtype != norm_dtype:
+            raise ValueError("q_norm and k_norm must be of one type")
+        norm_dtype = k_dtype
     if positions is not None:
         if positions.shape != (b, t) or positions.dtype != torch.int64 or positions.device != device:
             raise ValueError(f"positions must be int64 [{b}, {t}] on {device}")
         positions = positions.contiguous()
-    kp, kb, ks = None, 0, 0
+    kb = ks = 0
     if keep is not None:
-        if keep.shape != (b, t) or keep.dtype not in (torch.bool, torch.uint8) or keep.device != device:
+        if keep.shape != (b, t) or keep.element_size() != 1 or keep.device != device:
             raise ValueError(f"keep must be bool [{b}, {t}] on {device}")
-        kp = keep.view(torch.uint8)
-        kb, ks = kp.stride()
-    table, pos = attention.table_and_base(block_table, base_pos)
-    out = torch.empty(b, t, heads, hd, dtype=torch.bfloat16, device=device)
+        kb, ks = keep.stride()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.numel() == 0:
         return out
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    st = [_mtpk.strides(x, 0, 2, 1) for x in (q, k, v, out)]
-    qs, ks_, vs, os_ = (ctypes.addressof(s) for s in st)
+    q, k, v = (x if _mtpk.rows16(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
+    st = []
+    for x in (q, k, v, out):
+        s = x.stride()
+        st.append(_Three(s[0], s[2], s[1]))
+    qs, ks_, vs, os_ = st
     with _mtpk.on(device):
-        _mtpk.check(_mtpk.lib().mtpk_rotate_to_cache(
-            q.data_ptr(), qs, k.data_ptr(), ks_, v.data_ptr(), vs, _mtpk.ptr(q_norm), _mtpk.ptr(k_norm),
-            _mtpk.float_code(norm.dtype) if norm is not None else 0, eps, rates.data_ptr(), rot, int(interleaved),
-            magnitude, k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], table.data_ptr(), table.shape[1],
-            pos.data_ptr(), _mtpk.ptr(positions), _mtpk.ptr(kp), kb, ks, b, t, heads, kvh, hd, out.data_ptr(),
-            os_, _mtpk.stream_of(device),
-        ), "mtpk_rotate_to_cache")  # fmt: skip
+        status = _mtpk.lib().mtpk_rotate_to_cache(
+            q.data_ptr(), ctypes.addressof(qs), k.data_ptr(), ctypes.addressof(ks_), v.data_ptr(), ctypes.addressof(vs),
+            _mtpk.ptr(q_norm), _mtpk.ptr(k_norm), norm_dtype, eps, rates.data_ptr(), rot, interleaved, magnitude,
+            k_pool.data_ptr(), v_pool.data_ptr(), k_pool.shape[0], table.data_ptr(), table.shape[1], pos.data_ptr(),
+            _mtpk.ptr(positions), _mtpk.ptr(keep), kb, ks, b, t, heads, kvh, hd, out.data_ptr(), ctypes.addressof(os_),
+            _mtpk.stream_of(device))
+    if status:
+        _mtpk.check(status, "mtpk_rotate_to_cache")
     return out
