@@ -20,11 +20,12 @@
 // rounded values, so that a row's weights sum to 1 as they are used. The output, with its gate, is
 // rounded once.
 //
-// Keys that a row does not see may hold anything: their scores are replaced, and where a tile that is
-// masked for some row holds a V value that is not finite, its second product takes a form of its own
-// (0 times infinity would be NaN in the rows that do not see it).
+// Keys that a row does not see may hold anything: their scores are replaced, and V is zeroed where no row of
+// the workgroup sees the key. A value that is not finite and that some of the rows sharing a tile see
+// makes all of them NaN (0 times infinity): such rows are found at the end and done again one by one.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mtpk_attention_common.h"
 #include "mtpk_host.h"
@@ -55,10 +56,9 @@ struct MaskedArgs {
   int window;  // 0: none
   int t, heads, kvh, lanes_kvh;
   int n_split, row_groups;
-  float scale2;                 // scale * log2(e)
   float cap2;                   // cap * log2(e), 0: none
   float cap_in;                 // 2 * log2(e) * scale / cap
-  float poly_max, c0, c1, c2, c3;  // cap2 * tanh(s scale / cap) as s (c0 + c1 s^2 + ..) up to |s| = poly_max
+  float poly_max, c0, c1, c2;   // cap2 * tanh(s scale / cap) as s (c0 + c1 s^2 + c2 s^4) up to |s| = poly_max; no cap: s c0
   float* part_o;
   float* part_ml;
 };
@@ -97,7 +97,6 @@ __device__ inline int wave_max_i(int v) {
 // What 32 rows (the two halves of a wave hold them twice) see together.
 struct RowSet {
   int lo_min, lo_max, hi_min, hi_max;
-  __device__ inline bool touches(int key0) const { return key0 < hi_max && key0 + kTileKeys > lo_min; }
   __device__ inline bool whole(int key0) const { return key0 >= lo_max && key0 + kTileKeys <= hi_min; }
 };
 // A row that sees nothing makes no key worth reading, and every tile that another row touches is masked.
@@ -157,7 +156,12 @@ __device__ inline void load_lds(rsrc_t r, uint8_t* to, uint32_t off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)to, 16, (int)off, 0, 0, 0);
 }
 
-// One row's running softmax: m in units of log2, l over the rounded P.
+// Scores are worked on in units of log2. What a row does not see becomes kUnseen, and a row's maximum starts
+// at kNoKey, far above it and far below any score in use: neither needs a comparison later on, and
+// both stay finite where the cap's line squares them. A row whose real scores all lie below, like one
+// with a value that is not finite in its sum, is done again by masked_row_slow.
+constexpr float kUnseen = -1e18f, kNoKey = -1e17f;
+
 struct RowSoft {
   float m, l;
 };
@@ -165,155 +169,106 @@ struct RowSoft {
 __device__ inline float cap_exact(const MaskedArgs& a, float s) {
   return fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.cap_in) + 1.f), -2.f * a.cap2, a.cap2);
 }
-__device__ inline float cap_poly(const MaskedArgs& a, float s) {
-  const float u = s * s;
-  return s * fmaf(u, fmaf(u, fmaf(u, a.c3, a.c2), a.c1), a.c0);
+
+// The larger of a value and of the other half's (lane ^ 32).
+__device__ inline float halves_max(float v) {
+  const uint32_t u = f32_bits(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(bits_f32(r[0]), bits_f32(r[1]));
 }
 
-// Scores of a tile (this lane's row, keys key0 + 16 (i / 8) + 8 h + i % 8) into P, and what O has to be
-// multiplied by first (1: nothing to do, for the whole wave).
+// One tile of scores on its way to P, in steps that the caller puts between its products: prepare, then
+// exponents [first, first + n) in any pieces.
 template <bool CAP, bool SLOPES>
-__device__ inline float tile_softmax(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole,
-                                     int key0, int h, RowSoft& r, bf16x8_t (&p)[2]) {
-  bool poly = true;
-  if (CAP) {
-    float am = fabsf(s[0]);
-#pragma unroll
-    for (int i = 1; i < 16; ++i) am = fmaxf(am, fabsf(s[i]));
-    poly = __ballot(!(am <= a.poly_max)) == 0ull;
+struct TileSoftmax {
+  float c0, c1, c2, ms;  // exponent of a score s: s (c0 + c1 s^2 + c2 s^4) - ms (without a cap: s c0 - ms)
+
+  __device__ inline float line(float s) const {
+    if (!CAP) return s * c0;
+    const float u = s * s;
+    return s * fmaf(u, fmaf(u, c2, c1), c0);
   }
-  const bool direct = !SLOPES && whole && poly;  // exponents straight from the scores
-  float tm;
-  if (direct) {
-    tm = s[0];
+
+  // Scores to where `line` makes exponents of them, and the row's new maximum. Returns what its sums are
+  // multiplied by, 1 for the whole wave in most tiles.
+  __device__ inline float prepare(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
+                                  int h, RowSoft& r) {
+    c0 = a.c0;
+    c1 = a.c1;
+    c2 = a.c2;
+    bool bent = false;  // some score past the cap's straight part
+    if (CAP) {
+      float am = fabsf(s[0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) tm = fmaxf(tm, s[i]);
-    tm = CAP ? cap_poly(a, tm) : tm * a.scale2;
-  } else {
-    if (CAP && !poly) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = cap_exact(a, s[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = CAP ? cap_poly(a, s[i]) : s[i] * a.scale2;
+      for (int i = 1; i < 16; ++i) am = fmaxf(am, fabsf(s[i]));
+      bent = __ballot(!(am <= a.poly_max)) != 0ull;
     }
-    if (SLOPES) {
-      const float away = (float)(row.pos - key0 - 8 * h);
+    if (SLOPES || !whole || bent) {  // uniform over the wave: in full here, and the line is the identity
+      if (CAP && bent) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = fmaf(fabsf(away - (float)(16 * (i >> 3) + (i & 7))), -slope2, s[i]);
-    }
-    if (!whole) {
-      const int lo = row.lo - key0 - 8 * h, n = row.hi - row.lo;  // seen: 0 <= i - lo < n, in one comparison
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[i] = (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)max(n, 0) ? s[i] : -INFINITY;
-    }
-    tm = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) tm = fmaxf(tm, s[i]);
-  }
-  tm = fmaxf(tm, __shfl_xor(tm, 32, kWave));
-  const float mn = fmaxf(r.m, tm);
-  float alpha = 1.f;
-  if (__ballot(mn > r.m) != 0ull) {  // uniform over the wave
-    alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.m - mn);
-    r.m = mn;
-    r.l *= alpha;
-  }
-  const float ms = r.m == -INFINITY ? 0.f : r.m;  // a row with no key so far: every e below is 0
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float x;
-    if (direct) {
-      if (CAP) {
-        const float u = s[i] * s[i];
-        x = fmaf(s[i], fmaf(u, fmaf(u, fmaf(u, a.c3, a.c2), a.c1), a.c0), -ms);
+        for (int i = 0; i < 16; ++i) s[i] = cap_exact(a, s[i]);
       } else {
-        x = fmaf(s[i], a.scale2, -ms);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = line(s[i]);
       }
-    } else {
-      x = s[i] - ms;
-    }
-    p[i >> 3][i & 7] = (__bf16)__builtin_amdgcn_exp2f(x);
-  }
-  const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
-  float part[2] = {0.f, 0.f};
+      if (SLOPES) {
+        const float away = (float)(row.pos - key0 - 8 * h);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    part[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i >> 2][2 * (i & 3)], p[i >> 2][2 * (i & 3) + 1]}, one,
-                                                  part[i & 1], false);
-  r.l += part[0] + part[1];
-  return alpha;
-}
-
-// Whether a tile of V^T in LDS holds a value that is not finite (each wave looks at the whole tile).
-template <int HD>
-__device__ inline bool tile_not_finite(const uint8_t* v, uint32_t vat) {
-  using G = TileGeom<HD>;
-  uint32_t bad = 0;
-#pragma unroll 2
-  for (int i = 0; i < G::kS; ++i) {
-    const u32x4_t w = lds16(v + vat + (i % G::kT) * 1024 + (i / G::kT) * G::kHalf);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f807f80u) + 0x00800080u;  // carries into bits 15, 31
-  }
-  return __ballot((bad & 0x80008000u) != 0u) != 0ull;
-}
-
-// V values with zeros where they are not finite: what the second product of such a tile takes.
-__device__ inline u32x4_t finite_only(u32x4_t w) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t lo = (w[e] & 0x7f80u) == 0x7f80u ? 0u : 0x0000ffffu;
-    const uint32_t hi = (w[e] & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u;
-    w[e] &= lo | hi;
-  }
-  return w;
-}
-
-// And what is not finite, into the sums of the rows that see it: two products, of ones in its places with
-// ones for the keys that a row sees, say where infinities of either sign (NaN: of both) belong.
-template <int HD>
-__device__ inline void add_not_finite(f32x16_t (&o)[HD / 32], const uint8_t* v, uint32_t vat, const RowKeys& row, int key0,
-                                      int h) {
-  using G = TileGeom<HD>;
-  bf16x8_t seen[2];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int key = key0 + 16 * (i >> 3) + 8 * h + (i & 7);
-    seen[i >> 3][i & 7] = (__bf16)(key >= row.lo && key < row.hi ? 1.f : 0.f);
-  }
-#pragma unroll
-  for (int dt = 0; dt < G::kT; ++dt)
-#pragma unroll
-    for (int sign = 0; sign < 2; ++sign) {
-      f32x16_t n;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) n[i] = 0.f;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        u32x4_t w = lds16(v + vat + dt * 1024 + x * G::kHalf);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t ones = 0;
-#pragma unroll
-          for (int y = 0; y < 32; y += 16) {
-            const uint32_t b = w[e] >> y & 0xffffu;
-            ones |= ((b & 0x7fffu) > 0x7f80u || b == (sign ? 0xff80u : 0x7f80u) ? 0x3f80u : 0u) << y;
-          }
-          w[e] = ones;
-        }
-        n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(w), seen[x], n, 0, 0, 0);
+        for (int i = 0; i < 16; ++i) s[i] = fmaf(fabsf(away - (float)(16 * (i >> 3) + (i & 7))), -slope2, s[i]);
       }
+      if (!whole) {
+        const int lo = row.lo - key0 - 8 * h, n = max(row.hi - row.lo, 0);  // seen: 0 <= i - lo < n, in one comparison
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[dt][i] += n[i] > 0.f ? (sign ? -INFINITY : INFINITY) : 0.f;
-      ring_fence();  // the rare path: few of its registers at a time
+        for (int i = 0; i < 16; ++i)
+          s[i] = (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)n ? s[i] : kUnseen;
+      }
+      c0 = 1.f;
+      c1 = c2 = 0.f;
     }
+    float tm = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) tm = fmaxf(tm, s[i]);
+    ms = fmaxf(r.m, halves_max(line(tm)));  // the line rises with the score
+    const float alpha = __builtin_amdgcn_exp2f(r.m - ms);
+    r.m = ms;
+    r.l *= alpha;
+    return alpha;
+  }
+
+  template <int FIRST, int N>
+  __device__ inline void exponents(const f32x16_t& s, bf16x8_t (&p)[2], RowSoft& r) const {
+    const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+    for (int i = FIRST; i < FIRST + N; i += 2) {
+      bf16x2_t e;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float x = s[i + j];
+        const float u = x * x;
+        e[j] = (__bf16)__builtin_amdgcn_exp2f(CAP ? fmaf(x, fmaf(u, fmaf(u, c2, c1), c0), -ms) : fmaf(x, c0, -ms));
+      }
+      p[i >> 3][i & 7] = e[0];
+      p[i >> 3][(i & 7) + 1] = e[1];
+      r.l = __builtin_amdgcn_fdot2_f32_bf16(e, one, r.l, false);  // the sum of what the product uses
+    }
+  }
+};
+
+// Steps of a loop as constants.
+template <int N, typename F, int I = 0>
+__device__ inline void static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, F, I + 1>(static_cast<F&&>(f));
+  }
 }
 
-// A row's sum is NaN where it saw keys and all of them at minus infinity, 0 where it saw none.
-__device__ inline float row_sum(float m, float l, bool seen) { return seen && m == -INFINITY ? __builtin_nanf("") : l; }
-__device__ inline bool row_sees(const RowKeys& row, int k0, int k1) { return max(row.lo, k0) < min(row.hi, k1); }
+// What a wave wrote to LDS, before its other lanes read it.
+__device__ inline void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_wave_barrier();
+}
 
 __device__ inline float row_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
@@ -339,15 +294,90 @@ __device__ inline void store_out8(const MaskedArgs& a, int b, int hq, int st, in
   }
 }
 
+// One row by one wave, key by key in fp32 straight from memory: for the rows whose result above is not
+// finite (a value or score that is not, seen by this row or by another one that shares its tiles), or
+// whose scores all lie below kNoKey. What the row does not see is not read.
+template <int HD>
+__device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, int lane) {
+  constexpr int NV = HD / kWave;
+  const RowKeys row = masked_row(a, b, step);
+  const int kh = hq / (a.heads / a.kvh);
+  const uint16_t* const q = a.q + a.qr.at(b, hq, step);
+  const int32_t* const trow = a.table + (int64_t)b * a.table_stride;
+  const float slope2 = a.slopes ? a.slopes[hq] * kLog2e : 0.f;
+  float acc[NV], odd[NV], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < NV; ++e) acc[e] = odd[e] = 0.f;
+#pragma unroll 1
+  for (int key0 = row.lo; key0 < row.hi; key0 += kWave) {
+    const int key = key0 + lane;
+    const bool live = key < row.hi;
+    const int id = live ? trow[key / kAttnBlock] : -1;
+    const bool held = id >= 0 && (int64_t)(id + 1) * kAttnBlock <= a.pool_rows;  // else the block reads as zeros
+    float s = 0.f;
+    if (held) {
+      const uint16_t* const k = a.k_pool + (((int64_t)id * kAttnBlock + key % kAttnBlock) * a.kvh + kh) * HD;
+#pragma unroll 1
+      for (int d = 0; d < HD; d += 8) {
+        float x[8], y[8];
+        load8(q, MTPK_BF16, d, x);
+        load8(k, MTPK_BF16, d, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+      }
+    }
+    s = a.cap2 > 0.f ? cap_exact(a, s) : s * a.c0;
+    s = live ? fmaf(fabsf((float)(row.pos - key)), -slope2, s) : -INFINITY;
+    const float mn = fmaxf(m, wave_max(s)), ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn), p = live ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
+    m = mn;
+    l = l * alpha + wave_sum(p);
+#pragma unroll
+    for (int e = 0; e < NV; ++e) acc[e] *= alpha;
+#pragma unroll 1
+    for (int j = 0; j < kWave && key0 + j < row.hi; ++j) {
+      const float pj = __shfl(p, j, kWave);
+      const int blk = __shfl(held ? id : -1, j, kWave);
+      if (blk < 0) continue;  // uniform
+      const uint16_t* const v = a.v_pool + (((int64_t)blk * a.kvh + kh) * HD + NV * lane) * kAttnBlock + (key0 + j) % kAttnBlock;
+#pragma unroll
+      for (int e = 0; e < NV; ++e) {
+        const float x = bf16_to_f32(v[e * kAttnBlock]);
+        if (fabsf(x) < INFINITY)
+          acc[e] = fmaf(pj, x, acc[e]);
+        else
+          odd[e] += x;
+      }
+    }
+  }
+  const float inv = row.hi <= row.lo ? 0.f : 1.f / l;  // keys all at minus infinity: 0 / 0
+  uint16_t* const to = a.out + a.orow.at(b, hq, step) + NV * lane;
+  const uint16_t* const gate = a.gate ? a.gate + a.gr.at(b, hq, step) + NV * lane : nullptr;
+#pragma unroll
+  for (int e = 0; e < NV; ++e) {
+    const float y = acc[e] * inv + odd[e];
+    to[e] = f32_to_bf16(gate ? y * sigmoid_of(gate[e]) : y);
+  }
+}
+
 // ---------------------------------------------------------------- many rows
 //
-// W waves of 32 rows to a workgroup, tiles shared by its waves, one tile ahead in two buffers with one
-// barrier per tile: prompts, and verify rows of more than one wave.
+// W waves of 32 rows to a workgroup, which share stages of NT tiles, one stage ahead in two buffers with
+// one barrier per stage: prompts, and verify rows of more than one wave. With two tiles a stage (heads up to
+// 128) the second tile's first product runs between the first one's exponents, and the first one's second
+// product between the second one's; with one (heads of 256, whose sums fill the registers) the exponents of
+// the tile's second block run between the products of its first.
 template <int HD, int W, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   using G = TileGeom<HD>;
-  constexpr int kRows = 32 * W;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[4 * G::kTile];  // two buffers of (K, V)
+  constexpr int NT = HD == 256 ? 1 : 2, kRows = 32 * W;
+  constexpr int RD = HD == 256 ? 2 : 4;  // products that an operand is read ahead
+  constexpr int QL = HD == 256 ? 3 : 0;  // pieces of Q that stay in LDS, where the registers hold no more
+  constexpr int kStageKeys = NT * kTileKeys, kBuffer = NT * 2 * G::kTile;  // a buffer: K tiles, then V tiles
+  constexpr int kLoadsAll = 2 * NT * G::kLoads, kMine = kLoadsAll / W;     // 1 KB loads of a stage and tensor
+  constexpr int kBlocks = kMine >= G::kLoads ? kMine / G::kLoads : 1;      // blocks that a wave takes part in
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kBuffer];
+  __shared__ __attribute__((aligned(16))) uint8_t q_smem[QL ? W * QL * 1024 : 16];
   __shared__ int wg_lo[W], wg_hi[W];
   const int group = a.heads / a.kvh, R = group * a.t;
   const int rg = a.row_groups - 1 - (int)blockIdx.x / a.lanes_kvh;  // the last rows, which see most, first
@@ -356,8 +386,15 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   const int h = lane >> 5, c = lane & 31;
   const int r = min(kRows * rg + 32 * wave + c, R - 1);  // rows past R repeat the last one
   const int step = r / group, hq = kh * group + r % group;
-  const RowKeys row = masked_row(a, b, step);
-  const RowSet set = row_set(row);
+  bf16x8_t q[G::kS - QL];
+  u32x4_t qd[G::kS];
+  {
+    const uint16_t* const qrow = a.q + a.qr.at(b, hq, step) + 8 * h;
+#pragma unroll
+    for (int s = 0; s < G::kS; ++s) qd[s] = ld16(qrow + 16 * s);
+  }
+  RowKeys row = masked_row(a, b, step);
+  RowSet set = row_set(row);
   if (lane == 0) {
     wg_lo[wave] = set.lo_min;
     wg_hi[wave] = set.hi_max;
@@ -375,43 +412,47 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   masked_split(lo, hi, a.n_split, sp, tile0, tiles);
   tile0 = uniform(tile0);
   tiles = uniform(tiles);
+  const int end = (tile0 + tiles) * kTileKeys;
+  // This split's keys alone: its last stage may reach into the next one's.
+  row.hi = min(row.hi, end);
+  set.hi_min = min(set.hi_min, end);
+  set.hi_max = min(set.hi_max, end);
+  hi = min(hi, end);
 
-  bf16x8_t q[G::kS];
-  {
-    const uint16_t* const qrow = a.q + a.qr.at(b, hq, step) + 8 * h;
-    u32x4_t d[G::kS];
-#pragma unroll
-    for (int s = 0; s < G::kS; ++s) d[s] = ld16(qrow + 16 * s);
-#pragma unroll
-    for (int s = 0; s < G::kS; ++s) {
-      asm volatile("" : "+v"(d[s]));  // landed before the loop: its waits count the tiles' loads alone
-      q[s] = as_bf16x8(d[s]);
-    }
-  }
   const float slope2 = SLOPES ? a.slopes[hq] * kLog2e : 0.f;
   const int32_t* const trow = a.table + (int64_t)b * a.table_stride;
   const int last_block = (int)min(a.table_stride, (int64_t)INT32_MAX) - 1;
 
-  // This wave loads one of the tile's two blocks, or half of one, K and V.
-  constexpr int kShare = W / 2, kMine = G::kLoads / kShare;
-  const int half = wave / kShare;
-  uint32_t koff[kMine];
+  // This wave's loads of a stage are [wave kMine, (wave + 1) kMine) of its kLoadsAll, block by block.
+  const int g0 = wave * kMine, block0 = g0 / G::kLoads, j0 = g0 % G::kLoads;
+  const uint32_t kpiece = (uint32_t)(((lane / G::kP * a.kvh + kh) * HD + (lane % G::kP) * 8) * 2);
+  const uint32_t kstep = (uint32_t)(64 / G::kP * a.kvh * HD * 2);  // bytes between loads of a block
+  const uint32_t voff = v_offset<HD>(lane, kh) + (uint32_t)(j0 * 1024);
+  const int klane = lane / G::kP;
+  int ids[kBlocks];
+  auto blocks = [&](int key0) {
 #pragma unroll
-  for (int j = 0; j < kMine; ++j) koff[j] = k_offset<HD>(lane, a.kvh, kh, half, (wave % kShare) * kMine + j);
-  const uint32_t voff = v_offset<HD>(lane, kh) + (uint32_t)((wave % kShare) * kMine * 1024);
-  auto block = [&](int key0) { return sload(trow, min(key0 / kAttnBlock + half, last_block)); };
-  auto stage = [&](int buf, int key0, int blk) {
-    const int at = key0 + kAttnBlock * half;
-    const BlockSource<HD> src(a, uniform(blk), at < hi && at + kAttnBlock > lo);
-    uint8_t* const to = smem + buf + wave * (kMine * 1024);
+    for (int x = 0; x < kBlocks; ++x) ids[x] = sload(trow, min(key0 / kAttnBlock + block0 + x, last_block));
+  };
+  auto stage = [&](int buf, int key0) {
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      load_lds(src.k, to + j * 1024, koff[j]);
-      load_lds(src.v, to + G::kTile + j * 1024, voff + 1024u * j);
+    for (int x = 0; x < kBlocks; ++x) {
+      const int at = key0 + kAttnBlock * (block0 + x);
+      const BlockSource<HD> src(a, uniform(ids[x]), at < hi && at + kAttnBlock > lo);
+      constexpr int kPer = kMine < G::kLoads ? kMine : G::kLoads;
+      uint8_t* const to = smem + buf + (block0 + x) * G::kHalf + j0 * 1024;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        // piece ^ flip of the key's row: the flip of 16 (block % 2) + key, of which the lane has its own share
+        const int key = 16 * ((block0 + x) & 1) + (j0 + j) * (64 / G::kP) + klane;
+        const uint32_t off = (kpiece ^ (uint32_t)(prompt_flip(prompt_swap(key)) * 16)) + (uint32_t)(j0 + j) * kstep;
+        load_lds(src.k, to + j * 1024, off);
+        load_lds(src.v, to + NT * G::kTile + j * 1024, voff + 1024u * j);
+      }
     }
   };
 
-  RowSoft soft{-INFINITY, 0.f};
+  RowSoft soft{kNoKey, 0.f};
   f32x16_t o[G::kT];
 #pragma unroll
   for (int dt = 0; dt < G::kT; ++dt)
@@ -420,75 +461,126 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   // this lane's K pieces: 2 s + h of tile row c, whose place is that of piece h with bits of s flipped
   const uint32_t kat = (uint32_t)(prompt_swap(c) * HD * 2 + ((h ^ prompt_flip(c)) * 16));
   // and its V^T keys: 8 h .. 8 h + 7 of each block, channel 32 dt + c
-  const uint32_t vat = (uint32_t)(c * 32 + (h ^ (c >> 2 & 1)) * 16);
+  const uint32_t vat = (uint32_t)(NT * G::kTile + c * 32 + (h ^ (c >> 2 & 1)) * 16);
 
-  int key0 = tile0 * kTileKeys, buf = 0, next = 0;
+  uint8_t* const q_mine = q_smem + (wave * QL * 64 + lane) * 16;
+  int key0 = tile0 * kTileKeys, buf = 0;
   if (tiles > 0) {
-    stage(0, key0, block(key0));
-    next = block(key0 + kTileKeys);
+    blocks(key0);
+    stage(0, key0);
+    blocks(key0 + kStageKeys);
   }
-  for (int n = 0; n < tiles; ++n, key0 += kTileKeys, buf ^= 2 * G::kTile) {
+#pragma unroll
+  for (int s = 0; s < G::kS; ++s) {
+    asm volatile("" : "+v"(qd[s]));  // landed before the loop: its waits count the tiles' loads alone
+    if (s >= QL)
+      q[s - QL] = as_bf16x8(qd[s]);
+    else
+      lds16_store(q_mine + s * 1024, qd[s]);
+  }
+  for (; key0 < end; key0 += kStageKeys, buf ^= kBuffer) {
     ring_fence();
-    vmcnt_wait<0>();  // this tile, issued a tile ago
+    vmcnt_wait<0>();  // this stage, issued a stage ago
     __builtin_amdgcn_s_barrier();
     ring_fence();
-    if (n + 1 < tiles) {
-      stage(buf ^ (2 * G::kTile), key0 + kTileKeys, next);  // last read a tile ago, before the barrier
-      next = block(key0 + 2 * kTileKeys);
+    if (key0 + kStageKeys < end) {
+      stage(buf ^ kBuffer, key0 + kStageKeys);  // last read a stage ago, before the barrier
+      blocks(key0 + 2 * kStageKeys);
     }
     ring_fence();
-    if (!set.touches(key0)) continue;
-    const bool whole = set.whole(key0);
-    const uint8_t* const kt = smem + buf;
-    const uint8_t* const vt = smem + buf + G::kTile;
-    f32x16_t s;
+    if (key0 < lo || key0 + kStageKeys > hi) {  // uniform: V at keys that no row of the workgroup sees becomes zeros
+      for (int i = tid; i < 2 * NT * HD; i += W * kWave) {
+        const int first = key0 + kAttnBlock * (i / HD), d = i % HD;
+        for (int e = 0; e < kAttnBlock; ++e)
+          if (first + e < lo || first + e >= hi)
+            *reinterpret_cast<uint16_t*>(smem + buf + NT * G::kTile + i * 32 + (((e >> 3) ^ (d >> 2 & 1)) * 16) + (e & 7) * 2) = 0;
+      }
+      __syncthreads();
+    }
+    if (key0 >= set.hi_max || key0 + kStageKeys <= set.lo_min) continue;  // uniform over the wave
+    const uint8_t* const at = smem + buf;
+    u32x4_t f[RD];
+    auto kfrag = [&](int n, int i) { return lds16(at + n * G::kTile + (kat ^ (32u * (i & 3))) + 128 * (i >> 2)); };
+    auto vfrag = [&](int n, int i) { return lds16(at + n * G::kTile + vat + (i % G::kT) * 1024 + (i / G::kT) * G::kHalf); };
+    auto rescale = [&](float alpha) {
+      if (__ballot(alpha != 1.f) != 0ull) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
-    // operands come from LDS four products ahead, fenced
-    u32x4_t f[4];
-    auto kfrag = [&](int i) { return lds16(kt + (kat ^ (32u * (i & 3))) + 128 * (i >> 2)); };
-    auto vfrag = [&](int i) { return lds16(vt + vat + (i % G::kT) * 1024 + (i / G::kT) * G::kHalf); };
+        for (int dt = 0; dt < G::kT; ++dt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = kfrag(i);
+          for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+      }
+    };
+    f32x16_t s[NT];
+    bf16x8_t p[NT][2];
+    TileSoftmax<CAP, SLOPES> soft_tile;
+    // operands come from LDS RD products ahead, fenced
+#pragma unroll
+    for (int i = 0; i < RD; ++i) f[i] = kfrag(0, i);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
     ring_fence();
 #pragma unroll
     for (int i = 0; i < G::kS; ++i) {
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i & 3]), q[i], s, 0, 0, 0);
-      f[i & 3] = i + 4 < G::kS ? kfrag(i + 4) : vfrag(i + 4 - G::kS);
+      const bf16x8_t qi = i < QL ? as_bf16x8(lds16(q_mine + i * 1024)) : q[i < QL ? 0 : i - QL];
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), qi, s[0], 0, 0, 0);
+      f[i % RD] = i + RD < G::kS ? kfrag(0, i + RD) : NT == 2 ? kfrag(NT - 1, i + RD - G::kS) : vfrag(0, i + RD - G::kS);
       ring_fence();
     }
-    bf16x8_t p[2];
-    const float alpha = tile_softmax<CAP, SLOPES>(a, s, row, slope2, whole, key0, h, soft, p);
-    if (__ballot(alpha != 1.f) != 0ull) {
-#pragma unroll
-      for (int dt = 0; dt < G::kT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
-    }
-    const bool bad = !whole && tile_not_finite<HD>(vt, vat);  // uniform over the wave
-    if (bad) {
-      add_not_finite<HD>(o, vt, vat, row, key0, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = vfrag(i);  // again: not held over the rare path
-    }
-#pragma unroll
-    for (int i = 0; i < G::kS; ++i) {
-      if (bad) f[i & 3] = finite_only(f[i & 3]);
-      o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i & 3]), p[i / G::kT], o[i % G::kT], 0, 0, 0);
-      if (i + 4 < G::kS) f[i & 3] = vfrag(i + 4);
+    if constexpr (NT == 2) {
+      constexpr int kE = 16 / G::kS;  // exponents beside each product
+      const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
+      rescale(alpha);
       ring_fence();
+      static_for<G::kS>([&](auto i) {
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), q[i], s[1], 0, 0, 0);
+        f[i % RD] = i + RD < G::kS ? kfrag(1, i + RD) : vfrag(0, i + RD - G::kS);
+        soft_tile.template exponents<i * kE, kE>(s[0], p[0], soft);
+        ring_fence();
+      });
+      // The second tile's maximum raises the first one's sums too, so its product goes into O as it is.
+      const float beta = soft_tile.prepare(a, s[1], row, slope2, set.whole(key0 + kTileKeys), key0 + kTileKeys, h, soft);
+      ring_fence();
+      static_for<G::kS>([&](auto i) {
+        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), p[0][i / G::kT], o[i % G::kT], 0, 0, 0);
+        f[i % RD] = i + RD < G::kS ? vfrag(0, i + RD) : vfrag(1, i + RD - G::kS);
+        soft_tile.template exponents<i * kE, kE>(s[1], p[1], soft);
+        ring_fence();
+      });
+      rescale(beta);
+      ring_fence();
+#pragma unroll
+      for (int i = 0; i < G::kS; ++i) {
+        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), p[1][i / G::kT], o[i % G::kT], 0, 0, 0);
+        if (i + RD < G::kS) f[i % RD] = vfrag(1, i + RD);
+        ring_fence();
+      }
+    } else {
+      const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
+      soft_tile.template exponents<0, 8>(s[0], p[0], soft);
+      rescale(alpha);
+      ring_fence();
+      static_for<G::kS>([&](auto i) {
+        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), p[0][i / G::kT], o[i % G::kT], 0, 0, 0);
+        if (i + RD < G::kS) f[i % RD] = vfrag(0, i + RD);
+        if (i < 4) soft_tile.template exponents<(i < 4 ? 8 + 2 * i : 8), 2>(s[0], p[0], soft);
+        ring_fence();
+      });
     }
   }
-  const float l = row_sum(soft.m, soft.l + __shfl_xor(soft.l, 32, kWave),
-                          row_sees(row, tile0 * kTileKeys, (tile0 + tiles) * kTileKeys));
+  const float l = soft.l + __shfl_xor(soft.l, 32, kWave);
+  const bool real = kRows * rg + 32 * wave + c < R;
   // o[dt][4 i + e] is channel 32 dt + 8 i + 4 h + e of the row
   if (a.n_split == 1) {
     // Through LDS, half of the channels at a time, into whole rows: a lane holds 8 bytes here and there
     // of its row. A wave's 32 rows are its own; 16-byte pieces (4 floats) at [row][piece ^ row].
     constexpr int kRow = HD * 2, kPieces = HD / 8, kFlip = kPieces - 1;  // bytes and pieces of half a row
+    static_assert(W * 32 * kRow <= 2 * kBuffer, "half of the rows' floats fit the buffers");
     const float inv = row_inverse(l);
+    float odd = 0.f;  // NaN where some value of the row is not finite
     uint8_t* const mine = smem + wave * (32 * kRow);
-    __syncthreads();  // the last tile's reads are done
+    __syncthreads();  // the last stage's reads are done
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
 #pragma unroll
@@ -497,10 +589,12 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
         for (int i = 0; i < 4; ++i) {
           const int piece = 8 * dt + 2 * i + h;
           const f32x16_t& x = o[part * (G::kT / 2) + dt];
-          *reinterpret_cast<f32x4_t*>(mine + c * kRow + ((piece ^ c) & kFlip) * 16) =
-              f32x4_t{x[4 * i] * inv, x[4 * i + 1] * inv, x[4 * i + 2] * inv, x[4 * i + 3] * inv};
+          const f32x4_t y = {x[4 * i] * inv, x[4 * i + 1] * inv, x[4 * i + 2] * inv, x[4 * i + 3] * inv};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = fmaf(y[e], 0.f, odd);
+          *reinterpret_cast<f32x4_t*>(mine + c * kRow + ((piece ^ c) & kFlip) * 16) = y;
         }
-      __syncthreads();
+      wave_lds_fence();
 #pragma unroll 2
       for (int i = lane; i < 32 * kPieces / 2; i += kWave) {
         const int rl = i / (kPieces / 2), pc = i % (kPieces / 2), ro = kRows * rg + 32 * wave + rl;
@@ -514,10 +608,17 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
         }
         store_out8(a, b, kh * group + ro % group, ro / group, part * (HD / 2) + 8 * pc, y);
       }
-      __syncthreads();
+      wave_lds_fence();
+    }
+    uint64_t again = __ballot(real && (odd != 0.f || (l == 0.f && row.hi > row.lo)));
+    again = (again | again >> 32) & 0xffffffffull;
+    while (again != 0ull) {
+      const int rl = uniform(__builtin_ctzll(again)), ro = kRows * rg + 32 * wave + rl;
+      again &= again - 1ull;
+      masked_row_slow<HD>(a, b, kh * group + ro % group, ro / group, lane);
     }
   } else {
-    if (kRows * rg + 32 * wave + c >= R) return;
+    if (!real) return;
     const int64_t pr = (((int64_t)bkh * a.row_groups + rg) * a.n_split + sp) * kRows + 32 * wave + c;
     float* const po = a.part_o + pr * HD;
     if (tiles > 0) {
@@ -529,7 +630,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
               f32x4_t{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
     }
     if (h == 0) {
-      a.part_ml[pr * 2] = soft.m;
+      a.part_ml[pr * 2] = tiles > 0 ? soft.m : -INFINITY;  // of a split without tiles nothing else is written
       a.part_ml[pr * 2 + 1] = l;
     }
   }
@@ -545,29 +646,23 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
   using G = TileGeom<HD>;
   __shared__ __attribute__((aligned(16))) uint8_t smem[4][2 * G::kTile];  // a wave's K and V tile
   __shared__ float ml[4][32][2];
-  __shared__ bool sees[32];
+  __shared__ int again[32];
   const int group = a.heads / a.kvh, R = group * a.t;
   const int bkh = blockIdx.x, kh = bkh % a.kvh, b = bkh / a.kvh, sp = blockIdx.y;
   const int tid = threadIdx.x, wave = uniform(tid / kWave), lane = tid & (kWave - 1);
   const int h = lane >> 5, c = lane & 31;
   const int r = min(c, R - 1);  // rows past R repeat the last one
   const int step = r / group, hq = kh * group + r % group;
+  u32x4_t qd[G::kS];
+  {
+    const uint16_t* const qrow = a.q + a.qr.at(b, hq, step) + 8 * h;
+#pragma unroll
+    for (int s = 0; s < G::kS; ++s) qd[s] = ld16(qrow + 16 * s);
+  }
   const RowKeys row = masked_row(a, b, step);
   const RowSet set = row_set(row);
   const int lo = set.lo_min, hi = set.hi_max;
   const float slope2 = SLOPES ? a.slopes[hq] * kLog2e : 0.f;
-  bf16x8_t q[G::kS];
-  {
-    const uint16_t* const qrow = a.q + a.qr.at(b, hq, step) + 8 * h;
-    u32x4_t d[G::kS];
-#pragma unroll
-    for (int s = 0; s < G::kS; ++s) d[s] = ld16(qrow + 16 * s);
-#pragma unroll
-    for (int s = 0; s < G::kS; ++s) {
-      asm volatile("" : "+v"(d[s]));  // landed before the loop: its waits count the tiles' loads alone
-      q[s] = as_bf16x8(d[s]);
-    }
-  }
   int tile0, tiles;
   masked_split(lo, hi, a.n_split, sp, tile0, tiles);
   tile0 = uniform(tile0);
@@ -601,7 +696,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     }
   };
 
-  RowSoft soft{-INFINITY, 0.f};
+  RowSoft soft{kNoKey, 0.f};
   f32x16_t o[G::kT];
 #pragma unroll
   for (int dt = 0; dt < G::kT; ++dt)
@@ -620,6 +715,12 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     stage_v(key0, b0, b1);
     b0 = block(key0 + kStep, 0);
     b1 = block(key0 + kStep, 1);
+  }
+  bf16x8_t q[G::kS];
+#pragma unroll
+  for (int s = 0; s < G::kS; ++s) {
+    asm volatile("" : "+v"(qd[s]));  // landed before the loop: its waits count the tiles' loads alone
+    q[s] = as_bf16x8(qd[s]);
   }
   for (; key0 < end; key0 += kStep) {
     const bool more = key0 + kStep < end;
@@ -643,9 +744,10 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     }
     if (more) stage_k(key0 + kStep, b0, b1);  // every read of K went into a product above
     ring_fence();
-    const bool whole = set.whole(key0);
+    TileSoftmax<CAP, SLOPES> soft_tile;
     bf16x8_t p[2];
-    const float alpha = tile_softmax<CAP, SLOPES>(a, s, row, slope2, whole, key0, h, soft, p);
+    const float alpha = soft_tile.prepare(a, s, row, slope2, set.whole(key0), key0, h, soft);
+    soft_tile.template exponents<0, 16>(s, p, soft);
     if (__ballot(alpha != 1.f) != 0ull) {
 #pragma unroll
       for (int dt = 0; dt < G::kT; ++dt)
@@ -658,14 +760,20 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     else
       vmcnt_wait<0>();
     ring_fence();
-    const bool bad = !whole && tile_not_finite<HD>(vt, vat);  // uniform over the wave
-    if (bad) add_not_finite<HD>(o, vt, vat, row, key0, h);
+    if (key0 < lo || key0 + kTileKeys > hi) {  // uniform: V at keys that no row sees becomes zeros
+      for (int i = lane; i < 2 * HD; i += kWave) {
+        const int first = key0 + kAttnBlock * (i / HD), d = i % HD;
+        for (int e = 0; e < kAttnBlock; ++e)
+          if (first + e < lo || first + e >= hi)
+            *reinterpret_cast<uint16_t*>(vt + i * 32 + (((e >> 3) ^ (d >> 2 & 1)) * 16) + (e & 7) * 2) = 0;
+      }
+      wave_lds_fence();
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = vfrag(i);
     ring_fence();
 #pragma unroll
     for (int i = 0; i < G::kS; ++i) {
-      if (bad) f[i & 3] = finite_only(f[i & 3]);
       o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i & 3]), p[i / G::kT], o[i % G::kT], 0, 0, 0);
       if (i + 4 < G::kS) f[i & 3] = vfrag(i + 4);
       ring_fence();
@@ -692,23 +800,21 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
   if (h == 0) {
     ml[wave][c][0] = soft.m;
     ml[wave][c][1] = l;
-    if (wave == 0) sees[c] = row_sees(row, tile0 * kTileKeys, end);
+    if (wave == 0) again[c] = 0;
   }
   __syncthreads();
   for (int i = tid; i < 32 * G::kP; i += 256) {
     const int rl = i / G::kP, pc = i % G::kP;
     if (rl >= R) break;
-    float m = -INFINITY, sum = 0.f, y[8];
+    float m = kNoKey, sum = 0.f, y[8];
 #pragma unroll
     for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][rl][0]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float mw = ml[w][rl][0], lw = ml[w][rl][1];
-      const float wt = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
-      sum += lw * (mw == -INFINITY ? 1.f : wt);  // a sum without a maximum is 0 or NaN
-      if (mw == -INFINITY) continue;             // such a wave holds nothing
+      const float wt = __builtin_amdgcn_exp2f(ml[w][rl][0] - m);
+      sum = fmaf(ml[w][rl][1], wt, sum);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(smem[w] + rl * kRow + (((2 * pc + e) ^ rl) & kFlip) * 16);
@@ -716,12 +822,16 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
         for (int g = 0; g < 4; ++g) y[4 * e + g] = fmaf(x[g], wt, y[4 * e + g]);
       }
     }
-    sum = row_sum(m, sum, sees[rl]);
     if (a.n_split == 1) {
       const float inv = row_inverse(sum);
+      float odd = sum == 0.f ? 1.f : 0.f;  // not 0: the row is done again, below
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] *= inv;
+      for (int e = 0; e < 8; ++e) {
+        y[e] *= inv;
+        odd = fmaf(y[e], 0.f, odd);
+      }
       store_out8(a, b, kh * group + rl % group, rl / group, 8 * pc, y);
+      if (odd != 0.f) again[rl] = 1;
     } else {
       const int64_t pr = ((int64_t)bkh * a.n_split + sp) * 32 + rl;
       float* const po = a.part_o + pr * HD + 8 * pc;
@@ -732,6 +842,11 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
         a.part_ml[pr * 2 + 1] = sum;
       }
     }
+  }
+  if (a.n_split > 1) return;
+  __syncthreads();
+  for (int rl = wave; rl < min(R, 32); rl += 4) {
+    if (uniform(again[rl]) != 0) masked_row_slow<HD>(a, b, kh * group + rl % group, rl / group, lane);
   }
 }
 
@@ -753,9 +868,8 @@ __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, in
   const bool live = lane < a.n_split;
   const float m = live ? a.part_ml[(base + (int64_t)lane * group_rows) * 2] : -INFINITY;
   const float l = live ? a.part_ml[(base + (int64_t)lane * group_rows) * 2 + 1] : 0.f;
-  const float mx = wave_max(m);
-  const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-  const float inv = row_inverse(wave_sum(m == -INFINITY ? l : l * w));
+  const float mx = fmaxf(wave_max(m), kNoKey);
+  const float w = __builtin_amdgcn_exp2f(m - mx), sum = wave_sum(l * w), inv = row_inverse(sum);
   const uint64_t held = __ballot(m != -INFINITY);  // the other splits hold nothing: their rows are not written
   vec_t acc = {};
   for (int s0 = wave; s0 < a.n_split; s0 += 4 * W) {
@@ -780,11 +894,14 @@ __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, in
   }
   uint16_t* const orow = a.out + a.orow.at(b, hq, st) + NV * lane;
   const uint16_t* const grow = a.gate ? a.gate + a.gr.at(b, hq, st) + NV * lane : nullptr;
+  float odd = sum == 0.f ? 1.f : 0.f;
 #pragma unroll
   for (int e = 0; e < NV; ++e) {
     const float y = acc[e] * inv;
+    odd = fmaf(y, 0.f, odd);
     orow[e] = f32_to_bf16(grow ? y * sigmoid_of(grow[e]) : y);
   }
+  if (__ballot(odd != 0.f) != 0ull) masked_row_slow<HD>(a, b, hq, st, lane);
 }
 
 namespace {
@@ -912,18 +1029,17 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
   a.lanes_kvh = (int)(batch * kv_heads);
   a.n_split = n_split;
   a.row_groups = (int)masked_row_groups(rows);
-  a.scale2 = scale * kLog2e;
+  a.c0 = scale * kLog2e;
   if (softcap > 0.f) {
-    // cap * tanh(u) log2(e), u = s * scale / cap: u - u^3 / 3 + 2 u^5 / 15 - 17 u^7 / 315 is within 3e-7 of
-    // tanh(u), relative, up to |u| = 0.23
+    // tanh(u) / u on |u| <= 1/4 as the quadratic in u^2 that interpolates it at Chebyshev's points: within
+    // 4e-7, where Taylor's of the same length is off by 1.3e-5
     const double k = (double)scale / softcap, c = (double)softcap * 1.4426950408889634;
     a.cap2 = (float)c;
     a.cap_in = (float)(2. * 1.4426950408889634 * k);
-    a.poly_max = (float)(0.23 / k);
-    a.c0 = (float)(c * k);
-    a.c1 = (float)(-c * k * k * k / 3.);
-    a.c2 = (float)(c * k * k * k * k * k * 2. / 15.);
-    a.c3 = (float)(-c * k * k * k * k * k * k * k * 17. / 315.);
+    a.poly_max = (float)(0.25 / k);
+    a.c0 = (float)(c * k * 0.99999961);
+    a.c1 = (float)(c * k * k * k * -0.33321928);
+    a.c2 = (float)(c * k * k * k * k * k * 0.12841935);
   }
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o ? a.part_o + batch * kv_heads * a.row_groups * masked_group_rows(rows) * n_split * head_dim : nullptr;

@@ -144,10 +144,13 @@ def test_unseen_keys_may_hold_anything(dev, heads, kvh, hd, t, base, value) -> N
     k[unseen], v[unseen] = value, value
     k[:16], v[:16] = value, value
     assert torch.equal(run(dev, q, k, v, table, b0, hd**-0.5, first=first).double().cpu(), clean)
-    if t > 1:  # the last row's own key and value: no earlier row changes
+    if t > 1:  # the last row's own key and value: the earlier rows are done without them, as the oracle does them
+        want, spread = ref.paged_attention_masked(q[:, :-1], k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0), table, b0, hd**-0.5,
+                                                  first=first[:, :-1])
         k[rows[base[0] + t - 1]], v[rows[base[0] + t - 1]] = value, value
-        got = run(dev, q, k, v, table, b0, hd**-0.5, first=first).double().cpu()
-        assert torch.equal(got[:, :-1], clean[:, :-1])
+        got = run(dev, q, k, v, table, b0, hd**-0.5, first=first).double().cpu()[:, :-1]
+        worst = float(((got - want).abs() / bars(want, spread)).max())
+        assert worst <= 1.0  # and no NaN
 
 
 @pytest.mark.parametrize("heads,kvh,hd,t,base", [(8, 2, 64, 3, [40]), (32, 2, 256, 6, [100]), (16, 4, 128, 60, [7]), (8, 2, 128, 1, [5000])])
