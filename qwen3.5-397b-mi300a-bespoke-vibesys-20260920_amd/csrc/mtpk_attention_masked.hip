@@ -58,7 +58,9 @@ struct MaskedArgs {
   int n_split, row_groups;
   float cap2;                   // cap * log2(e), 0: none
   float cap_in;                 // 2 * log2(e) * scale / cap
-  float poly_max, c0, c1, c2;   // cap2 * tanh(s scale / cap) as s (c0 + c1 s^2 + c2 s^4) up to |s| = poly_max; no cap: s c0
+  // cap2 * tanh(s scale / cap) as s (c0 + c1 s^2) up to |s| = cubic_max, s (d0 + d1 s^2 + d2 s^4) up to
+  // quintic_max; s c0 without a cap
+  float cubic_max, quintic_max, c0, c1, d0, d1, d2;
   float* part_o;
   float* part_ml;
 };
@@ -158,9 +160,11 @@ __device__ inline void load_lds(rsrc_t r, uint8_t* to, uint32_t off) {
 
 // Scores are worked on in units of log2. What a row does not see becomes kUnseen, and a row's maximum starts
 // at kNoKey, far above it and far below any score in use: neither needs a comparison later on, and
-// both stay finite where the cap's line squares them. A row whose real scores all lie below, like one
-// with a value that is not finite in its sum, is done again by masked_row_slow.
-constexpr float kUnseen = -1e18f, kNoKey = -1e17f;
+// both stay finite where the cap's line squares them. Capped scores up to 2^kCapMost need no maximum at all:
+// their exponentials and sums stay inside fp32's and bf16's range as they are, and so the largest part of
+// the work between the two products falls away. A row whose sum all the same comes out below kLeastSum (its
+// keys all far below, or none: 0), or that holds a value that is not finite, is done again by masked_row_slow.
+constexpr float kUnseen = -1e18f, kNoKey = -1e17f, kLeastSum = 0x1p-102f, kCapMost = 100.f;
 
 struct RowSoft {
   float m, l;
@@ -181,35 +185,34 @@ __device__ inline float halves_max(float v) {
 // exponents [first, first + n) in any pieces.
 template <bool CAP, bool SLOPES>
 struct TileSoftmax {
-  float c0, c1, c2, ms;  // exponent of a score s: s (c0 + c1 s^2 + c2 s^4) - ms (without a cap: s c0 - ms)
+  float c0, c1, ms;  // exponent of a score s: s (c0 + c1 s^2) with a cap, s c0 - ms without one
 
-  __device__ inline float line(float s) const {
-    if (!CAP) return s * c0;
-    const float u = s * s;
-    return s * fmaf(u, fmaf(u, c2, c1), c0);
-  }
-
-  // Scores to where `line` makes exponents of them, and the row's new maximum. Returns what its sums are
-  // multiplied by, 1 for the whole wave in most tiles.
+  // Scores to where `exponents` takes them from there, and without a cap the row's new maximum. Returns what the
+  // row's sums are multiplied by, 1 for the whole wave in most tiles.
   __device__ inline float prepare(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
                                   int h, RowSoft& r) {
     c0 = a.c0;
     c1 = a.c1;
-    c2 = a.c2;
-    bool bent = false;  // some score past the cap's straight part
+    float am = 0.f;  // the largest magnitude, where the cap is on
     if (CAP) {
-      float am = fabsf(s[0]);
+      am = fabsf(s[0]);
 #pragma unroll
       for (int i = 1; i < 16; ++i) am = fmaxf(am, fabsf(s[i]));
-      bent = __ballot(!(am <= a.poly_max)) != 0ull;
     }
-    if (SLOPES || !whole || bent) {  // uniform over the wave: in full here, and the line is the identity
-      if (CAP && bent) {
+    const bool bent = CAP ? __ballot(!(am <= a.cubic_max)) != 0ull : a.cap2 > 0.f;  // past the cap's cubic part
+    if (SLOPES || !whole || bent) {  // uniform over the wave: in full here, and the exponent is the score
+      if (!bent) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = cap_exact(a, s[i]);
+        for (int i = 0; i < 16; ++i) s[i] = CAP ? s[i] * fmaf(s[i] * s[i], c1, c0) : s[i] * c0;
+      } else if (CAP && __ballot(!(am <= a.quintic_max)) == 0ull) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float u = s[i] * s[i];
+          s[i] = s[i] * fmaf(u, fmaf(u, a.d2, a.d1), a.d0);
+        }
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = line(s[i]);
+        for (int i = 0; i < 16; ++i) s[i] = cap_exact(a, s[i]);
       }
       if (SLOPES) {
         const float away = (float)(row.pos - key0 - 8 * h);
@@ -223,12 +226,13 @@ struct TileSoftmax {
           s[i] = (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)n ? s[i] : kUnseen;
       }
       c0 = 1.f;
-      c1 = c2 = 0.f;
+      c1 = 0.f;
     }
+    if (CAP) return 1.f;
     float tm = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) tm = fmaxf(tm, s[i]);
-    ms = fmaxf(r.m, halves_max(line(tm)));  // the line rises with the score
+    ms = fmaxf(r.m, halves_max(tm * c0));
     const float alpha = __builtin_amdgcn_exp2f(r.m - ms);
     r.m = ms;
     r.l *= alpha;
@@ -244,8 +248,7 @@ struct TileSoftmax {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float x = s[i + j];
-        const float u = x * x;
-        e[j] = (__bf16)__builtin_amdgcn_exp2f(CAP ? fmaf(x, fmaf(u, fmaf(u, c2, c1), c0), -ms) : fmaf(x, c0, -ms));
+        e[j] = (__bf16)__builtin_amdgcn_exp2f(CAP ? x * fmaf(x * x, c1, c0) : fmaf(x, c0, -ms));
       }
       p[i >> 3][i & 7] = e[0];
       p[i >> 3][(i & 7) + 1] = e[1];
@@ -326,7 +329,7 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
         for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
       }
     }
-    s = a.cap2 > 0.f ? cap_exact(a, s) : s * a.c0;
+    s = a.cap2 > 0.f ? cap_exact(a, s) : s * a.c0;  // c0 without a cap: the scale
     s = live ? fmaf(fabsf((float)(row.pos - key)), -slope2, s) : -INFINITY;
     const float mn = fmaxf(m, wave_max(s)), ms = mn == -INFINITY ? 0.f : mn;
     const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn), p = live ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
@@ -452,7 +455,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     }
   };
 
-  RowSoft soft{kNoKey, 0.f};
+  RowSoft soft{CAP ? 0.f : kNoKey, 0.f};
   f32x16_t o[G::kT];
 #pragma unroll
   for (int dt = 0; dt < G::kT; ++dt)
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     if constexpr (NT == 2) {
       constexpr int kE = 16 / G::kS;  // exponents beside each product
       const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
-      rescale(alpha);
+      if (!CAP) rescale(alpha);
       ring_fence();
       static_for<G::kS>([&](auto i) {
         s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), q[i], s[1], 0, 0, 0);
@@ -548,7 +551,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
         soft_tile.template exponents<i * kE, kE>(s[1], p[1], soft);
         ring_fence();
       });
-      rescale(beta);
+      if (!CAP) rescale(beta);
       ring_fence();
 #pragma unroll
       for (int i = 0; i < G::kS; ++i) {
@@ -559,7 +562,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     } else {
       const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
       soft_tile.template exponents<0, 8>(s[0], p[0], soft);
-      rescale(alpha);
+      if (!CAP) rescale(alpha);
       ring_fence();
       static_for<G::kS>([&](auto i) {
         o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), p[0][i / G::kT], o[i % G::kT], 0, 0, 0);
@@ -610,7 +613,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       }
       wave_lds_fence();
     }
-    uint64_t again = __ballot(real && (odd != 0.f || (l == 0.f && row.hi > row.lo)));
+    uint64_t again = __ballot(real && (odd != 0.f || (l < kLeastSum && row.hi > row.lo)));
     again = (again | again >> 32) & 0xffffffffull;
     while (again != 0ull) {
       const int rl = uniform(__builtin_ctzll(again)), ro = kRows * rg + 32 * wave + rl;
@@ -696,7 +699,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     }
   };
 
-  RowSoft soft{kNoKey, 0.f};
+  RowSoft soft{CAP ? 0.f : kNoKey, 0.f};
   f32x16_t o[G::kT];
 #pragma unroll
   for (int dt = 0; dt < G::kT; ++dt)
@@ -748,7 +751,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     bf16x8_t p[2];
     const float alpha = soft_tile.prepare(a, s, row, slope2, set.whole(key0), key0, h, soft);
     soft_tile.template exponents<0, 16>(s, p, soft);
-    if (__ballot(alpha != 1.f) != 0ull) {
+    if (!CAP && __ballot(alpha != 1.f) != 0ull) {
 #pragma unroll
       for (int dt = 0; dt < G::kT; ++dt)
 #pragma unroll
@@ -824,7 +827,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     }
     if (a.n_split == 1) {
       const float inv = row_inverse(sum);
-      float odd = sum == 0.f ? 1.f : 0.f;  // not 0: the row is done again, below
+      float odd = sum < kLeastSum ? 1.f : 0.f;  // not 0: the row is done again, below
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         y[e] *= inv;
@@ -894,7 +897,7 @@ __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, in
   }
   uint16_t* const orow = a.out + a.orow.at(b, hq, st) + NV * lane;
   const uint16_t* const grow = a.gate ? a.gate + a.gr.at(b, hq, st) + NV * lane : nullptr;
-  float odd = sum == 0.f ? 1.f : 0.f;
+  float odd = sum < kLeastSum ? 1.f : 0.f;
 #pragma unroll
   for (int e = 0; e < NV; ++e) {
     const float y = acc[e] * inv;
@@ -942,7 +945,7 @@ int masked_launch(const MaskedArgs& a, int64_t batch, hipStream_t st) {
 
 template <int HD>
 int masked_flags(const MaskedArgs& a, int64_t batch, hipStream_t st) {
-  const bool cap = a.cap2 > 0.f;
+  const bool cap = a.cap2 > 0.f && a.cap2 <= kCapMost;  // a wider one: in full for every tile, with a maximum
   if (a.slopes) return cap ? masked_launch<HD, true, true>(a, batch, st) : masked_launch<HD, false, true>(a, batch, st);
   return cap ? masked_launch<HD, true, false>(a, batch, st) : masked_launch<HD, false, false>(a, batch, st);
 }
@@ -1031,15 +1034,20 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
   a.row_groups = (int)masked_row_groups(rows);
   a.c0 = scale * kLog2e;
   if (softcap > 0.f) {
-    // tanh(u) / u on |u| <= 1/4 as the quadratic in u^2 that interpolates it at Chebyshev's points: within
-    // 4e-7, where Taylor's of the same length is off by 1.3e-5
+    // tanh(u) / u by polynomials in u^2 of least relative error: 8.4e-6 on |u| <= 0.15, which is 9e-5 of an exponent
+    // at cap 50 (a rounded probability is off by up to 2^-8), and 4e-7 on |u| <= 0.25
     const double k = (double)scale / softcap, c = (double)softcap * 1.4426950408889634;
     a.cap2 = (float)c;
     a.cap_in = (float)(2. * 1.4426950408889634 * k);
-    a.poly_max = (float)(0.25 / k);
-    a.c0 = (float)(c * k * 0.99999961);
-    a.c1 = (float)(c * k * k * k * -0.33321928);
-    a.c2 = (float)(c * k * k * k * k * k * 0.12841935);
+    a.cubic_max = (float)(0.15 / k);
+    a.quintic_max = (float)(0.25 / k);
+    if (c <= kCapMost) {
+      a.c0 = (float)(c * k * 0.99999165);
+      a.c1 = (float)(c * k * k * k * -0.33035765);
+      a.d0 = (float)(c * k * 0.99999961);
+      a.d1 = (float)(c * k * k * k * -0.33321928);
+      a.d2 = (float)(c * k * k * k * k * k * 0.12841935);
+    }
   }
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o ? a.part_o + batch * kv_heads * a.row_groups * masked_group_rows(rows) * n_split * head_dim : nullptr;
