@@ -119,7 +119,7 @@ __device__ inline void masked_split(int lo, int hi, int n_split, int sp, int& ti
 }
 
 // Staging of one 16-row block's K or V into LDS by `loads` 1 KB loads: a lane's offsets are the same
-// for every block. K as [key][piece ^ prompt_flip(row of the key)], V as [channel][piece ^ (channel / 4 & 1)].
+// for every block. K as [key][piece ^ prompt_flip(row of the key)], V as [channel][piece ^ v_swap(channel)].
 template <int HD>
 struct TileGeom {
   static constexpr int kS = HD / 16, kT = HD / 32, kP = HD / 8;  // k steps, channel tiles, 16-byte pieces of a key
@@ -141,6 +141,10 @@ struct BlockSource {
   }
 };
 
+// V's channel d holds two pieces of a block in LDS, exchanged by bits 2 and 3 of d: by bit 2 alone, its reads had
+// twice the bank conflicts.
+__device__ inline int v_swap(int d) { return ((d >> 2) ^ (d >> 3)) & 1; }
+
 // Byte offset of K load j (of kLoads) of a block: 1 KB covers 64 / kP keys.
 template <int HD>
 __device__ inline uint32_t k_offset(int lane, int kvh, int kh, int half, int j) {
@@ -151,7 +155,7 @@ __device__ inline uint32_t k_offset(int lane, int kvh, int kh, int half, int j) 
 // V load 0; load j is 1 KB further on.
 template <int HD>
 __device__ inline uint32_t v_offset(int lane, int kh) {
-  return (uint32_t)(kh * HD * 32 + (lane >> 1) * 32 + (((lane & 1) ^ (lane >> 3 & 1)) * 16));
+  return (uint32_t)(kh * HD * 32 + (lane >> 1) * 32 + (((lane & 1) ^ v_swap(lane >> 1)) * 16));
 }
 
 __device__ inline void load_lds(rsrc_t r, uint8_t* to, uint32_t off) {
@@ -240,7 +244,7 @@ struct TileSoftmax {
   }
 
   template <int FIRST, int N>
-  __device__ inline void exponents(const f32x16_t& s, bf16x8_t (&p)[2], RowSoft& r) const {
+  __device__ inline void exponents(const f32x16_t& s, u32x4_t (&p)[2], RowSoft& r) const {
     const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
     for (int i = FIRST; i < FIRST + N; i += 2) {
@@ -250,8 +254,9 @@ struct TileSoftmax {
         const float x = s[i + j];
         e[j] = (__bf16)__builtin_amdgcn_exp2f(CAP ? x * fmaf(x * x, c1, c0) : fmaf(x, c0, -ms));
       }
-      p[i >> 3][i & 7] = e[0];
-      p[i >> 3][(i & 7) + 1] = e[1];
+      uint32_t w = __builtin_bit_cast(uint32_t, e);
+      asm volatile("" : "+v"(w));  // here, beside the products around it, and not where the second product is
+      p[i >> 3][i >> 1 & 3] = w;
       r.l = __builtin_amdgcn_fdot2_f32_bf16(e, one, r.l, false);  // the sum of what the product uses
     }
   }
@@ -281,11 +286,13 @@ __device__ inline float sigmoid_of(uint16_t g) {
 }
 
 // Eight values of an output row, gated, rounded once.
-__device__ inline void store_out8(const MaskedArgs& a, int b, int hq, int st, int d, const float* v) {
+__device__ inline u32x4_t gate8(const MaskedArgs& a, int b, int hq, int st, int d) {
+  return a.gate ? ld16(a.gate + a.gr.at(b, hq, st) + d) : zero16();
+}
+__device__ inline void store_out8(const MaskedArgs& a, int b, int hq, int st, int d, const float* v, u32x4_t g) {
   float y[8];
   uint16_t* const to = a.out + a.orow.at(b, hq, st) + d;
   if (a.gate) {
-    const u32x4_t g = ld16(a.gate + a.gr.at(b, hq, st) + d);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       y[2 * e] = v[2 * e] * sigmoid_of((uint16_t)(g[e] & 0xffffu));
@@ -376,7 +383,8 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   constexpr int NT = HD == 256 ? 1 : 2, kRows = 32 * W;
   constexpr int RD = HD == 256 ? 2 : 4;  // products that an operand is read ahead
   constexpr int QL = HD == 256 ? 3 : 0;  // pieces of Q that stay in LDS, where the registers hold no more
-  constexpr int kStageKeys = NT * kTileKeys, kBuffer = NT * 2 * G::kTile;  // a buffer: K tiles, then V tiles
+  constexpr int kStageKeys = NT * kTileKeys, kVAt = NT * G::kTile;  // a buffer: K tiles, then V tiles
+  constexpr int kBuffer = kVAt + NT * G::kTile;
   constexpr int kLoadsAll = 2 * NT * G::kLoads, kMine = kLoadsAll / W;     // 1 KB loads of a stage and tensor
   constexpr int kBlocks = kMine >= G::kLoads ? kMine / G::kLoads : 1;      // blocks that a wave takes part in
   __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kBuffer];
@@ -443,14 +451,16 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       const int at = key0 + kAttnBlock * (block0 + x);
       const BlockSource<HD> src(a, uniform(ids[x]), at < hi && at + kAttnBlock > lo);
       constexpr int kPer = kMine < G::kLoads ? kMine : G::kLoads;
-      uint8_t* const to = smem + buf + (block0 + x) * G::kHalf + j0 * 1024;
+      const int half = (block0 + x) & 1;
+      uint8_t* const kto = smem + buf + (block0 + x) / 2 * G::kTile;
+      uint8_t* const vto = smem + buf + kVAt + (block0 + x) * G::kHalf + j0 * 1024;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         // piece ^ flip of the key's row: the flip of 16 (block % 2) + key, of which the lane has its own share
-        const int key = 16 * ((block0 + x) & 1) + (j0 + j) * (64 / G::kP) + klane;
+        const int first = 16 * half + (j0 + j) * (64 / G::kP), key = first + klane;
         const uint32_t off = (kpiece ^ (uint32_t)(prompt_flip(prompt_swap(key)) * 16)) + (uint32_t)(j0 + j) * kstep;
-        load_lds(src.k, to + j * 1024, off);
-        load_lds(src.v, to + NT * G::kTile + j * 1024, voff + 1024u * j);
+        load_lds(src.k, kto + first * (HD * 2), off);
+        load_lds(src.v, vto + j * 1024, voff + 1024u * j);
       }
     }
   };
@@ -464,7 +474,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   // this lane's K pieces: 2 s + h of tile row c, whose place is that of piece h with bits of s flipped
   const uint32_t kat = (uint32_t)(prompt_swap(c) * HD * 2 + ((h ^ prompt_flip(c)) * 16));
   // and its V^T keys: 8 h .. 8 h + 7 of each block, channel 32 dt + c
-  const uint32_t vat = (uint32_t)(NT * G::kTile + c * 32 + (h ^ (c >> 2 & 1)) * 16);
+  const uint32_t vat = (uint32_t)(kVAt + c * 32 + (h ^ v_swap(c)) * 16);
 
   uint8_t* const q_mine = q_smem + (wave * QL * 64 + lane) * 16;
   int key0 = tile0 * kTileKeys, buf = 0;
@@ -496,7 +506,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
         const int first = key0 + kAttnBlock * (i / HD), d = i % HD;
         for (int e = 0; e < kAttnBlock; ++e)
           if (first + e < lo || first + e >= hi)
-            *reinterpret_cast<uint16_t*>(smem + buf + NT * G::kTile + i * 32 + (((e >> 3) ^ (d >> 2 & 1)) * 16) + (e & 7) * 2) = 0;
+            *reinterpret_cast<uint16_t*>(smem + buf + kVAt + i * 32 + (((e >> 3) ^ v_swap(d)) * 16) + (e & 7) * 2) = 0;
       }
       __syncthreads();
     }
@@ -514,7 +524,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       }
     };
     f32x16_t s[NT];
-    bf16x8_t p[NT][2];
+    u32x4_t p[NT][2];
     TileSoftmax<CAP, SLOPES> soft_tile;
     // operands come from LDS RD products ahead, fenced
 #pragma unroll
@@ -524,6 +534,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
     ring_fence();
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < G::kS; ++i) {
       const bf16x8_t qi = i < QL ? as_bf16x8(lds16(q_mine + i * 1024)) : q[i < QL ? 0 : i - QL];
@@ -531,6 +542,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       f[i % RD] = i + RD < G::kS ? kfrag(0, i + RD) : NT == 2 ? kfrag(NT - 1, i + RD - G::kS) : vfrag(0, i + RD - G::kS);
       ring_fence();
     }
+    __builtin_amdgcn_s_setprio(0);
     if constexpr (NT == 2) {
       constexpr int kE = 16 / G::kS;  // exponents beside each product
       const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
@@ -546,30 +558,34 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       const float beta = soft_tile.prepare(a, s[1], row, slope2, set.whole(key0 + kTileKeys), key0 + kTileKeys, h, soft);
       ring_fence();
       static_for<G::kS>([&](auto i) {
-        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), p[0][i / G::kT], o[i % G::kT], 0, 0, 0);
+        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[0][i / G::kT]), o[i % G::kT], 0, 0, 0);
         f[i % RD] = i + RD < G::kS ? vfrag(0, i + RD) : vfrag(1, i + RD - G::kS);
         soft_tile.template exponents<i * kE, kE>(s[1], p[1], soft);
         ring_fence();
       });
       if (!CAP) rescale(beta);
       ring_fence();
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < G::kS; ++i) {
-        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), p[1][i / G::kT], o[i % G::kT], 0, 0, 0);
+        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[1][i / G::kT]), o[i % G::kT], 0, 0, 0);
         if (i + RD < G::kS) f[i % RD] = vfrag(1, i + RD);
         ring_fence();
       }
+      __builtin_amdgcn_s_setprio(0);
     } else {
       const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
       soft_tile.template exponents<0, 8>(s[0], p[0], soft);
       if (!CAP) rescale(alpha);
       ring_fence();
+      __builtin_amdgcn_s_setprio(1);
       static_for<G::kS>([&](auto i) {
-        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), p[0][i / G::kT], o[i % G::kT], 0, 0, 0);
+        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[0][i / G::kT]), o[i % G::kT], 0, 0, 0);
         if (i + RD < G::kS) f[i % RD] = vfrag(0, i + RD);
         if (i < 4) soft_tile.template exponents<(i < 4 ? 8 + 2 * i : 8), 2>(s[0], p[0], soft);
         ring_fence();
       });
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   const float l = soft.l + __shfl_xor(soft.l, 32, kWave);
@@ -580,6 +596,14 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     // of its row. A wave's 32 rows are its own; 16-byte pieces (4 floats) at [row][piece ^ row].
     constexpr int kRow = HD * 2, kPieces = HD / 8, kFlip = kPieces - 1;  // bytes and pieces of half a row
     static_assert(W * 32 * kRow <= 2 * kBuffer, "half of the rows' floats fit the buffers");
+    constexpr int kEach = 32 * kPieces / 2 / kWave;  // pieces of 8 channels that a lane stores of a half
+    // the gates, all on their way before the first is used: one memory latency for the workgroup's last step
+    u32x4_t gates[2 * kEach];
+#pragma unroll
+    for (int i = 0; i < 2 * kEach; ++i) {
+      const int at = lane + kWave * (i % kEach), ro = min(kRows * rg + 32 * wave + at / (kPieces / 2), R - 1);
+      gates[i] = gate8(a, b, kh * group + ro % group, ro / group, i / kEach * (HD / 2) + 8 * (at % (kPieces / 2)));
+    }
     const float inv = row_inverse(l);
     float odd = 0.f;  // NaN where some value of the row is not finite
     uint8_t* const mine = smem + wave * (32 * kRow);
@@ -598,9 +622,9 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
           *reinterpret_cast<f32x4_t*>(mine + c * kRow + ((piece ^ c) & kFlip) * 16) = y;
         }
       wave_lds_fence();
-#pragma unroll 2
-      for (int i = lane; i < 32 * kPieces / 2; i += kWave) {
-        const int rl = i / (kPieces / 2), pc = i % (kPieces / 2), ro = kRows * rg + 32 * wave + rl;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int at = lane + kWave * i, rl = at / (kPieces / 2), pc = at % (kPieces / 2), ro = kRows * rg + 32 * wave + rl;
         if (ro >= R) continue;
         float y[8];
 #pragma unroll
@@ -609,7 +633,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) y[4 * e + g] = w[g];
         }
-        store_out8(a, b, kh * group + ro % group, ro / group, part * (HD / 2) + 8 * pc, y);
+        store_out8(a, b, kh * group + ro % group, ro / group, part * (HD / 2) + 8 * pc, y, gates[part * kEach + i]);
       }
       wave_lds_fence();
     }
@@ -706,7 +730,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   const uint32_t kat = (uint32_t)(prompt_swap(c) * HD * 2 + ((h ^ prompt_flip(c)) * 16));
-  const uint32_t vat = (uint32_t)(c * 32 + (h ^ (c >> 2 & 1)) * 16);
+  const uint32_t vat = (uint32_t)(c * 32 + (h ^ v_swap(c)) * 16);
   constexpr int kStep = 4 * kTileKeys;
   const int end = (tile0 + tiles) * kTileKeys;
   int key0 = (tile0 + wave) * kTileKeys;
@@ -748,7 +772,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     if (more) stage_k(key0 + kStep, b0, b1);  // every read of K went into a product above
     ring_fence();
     TileSoftmax<CAP, SLOPES> soft_tile;
-    bf16x8_t p[2];
+    u32x4_t p[2];
     const float alpha = soft_tile.prepare(a, s, row, slope2, set.whole(key0), key0, h, soft);
     soft_tile.template exponents<0, 16>(s, p, soft);
     if (!CAP && __ballot(alpha != 1.f) != 0ull) {
@@ -768,7 +792,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
         const int first = key0 + kAttnBlock * (i / HD), d = i % HD;
         for (int e = 0; e < kAttnBlock; ++e)
           if (first + e < lo || first + e >= hi)
-            *reinterpret_cast<uint16_t*>(vt + i * 32 + (((e >> 3) ^ (d >> 2 & 1)) * 16) + (e & 7) * 2) = 0;
+            *reinterpret_cast<uint16_t*>(vt + i * 32 + (((e >> 3) ^ v_swap(d)) * 16) + (e & 7) * 2) = 0;
       }
       wave_lds_fence();
     }
@@ -777,7 +801,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     ring_fence();
 #pragma unroll
     for (int i = 0; i < G::kS; ++i) {
-      o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i & 3]), p[i / G::kT], o[i % G::kT], 0, 0, 0);
+      o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i & 3]), as_bf16x8(p[i / G::kT]), o[i % G::kT], 0, 0, 0);
       if (i + 4 < G::kS) f[i & 3] = vfrag(i + 4);
       ring_fence();
     }
@@ -809,6 +833,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
   for (int i = tid; i < 32 * G::kP; i += 256) {
     const int rl = i / G::kP, pc = i % G::kP;
     if (rl >= R) break;
+    const u32x4_t gate = a.n_split == 1 ? gate8(a, b, kh * group + rl % group, rl / group, 8 * pc) : zero16();
     float m = kNoKey, sum = 0.f, y[8];
 #pragma unroll
     for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][rl][0]);
@@ -833,7 +858,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
         y[e] *= inv;
         odd = fmaf(y[e], 0.f, odd);
       }
-      store_out8(a, b, kh * group + rl % group, rl / group, 8 * pc, y);
+      store_out8(a, b, kh * group + rl % group, rl / group, 8 * pc, y, gate);
       if (odd != 0.f) again[rl] = 1;
     } else {
       const int64_t pr = ((int64_t)bkh * a.n_split + sp) * 32 + rl;
