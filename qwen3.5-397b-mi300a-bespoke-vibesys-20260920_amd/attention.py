@@ -300,13 +300,18 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
     take the torch spelling."""
     if not pools:
         raise ValueError("copy_blocks takes at least one pool")
-    device, n_blocks = pools[0].device, 0
+    first = pools[0]
+    device, where = first.device, first.get_device()
+    n_blocks = first.size(0) // (1 if first.dim() == 4 else block)
+    rows = n_blocks * block
     for p in pools:
-        n = p.shape[0] if p.dim() == 4 else p.shape[0] // block if p.dim() == 3 and p.shape[0] % block == 0 else 0
-        n_blocks = n_blocks or n
-        if n != n_blocks or p.numel() == 0 or not p.is_contiguous() or p.device != device:
+        n = p.size(0) if p.dim() in (3, 4) else -1
+        if n != (n_blocks if p.dim() == 4 else rows) or n == 0 or p.get_device() != where or not p.is_contiguous():
             raise ValueError("pools must be contiguous K caches [rows, kv_heads, hd] and V caches [blocks, kv_heads, hd, "
                              f"{block}] of one number of blocks on one device, got {tuple(p.shape)} on {p.device}")
+    sizes = [p.nbytes // n_blocks for p in pools]
+    if 0 in sizes:
+        raise ValueError("pools must not be empty")
     checked = not (torch.is_tensor(src) and src.is_cuda)
     if checked != (not (torch.is_tensor(dst) and dst.is_cuda)):
         raise ValueError("src and dst must both be on the host or both on the device")
@@ -333,13 +338,12 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
         src, dst = torch.stack((src, dst)).pin_memory().to(device, non_blocking=True).unbind(0)
     elif src.device != device or dst.device != device:
         raise ValueError(f"src and dst must be on {device}")
-    sizes = [p.numel() // n_blocks * p.element_size() for p in pools]
-    if any(s % 16 or p.data_ptr() % 16 for s, p in zip(sizes, pools)):
-        raise ValueError("blocks must be multiples of 16 bytes and lie on 16 bytes")
+    at = [p.data_ptr() for p in pools]
     src, dst = src.contiguous(), dst.contiguous()
-    ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
-    bytes_ = (ctypes.c_int64 * len(pools))(*sizes)
+    ptrs, bytes_ = (ctypes.c_void_p * len(at))(*at), (ctypes.c_int64 * len(at))(*sizes)
     with _mtpk.on(device):
-        _mtpk.check(_mtpk.lib().mtpk_copy_blocks(
-            ctypes.addressof(ptrs), ctypes.addressof(bytes_), len(pools), n_blocks, src.data_ptr(), dst.data_ptr(),
-            _mtpk.index_code(src.dtype), pairs, _mtpk.stream_of(device)), "mtpk_copy_blocks")  # fmt: skip
+        status = _mtpk.lib().mtpk_copy_blocks(
+            ctypes.addressof(ptrs), ctypes.addressof(bytes_), len(at), n_blocks, src.data_ptr(), dst.data_ptr(),
+            _mtpk.index_code(src.dtype), pairs, _mtpk.stream_of(device))
+    if status:
+        _mtpk.check(status, "mtpk_copy_blocks (blocks of a multiple of 16 bytes, pools on 16 bytes)")
