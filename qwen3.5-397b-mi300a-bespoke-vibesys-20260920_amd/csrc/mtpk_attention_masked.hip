@@ -119,12 +119,13 @@ __device__ inline void masked_split(int lo, int hi, int n_split, int sp, int& ti
 }
 
 // Staging of one 16-row block's K or V into LDS by `loads` 1 KB loads: a lane's offsets are the same
-// for every block. K as [key][piece ^ prompt_flip(row of the key)], V as [channel][piece ^ v_swap(channel)].
+// for every block. K as [key][piece ^ k_flip(row of the key)], V as [channel][piece ^ v_swap(channel)].
 template <int HD>
 struct TileGeom {
   static constexpr int kS = HD / 16, kT = HD / 32, kP = HD / 8;  // k steps, channel tiles, 16-byte pieces of a key
   static constexpr int kHalf = kAttnBlock * HD * 2;              // bytes of a block's K (or V) of one kv head
-  static constexpr int kTile = 2 * kHalf;
+  static constexpr int kTile = 2 * kHalf;                        // of a tile's V
+  static constexpr int kKTile = kTile + (HD == 256 ? 1024 : 0);   // of a tile's K, with its rows' shifts
   static constexpr int kLoads = kHalf / 1024;  // 1 KB loads of a block
 };
 
@@ -141,8 +142,21 @@ struct BlockSource {
   }
 };
 
-// V's channel d holds two pieces of a block in LDS, exchanged by bits 2 and 3 of d: by bit 2 alone, its reads had
-// twice the bank conflicts.
+// The places of a tile's 16-byte pieces in LDS. One cycle of a read serves 16 lanes with 256 bytes: lanes 0-3, 8-11,
+// 20-23 and 28-31, then 4-7, 12-15, 16-19 and 24-27, and so on in the upper half (the counted bank conflicts are those
+// that this makes). So what a lane's c is to choose among 16 places is bits 0 to 3 of c. K's row for c
+// (prompt_swap(c)) has its pieces flipped by three of them. Heads of 64, two rows to 256 bytes, have bit 0 in the row
+// itself; heads of 256 have their rows shifted by 128 bytes for every 4, which is bit 3 (4095 packed rows: 94.0
+// without, 93.2 us with it); heads of 128 are left with K's conflicts of two, as the same shift, though it ends
+// them, made 8000 rows slower (318 to 322 us). V's channel d holds two pieces of a block, exchanged by bits 2 and 3 of d.
+template <int HD>
+__device__ inline int k_flip(int c) {
+  return HD == 64 ? c >> 1 & 7 : ((c & 3) << 1) | (c >> 2 & 1);
+}
+template <int HD>
+__device__ inline constexpr int k_row(int r) {
+  return r * HD * 2 + (HD == 256 ? (r >> 2) * 128 : 0);
+}
 __device__ inline int v_swap(int d) { return ((d >> 2) ^ (d >> 3)) & 1; }
 
 // Byte offset of K load j (of kLoads) of a block: 1 KB covers 64 / kP keys.
@@ -150,12 +164,29 @@ template <int HD>
 __device__ inline uint32_t k_offset(int lane, int kvh, int kh, int half, int j) {
   using G = TileGeom<HD>;
   const int key = j * (64 / G::kP) + lane / G::kP;
-  return (uint32_t)(((key * kvh + kh) * HD + ((lane % G::kP) ^ prompt_flip(prompt_swap(16 * half + key))) * 8) * 2);
+  return (uint32_t)(((key * kvh + kh) * HD + ((lane % G::kP) ^ k_flip<HD>(prompt_swap(16 * half + key))) * 8) * 2);
 }
 // V load 0; load j is 1 KB further on.
 template <int HD>
 __device__ inline uint32_t v_offset(int lane, int kh) {
   return (uint32_t)(kh * HD * 32 + (lane >> 1) * 32 + (((lane & 1) ^ v_swap(lane >> 1)) * 16));
+}
+
+// V of `blocks` blocks in LDS, the first one's keys from key0 on: zeros at the keys outside [lo, hi), 16 bytes (8 keys
+// of a channel) a thread.
+template <int HD>
+__device__ inline void zero_unseen(uint8_t* v, int blocks, int key0, int lo, int hi, int tid, int threads) {
+  for (int i = tid; i < blocks * HD * 2; i += threads) {
+    const int d = i / 2 % HD, first = key0 + kAttnBlock * (i / (2 * HD)) + 8 * ((i & 1) ^ v_swap(d));
+    if (first >= lo && first + 8 <= hi) continue;
+    u32x4_t w = lds16(v + i * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int key = first + 2 * e;
+      w[e] &= (key >= lo && key < hi ? 0x0000ffffu : 0u) | (key + 1 >= lo && key + 1 < hi ? 0xffff0000u : 0u);
+    }
+    lds16_store(v + i * 16, w);
+  }
 }
 
 __device__ inline void load_lds(rsrc_t r, uint8_t* to, uint32_t off) {
@@ -383,7 +414,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   constexpr int NT = HD == 256 ? 1 : 2, kRows = 32 * W;
   constexpr int RD = HD == 256 ? 2 : 4;  // products that an operand is read ahead
   constexpr int QL = HD == 256 ? 3 : 0;  // pieces of Q that stay in LDS, where the registers hold no more
-  constexpr int kStageKeys = NT * kTileKeys, kVAt = NT * G::kTile;  // a buffer: K tiles, then V tiles
+  constexpr int kStageKeys = NT * kTileKeys, kVAt = NT * G::kKTile;  // a buffer: K tiles, then V tiles
   constexpr int kBuffer = kVAt + NT * G::kTile;
   constexpr int kLoadsAll = 2 * NT * G::kLoads, kMine = kLoadsAll / W;     // 1 KB loads of a stage and tensor
   constexpr int kBlocks = kMine >= G::kLoads ? kMine / G::kLoads : 1;      // blocks that a wave takes part in
@@ -452,14 +483,14 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       const BlockSource<HD> src(a, uniform(ids[x]), at < hi && at + kAttnBlock > lo);
       constexpr int kPer = kMine < G::kLoads ? kMine : G::kLoads;
       const int half = (block0 + x) & 1;
-      uint8_t* const kto = smem + buf + (block0 + x) / 2 * G::kTile;
+      uint8_t* const kto = smem + buf + (block0 + x) / 2 * G::kKTile;
       uint8_t* const vto = smem + buf + kVAt + (block0 + x) * G::kHalf + j0 * 1024;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         // piece ^ flip of the key's row: the flip of 16 (block % 2) + key, of which the lane has its own share
         const int first = 16 * half + (j0 + j) * (64 / G::kP), key = first + klane;
-        const uint32_t off = (kpiece ^ (uint32_t)(prompt_flip(prompt_swap(key)) * 16)) + (uint32_t)(j0 + j) * kstep;
-        load_lds(src.k, kto + first * (HD * 2), off);
+        const uint32_t off = (kpiece ^ (uint32_t)(k_flip<HD>(prompt_swap(key)) * 16)) + (uint32_t)(j0 + j) * kstep;
+        load_lds(src.k, kto + k_row<HD>(first), off);
         load_lds(src.v, vto + j * 1024, voff + 1024u * j);
       }
     }
@@ -472,7 +503,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   // this lane's K pieces: 2 s + h of tile row c, whose place is that of piece h with bits of s flipped
-  const uint32_t kat = (uint32_t)(prompt_swap(c) * HD * 2 + ((h ^ prompt_flip(c)) * 16));
+  const uint32_t kat = (uint32_t)(k_row<HD>(prompt_swap(c)) + ((h ^ k_flip<HD>(c)) * 16));
   // and its V^T keys: 8 h .. 8 h + 7 of each block, channel 32 dt + c
   const uint32_t vat = (uint32_t)(kVAt + c * 32 + (h ^ v_swap(c)) * 16);
 
@@ -491,29 +522,24 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     else
       lds16_store(q_mine + s * 1024, qd[s]);
   }
-  for (; key0 < end; key0 += kStageKeys, buf ^= kBuffer) {
+  for (; key0 < end; key0 += kStageKeys, buf = kBuffer - buf) {
     ring_fence();
     vmcnt_wait<0>();  // this stage, issued a stage ago
     __builtin_amdgcn_s_barrier();
     ring_fence();
     if (key0 + kStageKeys < end) {
-      stage(buf ^ kBuffer, key0 + kStageKeys);  // last read a stage ago, before the barrier
+      stage(kBuffer - buf, key0 + kStageKeys);  // last read a stage ago, before the barrier
       blocks(key0 + 2 * kStageKeys);
     }
     ring_fence();
     if (key0 < lo || key0 + kStageKeys > hi) {  // uniform: V at keys that no row of the workgroup sees becomes zeros
-      for (int i = tid; i < 2 * NT * HD; i += W * kWave) {
-        const int first = key0 + kAttnBlock * (i / HD), d = i % HD;
-        for (int e = 0; e < kAttnBlock; ++e)
-          if (first + e < lo || first + e >= hi)
-            *reinterpret_cast<uint16_t*>(smem + buf + kVAt + i * 32 + (((e >> 3) ^ v_swap(d)) * 16) + (e & 7) * 2) = 0;
-      }
+      zero_unseen<HD>(smem + buf + kVAt, 2 * NT, key0, lo, hi, tid, W * kWave);
       __syncthreads();
     }
     if (key0 >= set.hi_max || key0 + kStageKeys <= set.lo_min) continue;  // uniform over the wave
     const uint8_t* const at = smem + buf;
     u32x4_t f[RD];
-    auto kfrag = [&](int n, int i) { return lds16(at + n * G::kTile + (kat ^ (32u * (i & 3))) + 128 * (i >> 2)); };
+    auto kfrag = [&](int n, int i) { return lds16(at + n * G::kKTile + (kat ^ (32u * (i & 3))) + 128 * (i >> 2)); };
     auto vfrag = [&](int n, int i) { return lds16(at + n * G::kTile + vat + (i % G::kT) * 1024 + (i / G::kT) * G::kHalf); };
     auto rescale = [&](float alpha) {
       if (__ballot(alpha != 1.f) != 0ull) {
@@ -671,7 +697,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
 template <int HD, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
   using G = TileGeom<HD>;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[4][2 * G::kTile];  // a wave's K and V tile
+  __shared__ __attribute__((aligned(16))) uint8_t smem[4][G::kKTile + G::kTile];  // a wave's K and V tile
   __shared__ float ml[4][32][2];
   __shared__ int again[32];
   const int group = a.heads / a.kvh, R = group * a.t;
@@ -697,7 +723,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
   const int32_t* const trow = a.table + (int64_t)b * a.table_stride;
   const int last_block = (int)min(a.table_stride, (int64_t)INT32_MAX) - 1;
   uint8_t* const kt = smem[wave];
-  uint8_t* const vt = kt + G::kTile;
+  uint8_t* const vt = kt + G::kKTile;
   uint32_t koff[2][G::kLoads];
 #pragma unroll
   for (int x = 0; x < 2; ++x)
@@ -711,7 +737,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     for (int x = 0; x < 2; ++x) {
       const BlockSource<HD> src(a, uniform(x ? b1 : b0), wanted(key0, x));
 #pragma unroll
-      for (int j = 0; j < G::kLoads; ++j) load_lds(src.k, kt + x * G::kHalf + j * 1024, koff[x][j]);
+      for (int j = 0; j < G::kLoads; ++j) load_lds(src.k, kt + k_row<HD>(16 * x + j * (64 / G::kP)), koff[x][j]);
     }
   };
   auto stage_v = [&](int key0, int b0, int b1) {
@@ -729,7 +755,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
   for (int dt = 0; dt < G::kT; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-  const uint32_t kat = (uint32_t)(prompt_swap(c) * HD * 2 + ((h ^ prompt_flip(c)) * 16));
+  const uint32_t kat = (uint32_t)(k_row<HD>(prompt_swap(c)) + ((h ^ k_flip<HD>(c)) * 16));
   const uint32_t vat = (uint32_t)(c * 32 + (h ^ v_swap(c)) * 16);
   constexpr int kStep = 4 * kTileKeys;
   const int end = (tile0 + tiles) * kTileKeys;
@@ -788,12 +814,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
       vmcnt_wait<0>();
     ring_fence();
     if (key0 < lo || key0 + kTileKeys > hi) {  // uniform: V at keys that no row sees becomes zeros
-      for (int i = lane; i < 2 * HD; i += kWave) {
-        const int first = key0 + kAttnBlock * (i / HD), d = i % HD;
-        for (int e = 0; e < kAttnBlock; ++e)
-          if (first + e < lo || first + e >= hi)
-            *reinterpret_cast<uint16_t*>(vt + i * 32 + (((e >> 3) ^ v_swap(d)) * 16) + (e & 7) * 2) = 0;
-      }
+      zero_unseen<HD>(vt, 2, key0, lo, hi, lane, kWave);
       wave_lds_fence();
     }
 #pragma unroll
