@@ -6,7 +6,6 @@ missing or does not load, every device entry point raises: there is no silent fa
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from ctypes import c_int, c_int64, c_void_p
@@ -297,6 +296,38 @@ def lib() -> ctypes.CDLL:
     return handle
 
 
+_native = None
+_NATIVE_ENTRIES = ("mtpk_status_string", "mtpk_rotate", "mtpk_rotate_to_cache", "mtpk_attention_masked_splits",
+                   "mtpk_attention_masked_workspace_bytes", "mtpk_paged_attention_masked", "mtpk_copy_blocks")
+
+
+def native():
+    """The C++ calls on torch tensors (`_mtpk_torch.so`, csrc/mtpk_torch.cpp), bound to the loaded library;
+    raises `RuntimeError` if they are not built or do not load."""
+    global _native
+    if _native is None:
+        handle = lib()
+        try:
+            import _mtpk_torch
+        except ImportError as exc:
+            raise RuntimeError(f"_mtpk_torch.so is not built or does not load ({exc}); run `python __graft_entry__.py "
+                               "build` (or build_lib.py) first") from exc
+        if _mtpk_torch.abi_version != ABI_VERSION:
+            raise RuntimeError(f"_mtpk_torch.so was built against ABI version {_mtpk_torch.abi_version}, the binding expects "
+                               f"{ABI_VERSION}: rebuild it")
+        _mtpk_torch.bind({n: ctypes.cast(getattr(handle, n), c_void_p).value for n in _NATIVE_ENTRIES})
+        _native = _mtpk_torch
+    return _native
+
+
+def stream_for(x: torch.Tensor) -> int:
+    """Handle of torch's current stream on the device of `x`, a device tensor."""
+    index = x.get_device()
+    if index < 0:
+        raise ValueError("libmtpk entry points take device tensors")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def check(status: int, what: str) -> None:
     """Raise on a nonzero status; the message names the entry point and the cause."""
     if status != 0:
@@ -326,26 +357,6 @@ def stream_of(device: torch.device) -> int:
     """Handle of torch's current stream on `device` (what the kernels launch on): the handle alone, without
     the Stream object around it (0.1 against 2.1 us a call)."""
     return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-_HERE = contextlib.nullcontext()
-
-
-def on(device: torch.device):
-    """A context in which `device` is the current one: launches and workgroup counts go by it, also
-    where the tensors are not on the device that the caller has selected."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def rows16(x: torch.Tensor) -> bool:
-    """Whether every row of `x` along its last dim is contiguous and starts on 16 bytes."""
-    unit, strides = 16 // x.element_size(), x.stride()
-    if strides[-1] != 1 or x.data_ptr() % 16:
-        return False
-    for s in strides[:-1]:
-        if s % unit:
-            return False
-    return True
 
 
 def float_code(dtype: torch.dtype) -> int:

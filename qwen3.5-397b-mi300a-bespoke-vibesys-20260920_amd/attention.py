@@ -13,7 +13,6 @@ bf16 `[B, heads, t, hd]`.
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -181,32 +180,6 @@ def kv_write(k_pool: torch.Tensor, v_pool: torch.Tensor, k: torch.Tensor, v: tor
         kvh, hd, _mtpk.stream_of(device)), "mtpk_kv_write")  # fmt: skip
 
 
-def cache_operands(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, base_pos: torch.Tensor,
-                   batch: int, kv_heads: int, head_dim: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """`(table, base)` as the kernels read them, contiguous int32 and int64; raises unless the pools are a
-    K and a V cache of these heads, contiguous bf16, with a table and a base position for each lane."""
-    rows = k_pool.shape[0]
-    if k_pool.shape != (rows, kv_heads, head_dim) or rows % BLOCK or rows == 0:
-        raise ValueError(f"k_pool must be [rows, {kv_heads}, {head_dim}] of {BLOCK}-row blocks, got {list(k_pool.shape)}")
-    if v_pool.shape != (rows // BLOCK, kv_heads, head_dim, BLOCK):
-        raise ValueError(f"v_pool must be {[rows // BLOCK, kv_heads, head_dim, BLOCK]} (V transposed per block), "
-                         f"got {list(v_pool.shape)}")
-    if not k_pool.dtype == v_pool.dtype == torch.bfloat16 or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
-        raise ValueError("pools must be contiguous bf16")
-    if block_table.dim() != 2 or block_table.shape[0] != batch or base_pos.shape != (batch,):
-        raise ValueError(f"block_table must be [{batch}, blocks] and base_pos [{batch}], got "
-                         f"{list(block_table.shape)} and {list(base_pos.shape)}")
-    if block_table.dtype != torch.int32:
-        if block_table.dtype != torch.int64:
-            raise ValueError(f"block_table must be int32 or int64, got {block_table.dtype}")
-        block_table = block_table.to(torch.int32)
-    if base_pos.dtype != torch.int64:
-        if base_pos.dtype != torch.int32:
-            raise ValueError(f"base_pos must be int32 or int64, got {base_pos.dtype}")
-        base_pos = base_pos.to(torch.int64)
-    return block_table.contiguous(), base_pos.contiguous()
-
-
 def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                            base_pos: torch.Tensor, ctx_len: int, scale: float, *, softcap: float = 0.0,
                            window: int = 0, slopes: torch.Tensor | None = None,
@@ -223,70 +196,8 @@ def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     `gate` of q's shape multiplies the output by its sigmoid. Keys that a row does not see never reach its
     output, whatever they hold. `ctx_len` is a host bound on `max(base_pos) + t`; it sizes the key splits
     alone. bf16 with fp32 scores, statistics and sums; the output is rounded once."""
-    device = _mtpk.require_device(q, k_pool, v_pool, block_table, base_pos)
-    if q.dim() != 4 or q.dtype != torch.bfloat16:
-        raise ValueError(f"q must be bf16 [B, t, heads, hd], got {q.dtype} {tuple(q.shape)}")
-    b, t, heads, hd = q.shape
-    if hd not in HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {hd}")
-    if k_pool.dim() != 3:
-        raise ValueError(f"k_pool must be [rows, kv_heads, {hd}], got {list(k_pool.shape)}")
-    kvh = k_pool.shape[1]
-    table, pos = cache_operands(k_pool, v_pool, block_table, base_pos, b, kvh, hd)
-    if heads == 0 or kvh == 0 or heads % kvh:
-        raise ValueError(f"{heads} q heads are not a multiple of {kvh} kv heads")
-    if not 0 <= ctx_len <= table.shape[1] * BLOCK:
-        raise ValueError(f"context bound {ctx_len} exceeds the table's {table.shape[1]} blocks")
-    if not 0 < scale < math.inf or not 0 <= softcap < math.inf or window < 0:
-        raise ValueError(f"scale must be positive, softcap and window not negative, got {scale}, {softcap} and {window}")
-    gs = prefix_dt = first_dt = 0
-    if gate is not None:
-        if gate.shape != q.shape or gate.dtype != torch.bfloat16 or gate.device != device:
-            raise ValueError("gate must be bf16 of q's shape on its device")
-        if not _mtpk.rows16(gate):
-            gate = gate.clone(memory_format=torch.contiguous_format)
-        s = gate.stride()
-        gate_strides = _Three(s[0], s[2], s[1])
-        gs = ctypes.addressof(gate_strides)
-    if slopes is not None:
-        if slopes.shape != (heads,) or slopes.dtype != torch.float32 or slopes.device != device:
-            raise ValueError(f"slopes must be float32 [{heads}] on {device}")
-        slopes = slopes.contiguous()
-    if prefix is not None:
-        prefix, prefix_dt = _integers(prefix, "prefix", (b,), device)
-    if first is not None:
-        first, first_dt = _integers(first, "first", (b, t), device)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if out.numel() == 0:
-        return out
-    if not _mtpk.rows16(q):
-        q = q.clone(memory_format=torch.contiguous_format)
-    s, z = q.stride(), out.stride()
-    qs, os_ = _Three(s[0], s[2], s[1]), _Three(z[0], z[2], z[1])
-    lib = _mtpk.lib()
-    with _mtpk.on(device):
-        n_split = lib.mtpk_attention_masked_splits(b, t, heads, kvh, hd, ctx_len, window)
-        ws, ws_bytes = None, 0
-        if n_split > 1:
-            ws_bytes = lib.mtpk_attention_masked_workspace_bytes(b, t, heads, kvh, hd, n_split)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-        status = lib.mtpk_paged_attention_masked(
-            q.data_ptr(), ctypes.addressof(qs), _mtpk.ptr(gate), gs, b, t, heads, kvh, hd, k_pool.data_ptr(),
-            v_pool.data_ptr(), k_pool.shape[0], table.data_ptr(), table.shape[1], pos.data_ptr(), scale, softcap, window,
-            _mtpk.ptr(slopes), _mtpk.ptr(prefix), prefix_dt, _mtpk.ptr(first), first_dt, n_split, _mtpk.ptr(ws), ws_bytes,
-            out.data_ptr(), ctypes.addressof(os_), _mtpk.stream_of(device))
-    if status:
-        _mtpk.check(status, "mtpk_paged_attention_masked")
-    return out
-
-
-_Three = ctypes.c_int64 * 3
-
-
-def _integers(x: torch.Tensor, name: str, shape: tuple, device: torch.device) -> tuple[torch.Tensor, int]:
-    if x.shape != shape or x.dtype not in (torch.int32, torch.int64) or x.device != device:
-        raise ValueError(f"{name} must be int32 or int64 {list(shape)} on {device}, got {x.dtype} {list(x.shape)}")
-    return x.contiguous(), _mtpk.index_code(x.dtype)
+    return _mtpk.native().paged_attention_masked(q, k_pool, v_pool, block_table, base_pos, ctx_len, scale, softcap, window,
+                                                 slopes, prefix, first, gate, _mtpk.stream_for(q))
 
 
 def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None:
@@ -298,52 +209,29 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
     `ValueError`) and copied to the device, or int32 / int64 device tensors, which are taken as they are:
     a pair with an id outside the pools is skipped, and the rest of the rule is the caller's. CPU pools
     take the torch spelling."""
-    if not pools:
-        raise ValueError("copy_blocks takes at least one pool")
-    first = pools[0]
-    device, where = first.device, first.get_device()
-    n_blocks = first.size(0) // (1 if first.dim() == 4 else block)
-    rows = n_blocks * block
-    for p in pools:
-        n = p.size(0) if p.dim() in (3, 4) else -1
-        if n != (n_blocks if p.dim() == 4 else rows) or n == 0 or p.get_device() != where or not p.is_contiguous():
-            raise ValueError("pools must be contiguous K caches [rows, kv_heads, hd] and V caches [blocks, kv_heads, hd, "
-                             f"{block}] of one number of blocks on one device, got {tuple(p.shape)} on {p.device}")
-    sizes = [p.nbytes // n_blocks for p in pools]
-    if 0 in sizes:
-        raise ValueError("pools must not be empty")
-    checked = not (torch.is_tensor(src) and src.is_cuda)
-    if checked != (not (torch.is_tensor(dst) and dst.is_cuda)):
-        raise ValueError("src and dst must both be on the host or both on the device")
-    if checked:
-        src, dst = (torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in (src, dst))
-    if src.shape != dst.shape or src.dim() != 1 or src.dtype not in (torch.int32, torch.int64) or src.dtype != dst.dtype:
-        raise ValueError("src and dst must be int32 or int64 vectors of one length and type")
-    pairs = src.shape[0]
-    if pairs == 0:
+    native = _mtpk.native()
+    held = [torch.is_tensor(x) and x.is_cuda for x in (src, dst)]
+    if all(held):
+        native.copy_blocks(pools, src, dst, block, _mtpk.stream_for(src))
         return
-    if checked:
-        if int(min(src.min(), dst.min())) < 0 or int(max(src.max(), dst.max())) >= n_blocks:
-            raise ValueError(f"block ids must lie in [0, {n_blocks})")
-        kinds = torch.zeros(n_blocks, dtype=torch.int32)
-        kinds.index_add_(0, dst, torch.ones(pairs, dtype=torch.int32))
-        if int(kinds.max()) > 1 or int(kinds[src].max()) > 0:
-            raise ValueError("a block is the destination of two pairs, or source and destination")
+    if any(held):
+        raise ValueError("src and dst must both be on the host or both on the device")
+    n_blocks = native.pool_blocks(pools, block)
+    src, dst = (torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in (src, dst))
+    if src.shape != dst.shape:
+        raise ValueError("src and dst must be of one length")
+    if src.numel() == 0:
+        return
+    if int(min(src.min(), dst.min())) < 0 or int(max(src.max(), dst.max())) >= n_blocks:
+        raise ValueError(f"block ids must lie in [0, {n_blocks})")
+    taken = torch.bincount(dst, minlength=n_blocks)
+    if int(taken.max()) > 1 or int(taken[src].max()) > 0:
+        raise ValueError("a block is the destination of two pairs, or source and destination")
+    device = pools[0].device
     if device.type == "cpu":
         for p in pools:
             blocks = p.view(n_blocks, -1)
             blocks[dst] = blocks[src]
         return
-    if checked:
-        src, dst = torch.stack((src, dst)).pin_memory().to(device, non_blocking=True).unbind(0)
-    elif src.device != device or dst.device != device:
-        raise ValueError(f"src and dst must be on {device}")
-    at = [p.data_ptr() for p in pools]
-    src, dst = src.contiguous(), dst.contiguous()
-    ptrs, bytes_ = (ctypes.c_void_p * len(at))(*at), (ctypes.c_int64 * len(at))(*sizes)
-    with _mtpk.on(device):
-        status = _mtpk.lib().mtpk_copy_blocks(
-            ctypes.addressof(ptrs), ctypes.addressof(bytes_), len(at), n_blocks, src.data_ptr(), dst.data_ptr(),
-            _mtpk.index_code(src.dtype), pairs, _mtpk.stream_of(device))
-    if status:
-        _mtpk.check(status, "mtpk_copy_blocks (blocks of a multiple of 16 bytes, pools on 16 bytes)")
+    pairs = torch.stack((src, dst)).pin_memory().to(device, non_blocking=True)
+    native.copy_blocks(pools, pairs[0], pairs[1], block, _mtpk.stream_for(pairs))

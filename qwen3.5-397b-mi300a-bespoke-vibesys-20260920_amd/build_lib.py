@@ -1,4 +1,5 @@
-"""Builds `libmtpk.so` (gfx950) in this directory with hipcc, one object per translation unit.
+"""Builds `libmtpk.so` (gfx950) in this directory with hipcc, one object per translation unit, and
+`_mtpk_torch.so`, the C++ calls on torch tensors in front of some of its entry points, with g++.
 
 `python build_lib.py` or `build_lib.build()`; `__graft_entry__.build()` calls it. Rebuilds every
 time it is called (the build is the compile check), in parallel across translation units.
@@ -9,6 +10,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -16,6 +18,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 LIB = HERE / "libmtpk.so"
+TORCH_LIB = HERE / "_mtpk_torch.so"
 OBJ_DIR = HERE / "_build"
 ARCH = os.environ.get("MTPK_ARCH", "gfx950")
 SOURCES = ["mtpk_runtime.hip", "mtpk_moe.hip", "mtpk_router.hip", "mtpk_accept.hip", "mtpk_deltanet.hip",
@@ -53,10 +56,30 @@ def _compile(src: str) -> Path:
     return obj
 
 
+def _build_torch_calls() -> None:
+    """`_mtpk_torch.so`: host C++ against the installed torch, no device code and no link to libmtpk (its
+    entry points' addresses are handed over when it is loaded)."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", f"-isystem{root / 'include'}",
+           f"-isystem{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+           f"-isystem{sysconfig.get_paths()['include']}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-DTORCH_EXTENSION_NAME=_mtpk_torch", str(CSRC / "mtpk_torch.cpp"), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10"]  # fmt: skip
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for mtpk_torch.cpp:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, TORCH_LIB)
+
+
 def build(verbose: bool = False) -> Path:
     OBJ_DIR.mkdir(exist_ok=True)
     with ThreadPoolExecutor(max_workers=min(7, len(SOURCES))) as pool:
+        calls = pool.submit(_build_torch_calls)
         objs = list(pool.map(_compile, SOURCES))
+        calls.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -64,7 +87,7 @@ def build(verbose: bool = False) -> Path:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB)
     if verbose:
-        print(f"built {LIB}")
+        print(f"built {LIB} and {TORCH_LIB.name}")
     return LIB
 
 
