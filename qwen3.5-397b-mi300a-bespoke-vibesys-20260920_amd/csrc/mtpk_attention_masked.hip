@@ -134,7 +134,7 @@ struct BlockSource {
   rsrc_t k, v;
   __device__ inline BlockSource(const MaskedArgs& a, int blk, bool wanted) {
     const int64_t slab = (int64_t)kAttnBlock * a.kvh * HD;
-    const bool ok = wanted && blk >= 0 && (int64_t)(blk + 1) * kAttnBlock <= a.pool_rows;
+    const bool ok = wanted && blk >= 0 && ((int64_t)blk + 1) * kAttnBlock <= a.pool_rows;
     const int64_t at = (int64_t)uniform(ok ? blk : 0) * slab;
     const uint32_t bytes = (uint32_t)uniform(ok ? (int)(slab * 2) : 0);  // a block outside the pool reads as zeros
     k = make_rsrc(a.k_pool + at, bytes);
@@ -354,7 +354,7 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
     const int key = key0 + lane;
     const bool live = key < row.hi;
     const int id = live ? trow[key / kAttnBlock] : -1;
-    const bool held = id >= 0 && (int64_t)(id + 1) * kAttnBlock <= a.pool_rows;  // else the block reads as zeros
+    const bool held = id >= 0 && ((int64_t)id + 1) * kAttnBlock <= a.pool_rows;  // else the block reads as zeros
     float s = 0.f;
     if (held) {
       const uint16_t* const k = a.k_pool + (((int64_t)id * kAttnBlock + key % kAttnBlock) * a.kvh + kh) * HD;

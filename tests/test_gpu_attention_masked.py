@@ -194,7 +194,7 @@ def test_lanes_that_hold_nothing(dev) -> None:
     """Padding lanes: a negative base, a base past the table, a table entry outside the pool."""
     q, k, v, table, b0 = case(10, 4, 2, 8, 2, 64, [50, 50, 50, 50])
     b0[1], b0[2] = -2, table.shape[1] * 16 + 100
-    table[3, 1], table[3, 2] = -5, 10**8
+    table[3, 1], table[3, 2] = -5, 2**31 - 1
     got = run(dev, q, k, v, table, b0, 0.1, 52, window=30).double().cpu()
     assert not got[1].any() and not got[2].any()
     k[:16], v[:16] = 0, 0
