@@ -197,9 +197,13 @@ __device__ inline void load_lds(rsrc_t r, uint8_t* to, uint32_t off) {
 // at kNoKey, far above it and far below any score in use: neither needs a comparison later on, and
 // both stay finite where the cap's line squares them. Capped scores up to 2^kCapMost need no maximum at all:
 // their exponentials and sums stay inside fp32's and bf16's range as they are, and so the largest part of
-// the work between the two products falls away. A row whose sum all the same comes out below kLeastSum (its
+// the work between the two products falls away. A row whose sum all the same comes out below least_sum (its
 // keys all far below, or none: 0), or that holds a value that is not finite, is done again by masked_row_slow.
-constexpr float kUnseen = -1e18f, kNoKey = -1e17f, kLeastSum = 0x1p-102f, kCapMost = 100.f;
+constexpr float kUnseen = -1e18f, kNoKey = -1e17f, kCapMost = 100.f;
+
+// The cap alone leaves every key at least 2^-100. A bias may take keys below 2^-126, where they are lost: up to 2^20
+// of them are then less than 2^-26 of a sum that is at least 2^-80.
+__device__ inline float least_sum(const MaskedArgs& a) { return a.slopes ? 0x1p-80f : 0x1p-102f; }
 
 struct RowSoft {
   float m, l;
@@ -309,7 +313,8 @@ __device__ inline void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-__device__ inline float row_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+// NaN where the sum has left fp32's range, as a bias that raises the weights makes it: the row is then done again.
+__device__ inline float row_inverse(float l) { return l == 0.f ? 0.f : 1.f / l + (l - l); }
 
 __device__ inline float sigmoid_of(uint16_t g) {
   // exp2 and reciprocal, 1 ulp each; scaled, as the reciprocal of a value above 2^126 would be flushed
@@ -337,7 +342,7 @@ __device__ inline void store_out8(const MaskedArgs& a, int b, int hq, int st, in
 
 // One row by one wave, key by key in fp32 straight from memory: for the rows whose result above is not
 // finite (a value or score that is not, seen by this row or by another one that shares its tiles), or
-// whose scores all lie below kNoKey. What the row does not see is not read.
+// whose keys all weigh too little. What the row does not see is not read.
 template <int HD>
 __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, int lane) {
   constexpr int NV = HD / kWave;
@@ -663,7 +668,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       }
       wave_lds_fence();
     }
-    uint64_t again = __ballot(real && (odd != 0.f || (l < kLeastSum && row.hi > row.lo)));
+    uint64_t again = __ballot(real && (odd != 0.f || (l < least_sum(a) && row.hi > row.lo)));
     again = (again | again >> 32) & 0xffffffffull;
     while (again != 0ull) {
       const int rl = uniform(__builtin_ctzll(again)), ro = kRows * rg + 32 * wave + rl;
@@ -873,7 +878,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     }
     if (a.n_split == 1) {
       const float inv = row_inverse(sum);
-      float odd = sum < kLeastSum ? 1.f : 0.f;  // not 0: the row is done again, below
+      float odd = sum < least_sum(a) ? 1.f : 0.f;  // not 0: the row is done again, below
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         y[e] *= inv;
@@ -943,7 +948,7 @@ __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, in
   }
   uint16_t* const orow = a.out + a.orow.at(b, hq, st) + NV * lane;
   const uint16_t* const grow = a.gate ? a.gate + a.gr.at(b, hq, st) + NV * lane : nullptr;
-  float odd = sum < kLeastSum ? 1.f : 0.f;
+  float odd = sum < least_sum(a) ? 1.f : 0.f;
 #pragma unroll
   for (int e = 0; e < NV; ++e) {
     const float y = acc[e] * inv;

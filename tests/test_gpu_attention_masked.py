@@ -8,6 +8,8 @@ log2 at 2^-23 each, and the exponential: 3e-4 of a weight is allowed, twice for 
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -109,6 +111,51 @@ def test_scores_past_the_polynomial(dev, heads, kvh, hd, t, base) -> None:
     q, k, v, table, b0 = case(1, 1, t, heads, kvh, hd, base, q_std=8.0)
     check(dev, q, k, v, table, b0, hd**-0.5, softcap=2.0)
     check(dev, q, k, v, table, b0, hd**-0.5, softcap=9.0, window=60)
+
+
+@pytest.mark.parametrize("softcap", [69.0, 70.0, 1000.0])
+@pytest.mark.parametrize("heads,kvh,hd,t,base", [(32, 2, 256, 1, [500]), (32, 2, 256, 40, [9]), (16, 4, 128, 12, [3000])])
+def test_wide_caps(dev, heads, kvh, hd, t, base, softcap) -> None:
+    """Either side of the widest cap whose scores need no running maximum."""
+    q, k, v, table, b0 = case(1, 1, t, heads, kvh, hd, base, q_std=8.0)
+    check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap)
+    check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap, slopes=torch.linspace(0.0, 2.0, heads))
+
+
+@pytest.mark.parametrize("heads,kvh,hd,t,base", [(32, 2, 256, 1, [500]), (32, 2, 256, 40, [9]), (16, 4, 128, 12, [3000])])
+@pytest.mark.parametrize("softcap", [0.0, 30.0, 50.0, 69.0])
+def test_scores_far_from_zero(dev, heads, kvh, hd, t, base, softcap) -> None:
+    """All scores at the cap's lower or upper end (without a cap: at -3e4 and 3e4): weights are what differences
+    between them make, however small or large all of them are."""
+    q, k, v, table, b0 = case(2, 1, t, heads, kvh, hd, base)
+    far = torch.randn(1, kvh, hd).bfloat16()
+    k = (far + torch.randn(k.shape) * 0.02).bfloat16()
+    for sign in (1.0, -1.0):
+        qs = (sign * far.float().repeat_interleave(heads // kvh, 1) * 16.0).bfloat16().expand(1, t, heads, hd).contiguous()
+        check(dev, qs, k, v, table, b0, 1.0 if softcap else hd**-0.5, softcap=softcap)
+
+
+def test_biases_that_leave_little(dev) -> None:
+    """Rows that see only keys far ahead of them (a prefix, their document beginning behind them), so that the
+    bias takes every weight far down, and slopes below zero, which take them up."""
+    heads, kvh, hd, t = 8, 2, 128, 200
+    q, k, v, table, b0 = case(3, 1, t, heads, kvh, hd, [0])
+    pos = torch.arange(t)[None]
+    first = torch.where(pos < 100, pos + 90, pos - 3)
+    slopes = torch.tensor([0.0, 0.1, 0.6, 0.8, 0.9, 1.0, 2.0, 50.0])
+    for softcap in (0.0, 50.0):
+        check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap, slopes=slopes, first=first, prefix=b0 + t)
+        check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap, slopes=-slopes[:1].expand(8) - 1.5)
+
+
+@pytest.mark.parametrize("t,base", [(1, [3000]), (1, [200]), (12, [1500]), (40, [700])])
+def test_biases_that_pass_the_range_of_the_sum(dev, t, base) -> None:
+    """Slopes below zero whose largest weight is about 2^127, so that every weight and product is finite but their
+    sum is not: values are small."""
+    heads, kvh, hd = 8, 2, 128
+    q, k, v, table, b0 = case(4, 1, t, heads, kvh, hd, base, q_std=0.05)
+    slopes = -torch.linspace(120.0, 130.0, heads) * math.log(2.0) / base[0]
+    check(dev, q, k, (v.float() * 2.0**-30).bfloat16(), table, b0, hd**-0.5, softcap=50.0, slopes=slopes)
 
 
 @pytest.mark.parametrize("t,base,heads,kvh,hd", [(1, [29999, 7], 8, 2, 128), (4, [8000, 0, 515], 32, 2, 256), (20, [9000], 8, 2, 64)])
