@@ -203,8 +203,8 @@ Tensor rotate_to_cache(const Tensor& q_in, const Tensor& k_in, const Tensor& v_i
     pos = pos->contiguous();
   }
   if (keep) {
-    need(keep->dim() == 2 && keep->size(0) == b && keep->size(1) == t && keep->element_size() == 1, "keep must be bool [", b, ", ", t,
-         "]");
+    const bool flags = keep->scalar_type() == at::kBool || keep->scalar_type() == at::kByte;
+    need(flags && keep->dim() == 2 && keep->size(0) == b && keep->size(1) == t, "keep must be bool [", b, ", ", t, "]");
     on(device, *keep);
   }
   const Tensor out = at::empty_like(q_in, q_in.options(), at::MemoryFormat::Contiguous);
