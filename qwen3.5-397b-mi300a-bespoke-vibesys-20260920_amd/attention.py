@@ -207,8 +207,8 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
     `src` and `dst` are block ids of equal length: lists or CPU tensors, which are checked (each id inside
     the pools, no block the destination of two pairs, nor source of one and destination of another;
     `ValueError`) and copied to the device, or int32 / int64 device tensors, which are taken as they are:
-    a pair with an id outside the pools is skipped, and the rest of the rule is the caller's. CPU pools
-    take the torch spelling."""
+    a pair with an id outside the pools is skipped, and the rest of the rule is the caller's; a captured call
+    takes device ids alone. CPU pools take the torch spelling."""
     native = _mtpk.native()
     held = [torch.is_tensor(x) and x.is_cuda for x in (src, dst)]
     if all(held):
@@ -222,6 +222,8 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
         raise ValueError("src and dst must be of one length")
     if src.numel() == 0:
         return
+    if pools[0].is_cuda and torch.cuda.is_current_stream_capturing():
+        raise ValueError("host ids cannot be part of a graph: give src and dst on the device")
     if int(min(src.min(), dst.min())) < 0 or int(max(src.max(), dst.max())) >= n_blocks:
         raise ValueError(f"block ids must lie in [0, {n_blocks})")
     taken = torch.bincount(dst, minlength=n_blocks)

@@ -75,6 +75,21 @@ def test_in_a_graph(dev) -> None:
         assert all(torch.equal(a, b) for a, b in zip(pools, want))
 
 
+def test_host_ids_are_refused_in_a_capture(dev) -> None:
+    """The graph would read the host's ids again at every replay, long after they are gone."""
+    pools = _pools(dev, 1, 8, 2, 64)
+    attention.copy_blocks(pools, [1], [2])
+    before = [p.clone() for p in pools]
+    src, dst = torch.tensor([3], device=dev), torch.tensor([4], device=dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attention.copy_blocks(pools, src, dst)
+        with pytest.raises(ValueError, match="graph"):
+            attention.copy_blocks(pools, [1], [5])
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(pools, _want(before, src, dst, 8)))
+
+
 def test_offsets_past_four_gigabytes(dev) -> None:
     kvh, hd = 8, 256
     blocks = 2**32 // (16 * kvh * hd * 2) + 64
