@@ -1019,7 +1019,7 @@ int mtpk_attention_masked_splits(int64_t batch, int64_t t, int64_t heads, int64_
   if (!masked_shape(batch, t, heads, kv_heads, head_dim) || max_ctx < 0 || window < 0) return 0;
   const int64_t rows = heads / kv_heads * t;
   int64_t keys = max_ctx;
-  if (window > 0) keys = std::min(keys, window + masked_group_rows(rows) / (heads / kv_heads) + kTileKeys);
+  if (window > 0 && window < keys) keys = std::min(keys, window + masked_group_rows(rows) / (heads / kv_heads) + kTileKeys);
   return masked_splits(batch, kv_heads, rows, head_dim, keys);
 }
 

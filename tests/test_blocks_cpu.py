@@ -214,5 +214,8 @@ def test_masked_attention_sizes(lib) -> None:
     assert lib.mtpk_attention_masked_splits(2, 1, 8, 3, 64, 100, 0) == 0
     assert lib.mtpk_attention_masked_splits(2, 1, 8, 2, 96, 100, 0) == 0
     assert lib.mtpk_attention_masked_splits(2, 1, 8, 2, 64, 0, 0) == 1
+    for ctx in (0, 100, 30000):  # a window past every context is none
+        assert (lib.mtpk_attention_masked_splits(1, 1, 32, 2, 256, ctx, 2**63 - 1)
+                == lib.mtpk_attention_masked_splits(1, 1, 32, 2, 256, ctx, 0))
     assert lib.mtpk_attention_masked_workspace_bytes(2, 1, 8, 2, 64, 1) == 0
     assert lib.mtpk_attention_masked_workspace_bytes(2, 1, 8, 2, 64, 3) >= 2 * 2 * 4 * 3 * 66 * 4
