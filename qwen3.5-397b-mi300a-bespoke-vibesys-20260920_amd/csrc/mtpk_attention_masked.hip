@@ -45,7 +45,7 @@ struct MaskedArgs {
   AttnRows gr;
   const uint16_t* k_pool;
   const uint16_t* v_pool;
-  int64_t pool_rows;
+  uint32_t pool_blocks;  // at most 2^31: a table's entries are int32
   const int32_t* table;
   int64_t table_stride;
   const int64_t* base;
@@ -134,7 +134,7 @@ struct BlockSource {
   rsrc_t k, v;
   __device__ inline BlockSource(const MaskedArgs& a, int blk, bool wanted) {
     const int64_t slab = (int64_t)kAttnBlock * a.kvh * HD;
-    const bool ok = wanted && blk >= 0 && ((int64_t)blk + 1) * kAttnBlock <= a.pool_rows;
+    const bool ok = wanted && (uint32_t)blk < a.pool_blocks;
     const int64_t at = (int64_t)uniform(ok ? blk : 0) * slab;
     const uint32_t bytes = (uint32_t)uniform(ok ? (int)(slab * 2) : 0);  // a block outside the pool reads as zeros
     k = make_rsrc(a.k_pool + at, bytes);
@@ -172,25 +172,26 @@ __device__ inline uint32_t v_offset(int lane, int kh) {
   return (uint32_t)(kh * HD * 32 + (lane >> 1) * 32 + (((lane & 1) ^ v_swap(lane >> 1)) * 16));
 }
 
-// V of `blocks` blocks in LDS, the first one's keys from key0 on: zeros at the keys outside [lo, hi), 16 bytes (8 keys
-// of a channel) a thread.
+// V of `blocks` blocks in LDS, the first one's keys from key0 on: zeros at the keys outside [lo, hi). A wave takes 8 keys
+// of 64 channels at a time, so that what of them is seen is one scalar mask.
 template <int HD>
 __device__ inline void zero_unseen(uint8_t* v, int blocks, int key0, int lo, int hi, int tid, int threads) {
   for (int i = tid; i < blocks * HD * 2; i += threads) {
-    const int d = i / 2 % HD, first = key0 + kAttnBlock * (i / (2 * HD)) + 8 * ((i & 1) ^ v_swap(d));
-    if (first >= lo && first + 8 <= hi) continue;
-    u32x4_t w = lds16(v + i * 16);
+    const int x = uniform(i / HD), d = i % HD, from = lo - key0 - 8 * x, to = hi - key0 - 8 * x;
+    if (from <= 0 && to >= 8) continue;
+    uint8_t* const at = v + (x >> 1) * (HD * 32) + d * 32 + ((x & 1) ^ v_swap(d)) * 16;
+    u32x4_t w = lds16(at);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int key = first + 2 * e;
-      w[e] &= (key >= lo && key < hi ? 0x0000ffffu : 0u) | (key + 1 >= lo && key + 1 < hi ? 0xffff0000u : 0u);
-    }
-    lds16_store(v + i * 16, w);
+    for (int e = 0; e < 4; ++e)
+      w[e] &= (2 * e >= from && 2 * e < to ? 0x0000ffffu : 0u) | (2 * e + 1 >= from && 2 * e + 1 < to ? 0xffff0000u : 0u);
+    lds16_store(at, w);
   }
 }
 
+// 1 KB from off + AT of each lane to `to` + AT (at most 4095).
+template <int AT = 0>
 __device__ inline void load_lds(rsrc_t r, uint8_t* to, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)to, 16, (int)off, 0, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)to, 16, (int)off, 0, AT, 0);
 }
 
 // Scores are worked on in units of log2. What a row does not see becomes kUnseen, and a row's maximum starts
@@ -220,30 +221,29 @@ __device__ inline float halves_max(float v) {
   return fmaxf(bits_f32(r[0]), bits_f32(r[1]));
 }
 
-// One tile of scores on its way to P, in steps that the caller puts between its products: prepare, then
-// exponents [first, first + n) in any pieces.
+// One tile of scores on its way to P, in steps that the caller puts between its products: scan (every value once),
+// finish, and each value's exponent.
 template <bool CAP, bool SLOPES>
 struct TileSoftmax {
   float c0, c1, ms;  // exponent of a score s: s (c0 + c1 s^2) with a cap, s c0 - ms without one
+  float top;         // the largest score, with a cap the largest magnitude
+  float held;
 
-  // Scores to where `exponents` takes them from there, and without a cap the row's new maximum. Returns what the
+  __device__ inline void begin() { top = CAP ? 0.f : -INFINITY; }
+  __device__ inline void scan(float s) { top = fmaxf(top, CAP ? fabsf(s) : s); }
+
+  // Scores to where `exponent` takes them from there, and without a cap the row's new maximum. Returns what the
   // row's sums are multiplied by, 1 for the whole wave in most tiles.
-  __device__ inline float prepare(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
-                                  int h, RowSoft& r) {
+  __device__ inline float finish(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
+                                 int h, RowSoft& r) {
     c0 = a.c0;
     c1 = a.c1;
-    float am = 0.f;  // the largest magnitude, where the cap is on
-    if (CAP) {
-      am = fabsf(s[0]);
-#pragma unroll
-      for (int i = 1; i < 16; ++i) am = fmaxf(am, fabsf(s[i]));
-    }
-    const bool bent = CAP ? __ballot(!(am <= a.cubic_max)) != 0ull : a.cap2 > 0.f;  // past the cap's cubic part
+    const bool bent = CAP ? __ballot(!(top <= a.cubic_max)) != 0ull : a.cap2 > 0.f;  // past the cap's cubic part
     if (SLOPES || !whole || bent) {  // uniform over the wave: in full here, and the exponent is the score
       if (!bent) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = CAP ? s[i] * fmaf(s[i] * s[i], c1, c0) : s[i] * c0;
-      } else if (CAP && __ballot(!(am <= a.quintic_max)) == 0ull) {
+      } else if (CAP && __ballot(!(top <= a.quintic_max)) == 0ull) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float u = s[i] * s[i];
@@ -266,33 +266,41 @@ struct TileSoftmax {
       }
       c0 = 1.f;
       c1 = 0.f;
+      if (!CAP) {
+        begin();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) scan(s[i]);
+      }
     }
     if (CAP) return 1.f;
-    float tm = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) tm = fmaxf(tm, s[i]);
-    ms = fmaxf(r.m, halves_max(tm * c0));
+    ms = fmaxf(r.m, halves_max(top * c0));
     const float alpha = __builtin_amdgcn_exp2f(r.m - ms);
     r.m = ms;
     r.l *= alpha;
     return alpha;
   }
+  __device__ inline float prepare(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
+                                  int h, RowSoft& r) {
+    begin();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) scan(s[i]);
+    return finish(a, s, row, slope2, whole, key0, h, r);
+  }
 
-  template <int FIRST, int N>
-  __device__ inline void exponents(const f32x16_t& s, u32x4_t (&p)[2], RowSoft& r) const {
-    const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
-#pragma unroll
-    for (int i = FIRST; i < FIRST + N; i += 2) {
-      bf16x2_t e;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float x = s[i + j];
-        e[j] = (__bf16)__builtin_amdgcn_exp2f(CAP ? x * fmaf(x * x, c1, c0) : fmaf(x, c0, -ms));
-      }
+  // Value I of a tile; the odd ones, after their even neighbour, store both.
+  template <int I>
+  __device__ inline void exponent(const f32x16_t& s, u32x4_t (&p)[2], RowSoft& r) {
+    const float x = s[I], y = __builtin_amdgcn_exp2f(CAP ? x * fmaf(x * x, c1, c0) : fmaf(x, c0, -ms));
+    if constexpr (I % 2 == 0) {
+      held = y;
+    } else {
+      const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f}, e = {(__bf16)held, (__bf16)y};
       uint32_t w = __builtin_bit_cast(uint32_t, e);
       asm volatile("" : "+v"(w));  // here, beside the products around it, and not where the second product is
-      p[i >> 3][i >> 1 & 3] = w;
-      r.l = __builtin_amdgcn_fdot2_f32_bf16(e, one, r.l, false);  // the sum of what the product uses
+      p[I >> 3][I >> 1 & 3] = w;
+      // the sum of what the product uses
+      r.l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), one, r.l, false);
+      asm volatile("" : "+v"(r.l));
     }
   }
 };
@@ -317,8 +325,8 @@ __device__ inline void wave_lds_fence() {
 __device__ inline float row_inverse(float l) { return l == 0.f ? 0.f : 1.f / l + (l - l); }
 
 __device__ inline float sigmoid_of(uint16_t g) {
-  // exp2 and reciprocal, 1 ulp each; scaled, as the reciprocal of a value above 2^126 would be flushed
-  return __builtin_amdgcn_rcpf((1.f + __builtin_amdgcn_exp2f(-kLog2e * bf16_to_f32(g))) * 0x1p-32f) * 0x1p-32f;
+  // exp2 and reciprocal, 1 ulp each, of 2^-32 (1 + exp(-g)): the reciprocal of a value above 2^126 would be flushed
+  return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fmaf(-kLog2e, bf16_to_f32(g), -32.f)) + 0x1p-32f) * 0x1p-32f;
 }
 
 // Eight values of an output row, gated, rounded once.
@@ -359,7 +367,7 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
     const int key = key0 + lane;
     const bool live = key < row.hi;
     const int id = live ? trow[key / kAttnBlock] : -1;
-    const bool held = id >= 0 && ((int64_t)id + 1) * kAttnBlock <= a.pool_rows;  // else the block reads as zeros
+    const bool held = (uint32_t)id < a.pool_blocks;  // else the block reads as zeros
     float s = 0.f;
     if (held) {
       const uint16_t* const k = a.k_pool + (((int64_t)id * kAttnBlock + key % kAttnBlock) * a.kvh + kh) * HD;
@@ -408,22 +416,35 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
 
 // ---------------------------------------------------------------- many rows
 //
-// W waves of 32 rows to a workgroup, which share stages of NT tiles, one stage ahead in two buffers with
-// one barrier per stage: prompts, and verify rows of more than one wave. With two tiles a stage (heads up to
-// 128) the second tile's first product runs between the first one's exponents, and the first one's second
-// product between the second one's; with one (heads of 256, whose sums fill the registers) the exponents of
-// the tile's second block run between the products of its first.
+// W waves of 32 rows to a workgroup, which share stages of ST tiles, one stage ahead in two buffers with
+// one barrier per stage: prompts, and verify rows of more than one wave. With heads up to 128 a tile's first
+// product runs one tile ahead of its second (AHEAD): between the products of S^T of tile t + 1 and the first half of
+// O^T of tile t stand the exponents of tile t, spread evenly, between the others the scan of tile t + 1. Heads
+// of 256, whose sums fill the registers, have half of a tile's exponents between its own O^T's products.
+//
+// 8000 rows of 16 heads of 128: 314-335 us by box, 0.93 PFLOP/s of visible products, at 1.9 GHz: the card's power bounds
+// it (work that took 9 % of the cycles away made it 3 % faster), 42 % of the cycles being products. 4095 rows of 32
+// heads of 256 in documents of 700, gated: 89 us, 46 us of which the rows, gates and outputs take from memory at the copy
+// rate; a workgroup spends 7 us on its rows, 19 on 12 tiles, 11 on gates and outputs, and the card holds just two
+// rounds of them. Left out: two sets of 32 rows a wave, which read each operand once for both but leave one wave a
+// SIMD (heads of 128: 317 -> 361 us); three waves a SIMD there (453 -> 477, an earlier form).
 template <int HD, int W, bool CAP, bool SLOPES>
 __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   using G = TileGeom<HD>;
-  constexpr int NT = HD == 256 ? 1 : 2, kRows = 32 * W;
-  constexpr int RD = HD == 256 ? 2 : 4;  // products that an operand is read ahead
-  constexpr int QL = HD == 256 ? 3 : 0;  // pieces of Q that stay in LDS, where the registers hold no more
-  constexpr int kStageKeys = NT * kTileKeys, kVAt = NT * G::kKTile;  // a buffer: K tiles, then V tiles
-  constexpr int kBuffer = kVAt + NT * G::kTile;
-  constexpr int kLoadsAll = 2 * NT * G::kLoads, kMine = kLoadsAll / W;     // 1 KB loads of a stage and tensor
-  constexpr int kBlocks = kMine >= G::kLoads ? kMine / G::kLoads : 1;      // blocks that a wave takes part in
-  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kBuffer];
+  constexpr bool AHEAD = HD <= 128;
+  constexpr int ST = AHEAD ? 2 : 1, kRows = 32 * W, kLead = AHEAD ? kTileKeys : 0;  // keys that K is staged ahead of V
+  constexpr int RD = 4;  // products that an operand is read ahead
+  constexpr int QL = AHEAD ? 0 : 3;  // pieces of Q that stay in LDS, where the registers hold no more
+  constexpr int kStageKeys = ST * kTileKeys, kVAt = ST * G::kKTile;  // a buffer: K tiles, then V tiles
+  constexpr int kBuffer = kVAt + ST * G::kTile;
+  constexpr int kMine = 2 * ST * G::kLoads / W;                        // 1 KB loads of a stage and tensor that a wave makes
+  constexpr int kBlocks = kMine >= G::kLoads ? kMine / G::kLoads : 1;  // blocks that it takes part in
+  constexpr int kPer = kMine < G::kLoads ? kMine : G::kLoads;          // and of each its loads
+  constexpr int kFirst = 2 * G::kLoads / W;                            // of the first tile of K
+  static_assert(kFirst >= 1 && kFirst <= G::kLoads, "a wave loads from one block of the first tile");
+  // Two objects, and two stages written out below: what the loads write is then known not to be what is read, and no
+  // read waits for them.
+  __shared__ __attribute__((aligned(16))) uint8_t buf0[kBuffer], buf1[kBuffer];
   __shared__ __attribute__((aligned(16))) uint8_t q_smem[QL ? W * QL * 1024 : 16];
   __shared__ int wg_lo[W], wg_hi[W];
   const int group = a.heads / a.kvh, R = group * a.t;
@@ -431,9 +452,9 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   const int bkh = (int)blockIdx.x % a.lanes_kvh, kh = bkh % a.kvh, b = bkh / a.kvh, sp = blockIdx.y;
   const int tid = threadIdx.x, wave = uniform(tid / kWave), lane = tid & (kWave - 1);
   const int h = lane >> 5, c = lane & 31;
-  const int r = min(kRows * rg + 32 * wave + c, R - 1);  // rows past R repeat the last one
+  const int row0 = kRows * rg + 32 * wave;  // this wave's first row
+  const int r = min(row0 + c, R - 1);       // rows past R repeat the last one
   const int step = r / group, hq = kh * group + r % group;
-  bf16x8_t q[G::kS - QL];
   u32x4_t qd[G::kS];
   {
     const uint16_t* const qrow = a.q + a.qr.at(b, hq, step) + 8 * h;
@@ -463,42 +484,56 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   // This split's keys alone: its last stage may reach into the next one's.
   row.hi = min(row.hi, end);
   set.hi_min = min(set.hi_min, end);
-  set.hi_max = min(set.hi_max, end);
   hi = min(hi, end);
 
   const float slope2 = SLOPES ? a.slopes[hq] * kLog2e : 0.f;
   const int32_t* const trow = a.table + (int64_t)b * a.table_stride;
   const int last_block = (int)min(a.table_stride, (int64_t)INT32_MAX) - 1;
 
-  // This wave's loads of a stage are [wave kMine, (wave + 1) kMine) of its kLoadsAll, block by block.
+  // Stage s holds V of the tiles from ST s on and K of those kLead further on. This wave's loads of each are
+  // [wave kMine, (wave + 1) kMine) of them, block by block.
   const int g0 = wave * kMine, block0 = g0 / G::kLoads, j0 = g0 % G::kLoads;
   const uint32_t kpiece = (uint32_t)(((lane / G::kP * a.kvh + kh) * HD + (lane % G::kP) * 8) * 2);
   const uint32_t kstep = (uint32_t)(64 / G::kP * a.kvh * HD * 2);  // bytes between loads of a block
-  const uint32_t voff = v_offset<HD>(lane, kh) + (uint32_t)(j0 * 1024);
+  const uint32_t vpiece = v_offset<HD>(lane, kh);
   const int klane = lane / G::kP;
-  int ids[kBlocks];
-  auto blocks = [&](int key0) {
-#pragma unroll
-    for (int x = 0; x < kBlocks; ++x) ids[x] = sload(trow, min(key0 / kAttnBlock + block0 + x, last_block));
+  auto wanted = [&](int at) { return at < hi && at + kAttnBlock > lo; };
+  auto block = [&](int key) { return sload(trow, min(key / kAttnBlock, last_block)); };
+  // Load J of a block of K, into its tile's place: two to a setting of the LDS address, the second one's offset in the
+  // instruction, which counts for both sides. Its lanes' pieces ^ flip of the key's row: the flip of
+  // 16 (block % 2) + key, of which the lane has its own share.
+  auto load_k = [&](rsrc_t src, uint8_t* to, int half, int first, auto j) {
+    const int at = 16 * half + (first + j / 2 * 2) * (64 / G::kP), key = at + j % 2 * (64 / G::kP) + klane;
+    const uint32_t off = (kpiece ^ (uint32_t)(k_flip<HD>(prompt_swap(key)) * 16)) + (uint32_t)(first + j) * kstep;
+    load_lds<j % 2 * 1024>(src, to + k_row<HD>(at), off - j % 2 * 1024u);
   };
-  auto stage = [&](int buf, int key0) {
+  int kid[kBlocks], vid[kBlocks];
+  auto blocks = [&](int key) {
 #pragma unroll
     for (int x = 0; x < kBlocks; ++x) {
-      const int at = key0 + kAttnBlock * (block0 + x);
-      const BlockSource<HD> src(a, uniform(ids[x]), at < hi && at + kAttnBlock > lo);
-      constexpr int kPer = kMine < G::kLoads ? kMine : G::kLoads;
-      const int half = (block0 + x) & 1;
-      uint8_t* const kto = smem + buf + (block0 + x) / 2 * G::kKTile;
-      uint8_t* const vto = smem + buf + kVAt + (block0 + x) * G::kHalf + j0 * 1024;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        // piece ^ flip of the key's row: the flip of 16 (block % 2) + key, of which the lane has its own share
-        const int first = 16 * half + (j0 + j) * (64 / G::kP), key = first + klane;
-        const uint32_t off = (kpiece ^ (uint32_t)(k_flip<HD>(prompt_swap(key)) * 16)) + (uint32_t)(j0 + j) * kstep;
-        load_lds(src.k, kto + k_row<HD>(first), off);
-        load_lds(src.v, vto + j * 1024, voff + 1024u * j);
-      }
+      vid[x] = block(key + kAttnBlock * (block0 + x));
+      kid[x] = block(key + kLead + kAttnBlock * (block0 + x));
     }
+  };
+  // Load J of the 2 kMine of the stage at key: of each block K, then V. What lies past the keys is zeros, unread.
+  rsrc_t from;
+  auto load = [&](uint8_t* to, int key, auto j) {
+    constexpr int x = j / (2 * kPer), i = j % (2 * kPer);
+    const int at = key + kAttnBlock * (block0 + x);
+    if constexpr (i == 0) from = BlockSource<HD>(a, uniform(kid[x]), wanted(at + kLead)).k;
+    if constexpr (i == kPer) from = BlockSource<HD>(a, uniform(vid[x]), wanted(at)).v;
+    if constexpr (i < kPer) {
+      load_k(from, to + (block0 + x) / 2 * G::kKTile, (block0 + x) & 1, j0, std::integral_constant<int, i>{});
+    } else {
+      constexpr int n = (i - kPer) / 4 * 4, m = (i - kPer) % 4;
+      load_lds<m * 1024>(from, to + kVAt + (block0 + x) * G::kHalf + (j0 + n) * 1024, vpiece + 1024u * (j0 + n));
+    }
+  };
+  // The stage at `key` beside product `slot` of the first S of the one before: in one go its loads hold a wave up for
+  // 760 cycles of a stage's 3600 (heads of 128).
+  auto loads = [&](auto slot, auto slots, uint8_t* to, int key) {
+    constexpr int first = (slot * 2 * kMine + slots - 1) / slots, last = ((slot + 1) * 2 * kMine + slots - 1) / slots;
+    static_for<last - first>([&](auto j) { load(to, key, std::integral_constant<int, first + j>{}); });
   };
 
   RowSoft soft{CAP ? 0.f : kNoKey, 0.f};
@@ -513,12 +548,18 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   const uint32_t vat = (uint32_t)(kVAt + c * 32 + (h ^ v_swap(c)) * 16);
 
   uint8_t* const q_mine = q_smem + (wave * QL * 64 + lane) * 16;
-  int key0 = tile0 * kTileKeys, buf = 0;
+  int key0 = tile0 * kTileKeys;
   if (tiles > 0) {
+    if constexpr (AHEAD) {  // the first tile of K, as the last one of a stage before the first
+      const int g = wave * kFirst, x = g / G::kLoads;
+      const BlockSource<HD> src(a, uniform(block(key0 + kAttnBlock * x)), wanted(key0 + kAttnBlock * x));
+      static_for<kFirst>([&](auto j) { load_k(src.k, buf1 + (ST - 1) * G::kKTile, x, g % G::kLoads, j); });
+    }
     blocks(key0);
-    stage(0, key0);
+    static_for<2 * kMine>([&](auto j) { load(buf0, key0, j); });
     blocks(key0 + kStageKeys);
   }
+  bf16x8_t q[G::kS - QL];
 #pragma unroll
   for (int s = 0; s < G::kS; ++s) {
     asm volatile("" : "+v"(qd[s]));  // landed before the loop: its waits count the tiles' loads alone
@@ -527,118 +568,164 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     else
       lds16_store(q_mine + s * 1024, qd[s]);
   }
-  for (; key0 < end; key0 += kStageKeys, buf = kBuffer - buf) {
+
+  TileSoftmax<CAP, SLOPES> soft_tile;
+  u32x4_t p[2], f[RD];
+  const f32x16_t zero = {};
+  auto kfrag = [&](const uint8_t* k, int i) { return lds16(k + (kat ^ (32u * (i & 3))) + 128 * (i >> 2)); };
+  auto vfrag = [&](const uint8_t* v, int i) { return lds16(v + vat + (i % G::kT) * 1024 + (i / G::kT) * G::kHalf); };
+  auto begin = [&](const uint8_t* k) {
+#pragma unroll
+    for (int i = 0; i < RD; ++i) f[i] = kfrag(k, i);
     ring_fence();
-    vmcnt_wait<0>();  // this stage, issued a stage ago
+  };
+  auto qpiece = [&](auto i) {
+    if constexpr (i < QL)
+      return as_bf16x8(lds16(q_mine + i * 1024));
+    else
+      return q[i - QL];
+  };
+  auto rescale = [&](float alpha) {
+    if (!CAP && __ballot(alpha != 1.f) != 0ull) {
+#pragma unroll
+      for (int dt = 0; dt < G::kT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+    }
+    ring_fence();
+  };
+  auto finish = [&](f32x16_t& s, int key) {
+    return soft_tile.finish(a, s, row, slope2, set.whole(key), key, h, soft);
+  };
+  // Exponents [from, to) of a tile's 16.
+  auto exponents = [&](auto from, auto to, const f32x16_t& s) {
+    static_for<to - from>([&](auto j) { soft_tile.template exponent<from + j>(s, p, soft); });
+  };
+  // S^T of the tile at k into sn and O^T of the one at v with the scores sc. `next` (or null): where the K after that
+  // is; `to` (or null): where the next stage goes.
+  auto tile = [&](const uint8_t* k, const uint8_t* v, auto next, const f32x16_t& sc, f32x16_t& sn, auto to) {
+    constexpr bool kNext = !std::is_same_v<decltype(next), std::nullptr_t>;
+    constexpr bool kStage = !std::is_same_v<decltype(to), std::nullptr_t>;
+    constexpr int kSlots = G::kS + G::kT;  // products beside which the exponents stand, two thirds before O^T begins
+    auto beside = [&](auto slot) {
+      if constexpr (kStage) loads(slot, std::integral_constant<int, 2 * G::kS>{}, to, key0 + kStageKeys);
+      if constexpr (slot < kSlots)
+        exponents(std::integral_constant<int, (slot * 16 + kSlots - 1) / kSlots>{},
+                  std::integral_constant<int, ((slot + 1) * 16 + kSlots - 1) / kSlots>{}, sc);
+    };
+    static_for<G::kS>([&](auto i) {
+      sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), qpiece(i), i == 0 ? zero : sn, 0, 0, 0);
+      f[i % RD] = i + RD < G::kS ? kfrag(k, i + RD) : vfrag(v, i + RD - G::kS);
+      beside(i);
+      ring_fence();
+    });
+    soft_tile.begin();
+    static_for<G::kS>([&](auto i) {
+      o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[i / G::kT]), o[i % G::kT], 0, 0, 0);
+      if constexpr (i + RD < G::kS)
+        f[i % RD] = vfrag(v, i + RD);
+      else if constexpr (kNext)
+        f[i % RD] = kfrag(next, i + RD - G::kS);
+      beside(std::integral_constant<int, G::kS + i>{});
+      if constexpr (i >= G::kT) {
+#pragma unroll
+        for (int e = 0; e < 16 / G::kT; ++e) soft_tile.scan(sn[(i - G::kT) * (16 / G::kT) + e]);
+        asm volatile("" : "+v"(soft_tile.top));  // here as well
+      }
+      ring_fence();
+    });
+  };
+  // The stage in `at`; the next one's loads go to `to`.
+  f32x16_t s0, s1;
+  auto stage = [&](uint8_t* at, uint8_t* to) {
+    ring_fence();
+    vmcnt_wait<0>();  // this stage, loaded during the last one, which has been the last to read `to`
     __builtin_amdgcn_s_barrier();
     ring_fence();
-    if (key0 + kStageKeys < end) {
-      stage(kBuffer - buf, key0 + kStageKeys);  // last read a stage ago, before the barrier
-      blocks(key0 + 2 * kStageKeys);
-    }
-    ring_fence();
     if (key0 < lo || key0 + kStageKeys > hi) {  // uniform: V at keys that no row of the workgroup sees becomes zeros
-      zero_unseen<HD>(smem + buf + kVAt, 2 * NT, key0, lo, hi, tid, W * kWave);
+      zero_unseen<HD>(at + kVAt, 2 * ST, key0, lo, hi, tid, W * kWave);
       __syncthreads();
     }
-    if (key0 >= set.hi_max || key0 + kStageKeys <= set.lo_min) continue;  // uniform over the wave
-    const uint8_t* const at = smem + buf;
-    u32x4_t f[RD];
-    auto kfrag = [&](int n, int i) { return lds16(at + n * G::kKTile + (kat ^ (32u * (i & 3))) + 128 * (i >> 2)); };
-    auto vfrag = [&](int n, int i) { return lds16(at + n * G::kTile + vat + (i % G::kT) * 1024 + (i / G::kT) * G::kHalf); };
-    auto rescale = [&](float alpha) {
-      if (__ballot(alpha != 1.f) != 0ull) {
-#pragma unroll
-        for (int dt = 0; dt < G::kT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+    begin(at);
+    if constexpr (AHEAD) {
+      tile(at, at, at + G::kKTile, s0, s1, to);
+      blocks(key0 + 2 * kStageKeys);
+      if (key0 + kTileKeys < end) {
+        rescale(finish(s1, key0 + kTileKeys));
+        tile(at + G::kKTile, at + G::kTile, nullptr, s1, s0, nullptr);
+        if (key0 + kStageKeys < end) rescale(finish(s0, key0 + kStageKeys));
       }
-    };
-    f32x16_t s[NT];
-    u32x4_t p[NT][2];
-    TileSoftmax<CAP, SLOPES> soft_tile;
-    // operands come from LDS RD products ahead, fenced
-#pragma unroll
-    for (int i = 0; i < RD; ++i) f[i] = kfrag(0, i);
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
-    ring_fence();
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int i = 0; i < G::kS; ++i) {
-      const bf16x8_t qi = i < QL ? as_bf16x8(lds16(q_mine + i * 1024)) : q[i < QL ? 0 : i - QL];
-      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), qi, s[0], 0, 0, 0);
-      f[i % RD] = i + RD < G::kS ? kfrag(0, i + RD) : NT == 2 ? kfrag(NT - 1, i + RD - G::kS) : vfrag(0, i + RD - G::kS);
-      ring_fence();
+    } else {  // four operands ahead where no exponents are in the registers yet, two across the softmax (90.0 -> 88.9 us)
+      static_for<G::kS>([&](auto i) {
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), qpiece(i), i == 0 ? zero : s0, 0, 0, 0);
+        if constexpr (i + RD < G::kS) f[i % RD] = kfrag(at, i + RD);
+        loads(i, std::integral_constant<int, G::kS>{}, to, key0 + kStageKeys);
+        ring_fence();
+      });
+      blocks(key0 + 2 * kStageKeys);
+      const float alpha = soft_tile.prepare(a, s0, row, slope2, set.whole(key0), key0, h, soft);
+      f[0] = vfrag(at, 0);
+      f[1] = vfrag(at, 1);
+      exponents(std::integral_constant<int, 0>{}, std::integral_constant<int, 8>{}, s0);
+      rescale(alpha);
+      __builtin_amdgcn_s_setprio(1);
+      static_for<G::kS>([&](auto i) {
+        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[i / G::kT]), o[i % G::kT], 0, 0, 0);
+        if constexpr (i < 2) {
+          f[(2 * i + 2) % RD] = vfrag(at, 2 * i + 2);
+          f[(2 * i + 3) % RD] = vfrag(at, 2 * i + 3);
+        } else if constexpr (i + RD < G::kS) {
+          f[i % RD] = vfrag(at, i + RD);
+        }
+        if constexpr (i < 4) exponents(std::integral_constant<int, 8 + 2 * i>{}, std::integral_constant<int, 10 + 2 * i>{}, s0);
+        ring_fence();
+      });
+      __builtin_amdgcn_s_setprio(0);
     }
-    __builtin_amdgcn_s_setprio(0);
-    if constexpr (NT == 2) {
-      constexpr int kE = 16 / G::kS;  // exponents beside each product
-      const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
-      if (!CAP) rescale(alpha);
+    key0 += kStageKeys;
+  };
+  if constexpr (AHEAD) {
+    if (tiles > 0) {
+      vmcnt_wait<2 * kMine>();  // K of the first tile, the stage behind it may be on its way
+      __builtin_amdgcn_s_barrier();
       ring_fence();
+      const uint8_t* const k = buf1 + (ST - 1) * G::kKTile;
+      begin(k);
       static_for<G::kS>([&](auto i) {
-        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), q[i], s[1], 0, 0, 0);
-        f[i % RD] = i + RD < G::kS ? kfrag(1, i + RD) : vfrag(0, i + RD - G::kS);
-        soft_tile.template exponents<i * kE, kE>(s[0], p[0], soft);
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), qpiece(i), i == 0 ? zero : s0, 0, 0, 0);
+        if (i + RD < G::kS) f[i % RD] = kfrag(k, i + RD);
         ring_fence();
       });
-      // The second tile's maximum raises the first one's sums too, so its product goes into O as it is.
-      const float beta = soft_tile.prepare(a, s[1], row, slope2, set.whole(key0 + kTileKeys), key0 + kTileKeys, h, soft);
+      soft_tile.prepare(a, s0, row, slope2, set.whole(key0), key0, h, soft);  // no sums yet to multiply
       ring_fence();
-      static_for<G::kS>([&](auto i) {
-        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[0][i / G::kT]), o[i % G::kT], 0, 0, 0);
-        f[i % RD] = i + RD < G::kS ? vfrag(0, i + RD) : vfrag(1, i + RD - G::kS);
-        soft_tile.template exponents<i * kE, kE>(s[1], p[1], soft);
-        ring_fence();
-      });
-      if (!CAP) rescale(beta);
-      ring_fence();
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int i = 0; i < G::kS; ++i) {
-        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[1][i / G::kT]), o[i % G::kT], 0, 0, 0);
-        if (i + RD < G::kS) f[i % RD] = vfrag(1, i + RD);
-        ring_fence();
-      }
-      __builtin_amdgcn_s_setprio(0);
-    } else {
-      const float alpha = soft_tile.prepare(a, s[0], row, slope2, set.whole(key0), key0, h, soft);
-      soft_tile.template exponents<0, 8>(s[0], p[0], soft);
-      if (!CAP) rescale(alpha);
-      ring_fence();
-      __builtin_amdgcn_s_setprio(1);
-      static_for<G::kS>([&](auto i) {
-        o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[0][i / G::kT]), o[i % G::kT], 0, 0, 0);
-        if (i + RD < G::kS) f[i % RD] = vfrag(0, i + RD);
-        if (i < 4) soft_tile.template exponents<(i < 4 ? 8 + 2 * i : 8), 2>(s[0], p[0], soft);
-        ring_fence();
-      });
-      __builtin_amdgcn_s_setprio(0);
     }
   }
+  while (key0 < end) {
+    stage(buf0, buf1);
+    if (key0 >= end) break;
+    stage(buf1, buf0);
+  }
   const float l = soft.l + __shfl_xor(soft.l, 32, kWave);
-  const bool real = kRows * rg + 32 * wave + c < R;
+  const bool real = row0 + c < R;
   // o[dt][4 i + e] is channel 32 dt + 8 i + 4 h + e of the row
   if (a.n_split == 1) {
     // Through LDS, half of the channels at a time, into whole rows: a lane holds 8 bytes here and there
     // of its row. A wave's 32 rows are its own; 16-byte pieces (4 floats) at [row][piece ^ row].
     constexpr int kRow = HD * 2, kPieces = HD / 8, kFlip = kPieces - 1;  // bytes and pieces of half a row
-    static_assert(W * 32 * kRow <= 2 * kBuffer, "half of the rows' floats fit the buffers");
+    static_assert(W / 2 * 32 * kRow <= kBuffer, "half of the rows' floats fit the buffers");
     constexpr int kEach = 32 * kPieces / 2 / kWave;  // pieces of 8 channels that a lane stores of a half
     // the gates, all on their way before the first is used: one memory latency for the workgroup's last step
     u32x4_t gates[2 * kEach];
 #pragma unroll
     for (int i = 0; i < 2 * kEach; ++i) {
-      const int at = lane + kWave * (i % kEach), ro = min(kRows * rg + 32 * wave + at / (kPieces / 2), R - 1);
+      const int at = lane + kWave * (i % kEach), ro = min(row0 + at / (kPieces / 2), R - 1);
       gates[i] = gate8(a, b, kh * group + ro % group, ro / group, i / kEach * (HD / 2) + 8 * (at % (kPieces / 2)));
     }
     const float inv = row_inverse(l);
-    float odd = 0.f;  // NaN where some value of the row is not finite
-    uint8_t* const mine = smem + wave * (32 * kRow);
-    __syncthreads();  // the last stage's reads are done
+    float top = 0.f;  // the row's largest magnitude, NaN where a value is
+    uint8_t* const mine = (wave & 1 ? buf1 : buf0) + wave / 2 * (32 * kRow);
+    vmcnt_wait<0>();  // loads into the buffers, zeros behind the last stage, are over,
+    __syncthreads();  // and the reads of it
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
 #pragma unroll
@@ -649,13 +736,13 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
           const f32x16_t& x = o[part * (G::kT / 2) + dt];
           const f32x4_t y = {x[4 * i] * inv, x[4 * i + 1] * inv, x[4 * i + 2] * inv, x[4 * i + 3] * inv};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd = fmaf(y[e], 0.f, odd);
+          for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, fabsf(y[e]));
           *reinterpret_cast<f32x4_t*>(mine + c * kRow + ((piece ^ c) & kFlip) * 16) = y;
         }
       wave_lds_fence();
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        const int at = lane + kWave * i, rl = at / (kPieces / 2), pc = at % (kPieces / 2), ro = kRows * rg + 32 * wave + rl;
+        const int at = lane + kWave * i, rl = at / (kPieces / 2), pc = at % (kPieces / 2), ro = row0 + rl;
         if (ro >= R) continue;
         float y[8];
 #pragma unroll
@@ -668,10 +755,10 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       }
       wave_lds_fence();
     }
-    uint64_t again = __ballot(real && (odd != 0.f || (l < least_sum(a) && row.hi > row.lo)));
+    uint64_t again = __ballot(real && (!(top < INFINITY) || (l < least_sum(a) && row.hi > row.lo)));
     again = (again | again >> 32) & 0xffffffffull;
     while (again != 0ull) {
-      const int rl = uniform(__builtin_ctzll(again)), ro = kRows * rg + 32 * wave + rl;
+      const int rl = uniform(__builtin_ctzll(again)), ro = row0 + rl;
       again &= again - 1ull;
       masked_row_slow<HD>(a, b, kh * group + ro % group, ro / group, lane);
     }
@@ -805,7 +892,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     TileSoftmax<CAP, SLOPES> soft_tile;
     u32x4_t p[2];
     const float alpha = soft_tile.prepare(a, s, row, slope2, set.whole(key0), key0, h, soft);
-    soft_tile.template exponents<0, 16>(s, p, soft);
+    static_for<16>([&](auto i) { soft_tile.template exponent<i>(s, p, soft); });
     if (!CAP && __ballot(alpha != 1.f) != 0ull) {
 #pragma unroll
       for (int dt = 0; dt < G::kT; ++dt)
@@ -964,7 +1051,9 @@ namespace {
 int64_t masked_group_rows(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 int64_t masked_row_groups(int64_t rows) { return (rows + masked_group_rows(rows) - 1) / masked_group_rows(rows); }
 
-// Key splits: as many as bring the workgroups near the device's compute units, of at least 8 tiles each.
+// Key splits: as many as bring the workgroups near what the device holds at once, of at least 8 tiles each. 48 lanes of 2 kv
+// heads of 256 (96 workgroups): one step with a window of 4096, one workgroup a compute unit: 2 splits 82 us, 4 89,
+// 5 87, 8 90; four steps over 8000 keys, two a unit: 5 splits 149 us, 4 153, 6 202, 8 172.
 int masked_splits(int64_t batch, int64_t kvh, int64_t rows, int64_t hd, int64_t keys) {
   const int64_t wgs = std::max<int64_t>(batch * kvh * masked_row_groups(rows), 1);
   const int64_t per_cu = hd == 256 && rows <= 32 ? 1 : 2;
@@ -1067,7 +1156,7 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
   if (gate) a.gr = {gate_strides[0], gate_strides[1], gate_strides[2]};
   a.k_pool = k_pool;
   a.v_pool = v_pool;
-  a.pool_rows = pool_rows;
+  a.pool_blocks = (uint32_t)std::min<int64_t>(pool_rows / kAttnBlock, (int64_t)1 << 31);
   a.table = block_table;
   a.table_stride = table_stride;
   a.base = base_pos;
