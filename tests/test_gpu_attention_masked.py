@@ -9,6 +9,7 @@ log2 at 2^-23 each, and the exponential: 3e-4 of a weight is allowed, twice for 
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -103,6 +104,24 @@ def test_against_the_oracle(dev, heads, kvh, hd, t, base, kind) -> None:
         pos = b0[:, None] + torch.arange(t)
         none = kw["first"] > pos
         assert not got[none].any()
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_any_mix(dev, seed) -> None:
+    """Sizes, groups and masks drawn together."""
+    rng, g = random.Random(seed), torch.Generator().manual_seed(seed)
+    hd, kvh, group = (64, 128, 256)[seed % 3], rng.choice([1, 2, 3, 5]), rng.choice([1, 2, 3, 5, 8, 16, 33, 64])
+    heads, b = kvh * group, rng.choice([1, 2, 3])
+    t = max(1, min(rng.choice([1, 2, 5, 17, 64, 257]), 4000 // (heads * b)))
+    base = [rng.choice([0, 15, 16, 33, rng.randrange(2000)]) for _ in range(b)]
+    q, k, v, table, b0 = case(seed, b, t, heads, kvh, hd, base)
+    pos = b0[:, None] + torch.arange(t)
+    mixed = {"softcap": rng.choice([5.0, 50.0, 80.0]), "window": rng.choice([1, 31, 33, 64, 1000]),
+             "slopes": torch.rand(heads, generator=g) * rng.choice([0.1, 1.0, -0.05]),
+             "prefix": b0 + torch.randint(-3, t + 3, (b,), generator=g),
+             "first": (pos - torch.randint(-2, 80, (b, t), generator=g)).int(),
+             "gate": torch.randn(b, t, heads, hd, generator=g).bfloat16()}  # fmt: skip
+    check(dev, q, k, v, table, b0, hd**-0.5, **{n: x for n, x in mixed.items() if rng.random() < 0.5})
 
 
 @pytest.mark.parametrize("heads,kvh,hd,t,base", [(32, 2, 256, 1, [500]), (32, 2, 256, 40, [9]), (16, 4, 128, 12, [90])])
