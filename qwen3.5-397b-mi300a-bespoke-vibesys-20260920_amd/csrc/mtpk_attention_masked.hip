@@ -85,16 +85,15 @@ __device__ inline RowKeys masked_row(const MaskedArgs& a, int b, int s) {
   return RowKeys{(int)pos, (int)lo, (int)hi};
 }
 
+// Over the 16 lanes of a row by DPP, then the two rows of a half.
 __device__ inline int wave_min_i(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, kWave));
-  return uniform(v);
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, false));
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, false));
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, false));
+  v = min(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, false));
+  return min(uniform(v), __builtin_amdgcn_readlane(v, 16));
 }
-__device__ inline int wave_max_i(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, kWave));
-  return uniform(v);
-}
+__device__ inline int wave_max_i(int v) { return -1 - wave_min_i(-1 - v); }
 
 // What 32 rows (the two halves of a wave hold them twice) see together.
 struct RowSet {
@@ -783,14 +782,15 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
 
 // ---------------------------------------------------------------- few rows
 //
-// Up to 32 rows of a (lane, kv head) to a workgroup; its four waves take every fourth tile each, over
+// Up to 32 rows of a (lane, kv head) to a workgroup; its W waves take every W-th tile each, over
 // all of the rows, and stage it for themselves alone: no barrier until their results are merged. K's
-// place is loaded again as soon as the first product has read it, V's after the second.
-template <int HD, bool CAP, bool SLOPES>
-__global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
+// place is loaded again as soon as the first product has read it, V's after the second. 48 lanes of 2 kv heads of 256,
+// windows of 4096: 81 us with the merge, 5.2 TB/s in this kernel; 65,000 and 31,000 keys of 4 kv heads of 128: 50 us.
+template <int HD, int W, bool CAP, bool SLOPES>
+__global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
   using G = TileGeom<HD>;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[4][G::kKTile + G::kTile];  // a wave's K and V tile
-  __shared__ float ml[4][32][2];
+  __shared__ __attribute__((aligned(16))) uint8_t smem[W][G::kKTile + G::kTile];  // a wave's K and V tile
+  __shared__ float ml[W][32][2];
   __shared__ int again[32];
   const int group = a.heads / a.kvh, R = group * a.t;
   const int bkh = blockIdx.x, kh = bkh % a.kvh, b = bkh / a.kvh, sp = blockIdx.y;
@@ -849,7 +849,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   const uint32_t kat = (uint32_t)(k_row<HD>(prompt_swap(c)) + ((h ^ k_flip<HD>(c)) * 16));
   const uint32_t vat = (uint32_t)(c * 32 + (h ^ v_swap(c)) * 16);
-  constexpr int kStep = 4 * kTileKeys;
+  constexpr int kStep = W * kTileKeys;
   const int end = (tile0 + tiles) * kTileKeys;
   int key0 = (tile0 + wave) * kTileKeys;
   int b0 = 0, b1 = 0;
@@ -926,7 +926,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
       b1 = block(key0 + 2 * kStep, 1);
     }
   }
-  // The four waves' results through their own tiles' LDS: 32 rows of HD floats.
+  // The waves' results through their own tiles' LDS: 32 rows of HD floats.
   const float l = soft.l + __shfl_xor(soft.l, 32, kWave);
   constexpr int kRow = HD * 4, kFlip = HD / 4 - 1;
 #pragma unroll
@@ -943,17 +943,17 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
     if (wave == 0) again[c] = 0;
   }
   __syncthreads();
-  for (int i = tid; i < 32 * G::kP; i += 256) {
+  for (int i = tid; i < 32 * G::kP; i += W * kWave) {
     const int rl = i / G::kP, pc = i % G::kP;
     if (rl >= R) break;
     const u32x4_t gate = a.n_split == 1 ? gate8(a, b, kh * group + rl % group, rl / group, 8 * pc) : zero16();
     float m = kNoKey, sum = 0.f, y[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w][rl][0]);
+    for (int w = 0; w < W; ++w) m = fmaxf(m, ml[w][rl][0]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float wt = __builtin_amdgcn_exp2f(ml[w][rl][0] - m);
       sum = fmaf(ml[w][rl][1], wt, sum);
 #pragma unroll
@@ -986,7 +986,7 @@ __global__ __launch_bounds__(256, 1) void k_masked_few(MaskedArgs a) {
   }
   if (a.n_split > 1) return;
   __syncthreads();
-  for (int rl = wave; rl < min(R, 32); rl += 4) {
+  for (int rl = wave; rl < min(R, 32); rl += W) {
     if (uniform(again[rl]) != 0) masked_row_slow<HD>(a, b, kh * group + rl % group, rl / group, lane);
   }
 }
@@ -1056,11 +1056,28 @@ int64_t masked_row_groups(int64_t rows) { return (rows + masked_group_rows(rows)
 // 5 87, 8 90; four steps over 8000 keys, two a unit: 5 splits 149 us, 4 153, 6 202, 8 172.
 int masked_splits(int64_t batch, int64_t kvh, int64_t rows, int64_t hd, int64_t keys) {
   const int64_t wgs = std::max<int64_t>(batch * kvh * masked_row_groups(rows), 1);
-  const int64_t per_cu = hd == 256 && rows <= 32 ? 1 : 2;
+  const int64_t per_cu = hd > 64 && rows <= 32 ? 1 : 2;  // what LDS holds
   const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
   int64_t n = std::min<int64_t>(device_cu_count() * per_cu / wgs, tiles / 8);
   n = std::min<int64_t>(n, kMaskedSplits);
   return n < 1 ? 1 : (int)n;
+}
+
+// Up to 32 rows: eight waves a workgroup while the lanes' workgroups stay within the compute units, where more of a
+// lane's keys are on their way at once and fewer splits are left to merge (one lane of 300 keys, heads of 64: 7.4 -> 6.3
+// us; 48 of 4000 keys, 4 kv heads of 128: 79.5 -> 72 us); four, and two workgroups a unit, for more of them (48 of 500
+// keys, 8 kv heads: 20.3 us with four, 23.9 with eight). The tiles of eight waves of 256 channels do not fit LDS.
+bool masked_eight(int64_t lanes_kvh, int64_t hd) { return hd < 256 && lanes_kvh <= device_cu_count(); }
+
+template <int HD, bool CAP, bool SLOPES>
+void masked_few_launch(const MaskedArgs& a, dim3 grid, hipStream_t st) {
+  if constexpr (HD < 256) {
+    if (masked_eight(a.lanes_kvh, HD)) {
+      hipLaunchKernelGGL((k_masked_few<HD, 8, CAP, SLOPES>), grid, dim3(512), 0, st, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((k_masked_few<HD, 4, CAP, SLOPES>), grid, dim3(256), 0, st, a);
 }
 
 template <int HD, bool CAP, bool SLOPES>
@@ -1068,7 +1085,7 @@ int masked_launch(const MaskedArgs& a, int64_t batch, hipStream_t st) {
   const int64_t rows = (int64_t)(a.heads / a.kvh) * a.t;
   const dim3 grid((unsigned)(batch * a.kvh * a.row_groups), (unsigned)a.n_split);
   if (rows <= 32)
-    hipLaunchKernelGGL((k_masked_few<HD, CAP, SLOPES>), grid, dim3(256), 0, st, a);
+    masked_few_launch<HD, CAP, SLOPES>(a, grid, st);
   else if (rows <= 64)
     hipLaunchKernelGGL((k_masked_rows<HD, 2, CAP, SLOPES>), grid, dim3(128), 0, st, a);
   else
