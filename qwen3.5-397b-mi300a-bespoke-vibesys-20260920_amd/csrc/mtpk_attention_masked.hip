@@ -25,6 +25,7 @@
 // makes all of them NaN (0 times infinity): such rows are found at the end and done again one by one.
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "mtpk_attention_common.h"
@@ -1051,23 +1052,30 @@ namespace {
 int64_t masked_group_rows(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 int64_t masked_row_groups(int64_t rows) { return (rows + masked_group_rows(rows) - 1) / masked_group_rows(rows); }
 
-// Key splits: as many as bring the workgroups near what the device holds at once, of at least 8 tiles each. 48 lanes of 2 kv
-// heads of 256 (96 workgroups): one step with a window of 4096, one workgroup a compute unit: 2 splits 82 us, 4 89,
-// 5 87, 8 90; four steps over 8000 keys, two a unit: 5 splits 149 us, 4 153, 6 202, 8 172.
-int masked_splits(int64_t batch, int64_t kvh, int64_t rows, int64_t hd, int64_t keys) {
-  const int64_t wgs = std::max<int64_t>(batch * kvh * masked_row_groups(rows), 1);
-  const int64_t per_cu = hd > 64 && rows <= 32 ? 1 : 2;  // what LDS holds
-  const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
-  int64_t n = std::min<int64_t>(device_cu_count() * per_cu / wgs, tiles / 8);
-  n = std::min<int64_t>(n, kMaskedSplits);
-  return n < 1 ? 1 : (int)n;
-}
-
 // Up to 32 rows: eight waves a workgroup while the lanes' workgroups stay within the compute units, where more of a
 // lane's keys are on their way at once and fewer splits are left to merge (one lane of 300 keys, heads of 64: 7.4 -> 6.3
 // us; 48 of 4000 keys, 4 kv heads of 128: 79.5 -> 72 us); four, and two workgroups a unit, for more of them (48 of 500
 // keys, 8 kv heads: 20.3 us with four, 23.9 with eight). The tiles of eight waves of 256 channels do not fit LDS.
 bool masked_eight(int64_t lanes_kvh, int64_t hd) { return hd < 256 && lanes_kvh <= device_cu_count(); }
+
+// Key splits. At most what the device holds at once: 48 lanes of 2 kv heads of 256 (96 workgroups), one step with a
+// window of 4096, one workgroup a compute unit: 2 splits 82 us, 4 89, 8 90; four steps over 8000 keys, two a unit: 5 splits
+// 149 us, 4 153, 6 202. At most sqrt(32 tiles / workgroups): a split's tiles get fewer with each, but its start, its
+// partial sums and their merge are there for every workgroup (8 of these lanes, four steps over 1000 keys: 4 splits
+// 21.6 us, 8 20.1, 16 22.0; 24 lanes: 4 24.1, 6 23.6, 12 35). And some tiles for each: with up to 32 rows 4 for eight waves,
+// 3 for four, and none split below 3 tiles a wave (one lane, heads of 64: 700 keys 7.3 us whole, 7.7 as 4; 1500 keys 10.2
+// whole, 8.4 as 5, 7.7 as 12); else 2 (one lane, four steps over 700 keys: whole 33 us, 2 splits 22.6, 8 13.2, 12 12.4).
+int masked_splits(int64_t batch, int64_t kvh, int64_t rows, int64_t hd, int64_t keys) {
+  const int64_t wgs = std::max<int64_t>(batch * kvh * masked_row_groups(rows), 1);
+  const int64_t per_cu = hd > 64 && rows <= 32 ? 1 : 2;  // what LDS holds
+  const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
+  const int64_t waves = masked_eight(batch * kvh, hd) ? 8 : 4;
+  if (rows <= 32 && tiles <= 3 * waves) return 1;
+  int64_t n = std::min<int64_t>(device_cu_count() * per_cu / wgs, tiles / (rows > 32 ? 2 : waves == 8 ? 4 : 3));
+  n = std::min<int64_t>(n, (int64_t)std::sqrt(32. * (double)tiles / (double)wgs));
+  n = std::min<int64_t>(n, kMaskedSplits);
+  return n < 1 ? 1 : (int)n;
+}
 
 template <int HD, bool CAP, bool SLOPES>
 void masked_few_launch(const MaskedArgs& a, dim3 grid, hipStream_t st) {
