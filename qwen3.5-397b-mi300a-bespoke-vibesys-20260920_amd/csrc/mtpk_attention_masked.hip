@@ -621,6 +621,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     });
     soft_tile.begin();
     static_for<G::kS>([&](auto i) {
+      if constexpr (i == G::kT) __builtin_amdgcn_s_setprio(1);  // few instructions beside these
       o[i % G::kT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(f[i % RD]), as_bf16x8(p[i / G::kT]), o[i % G::kT], 0, 0, 0);
       if constexpr (i + RD < G::kS)
         f[i % RD] = vfrag(v, i + RD);
@@ -634,6 +635,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       }
       ring_fence();
     });
+    __builtin_amdgcn_s_setprio(0);
   };
   // The stage in `at`; the next one's loads go to `to`.
   f32x16_t s0, s1;
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
         } else if constexpr (i + RD < G::kS) {
           f[i % RD] = vfrag(at, i + RD);
         }
-        if constexpr (i < 4) exponents(std::integral_constant<int, 8 + 2 * i>{}, std::integral_constant<int, 10 + 2 * i>{}, s0);
+        if constexpr (i < 8) exponents(std::integral_constant<int, 8 + i>{}, std::integral_constant<int, 9 + i>{}, s0);
         ring_fence();
       });
       __builtin_amdgcn_s_setprio(0);
