@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import _mtpk
 import attention
 import verify_model as vm
 
@@ -88,6 +89,15 @@ def test_host_ids_are_refused_in_a_capture(dev) -> None:
             attention.copy_blocks(pools, [1], [5])
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(pools, _want(before, src, dst, 8)))
+
+
+def test_stream_handles(dev) -> None:
+    """The current stream's handle, of a device with and without an index."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for device in (torch.device("cuda"), torch.device("cuda", torch.cuda.current_device())):
+            assert _mtpk.stream_of(device) == stream.cuda_stream
+        assert _mtpk.stream_for(torch.empty(1, device=dev)) == stream.cuda_stream
 
 
 def test_offsets_past_four_gigabytes(dev) -> None:

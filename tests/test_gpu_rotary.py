@@ -253,7 +253,8 @@ def test_rotate_to_cache_refuses(dev) -> None:
     for kw in ({"q": q.float()}, {"k": k[:, :2]}, {"v": v[..., :32]}, {"k_pool": kp[:8]}, {"v_pool": vp[:-1]},
                {"v_pool": vp.transpose(2, 3)}, {"block_table": table[:1]}, {"block_table": table.float()},
                {"base_pos": base[:1]}, {"rates": rates.float()}, {"k": k[:, :, :1], "v": v[:, :, :1]},
-               {"keep": torch.ones(2, 3, device=dev)}, {"keep": torch.ones(3, 2, dtype=torch.bool, device=dev)},
+               {"keep": torch.ones(2, 3, device=dev)}, {"keep": torch.ones(2, 3, device=dev, dtype=torch.int8)},
+               {"keep": torch.ones(3, 2, dtype=torch.bool, device=dev)},
                {"positions": torch.zeros(2, 3, device=dev)}, {"q_norm": torch.zeros(32, device=dev)},
                {"q_norm": torch.zeros(64, device=dev), "k_norm": torch.zeros(64, device=dev).bfloat16()}):
         with pytest.raises(ValueError):
