@@ -644,7 +644,7 @@ int mtpk_rotate(const void* x, int dtype, const int64_t* x_strides, int64_t toke
                 const double* rates, int rot_dim, int interleaved, float magnitude, void* out,
                 const int64_t* out_strides, void* stream);
 
-/* The q and k heads of this round's rows normed and rotated as above, k and v into the paged caches, in
+/* The q and k heads of a verify step's rows normed and rotated as above, k and v into the paged caches, in
  * one launch (mtpk_rownorm of q, of k, and mtpk_kv_write, for a rotation without tables). q, k, v and out
  * bf16: element d of (lane b, head h, step s) at b * strides[0] + h * strides[1] + s * strides[2] + d
  * (three int64 strides each, multiples of 8; 16-byte aligned). q_norm, k_norm (norm_dtype f32 | bf16
