@@ -379,7 +379,7 @@ class BlockTables:
     shuffled order so that a lane's physical rows are not contiguous.
 
     A block may be held by several lanes (`fork`): it goes back to the free ones when the last of them
-    lets go of it. `fork` and `compact` return the block copies that they ask for, as `(src, dst)` lists
+    lets go of it. `fork`, `trim` and `compact` return the block copies that they ask for, as `(src, dst)` lists
     for `attention.copy_blocks` over every pool that is read through these tables; the tables themselves
     are written at once, so the copies come before the next read or write through them.
     """
@@ -456,18 +456,33 @@ class BlockTables:
             elif left == 0:
                 self._free.append(block)
 
-    def trim(self, lane: int, length: int) -> None:
-        """Let go of the blocks of lane `lane` past its first `length` positions."""
+    def trim(self, lane: int, length: int) -> tuple[list[int], list[int]]:
+        """Let go of the blocks of lane `lane` past its first `length` positions. A last kept block that is
+        then partly filled, and that another lane holds too, is replaced by one of the lane's own, so that its
+        next positions are not written into the other lane's. Returns that block's copy, at most one
+        `(src, dst)` pair."""
         if length < 0:
             raise ValueError(f"lane {lane}: cannot keep {length} positions")
         need = (length + self.block_size - 1) // self.block_size
         have = self.host[lane]
-        if need >= len(have):
-            return
-        self._let_go(have[need:])
-        self.table[lane, need : len(have)] = 0
+        if need > len(have):
+            return [], []
+        gone = have[need:]
+        shared = length % self.block_size > 0 and have[need - 1] in self._holders
+        if shared and not self._free and all(block in self._holders for block in gone):
+            raise ValueError("no free block for the lane's last one")
+        if gone:
+            self.table[lane, need : len(have)] = 0
+        self._let_go(gone)
         del have[need:]
         self.held_positions[lane] = need * self.block_size
+        if not shared:
+            return [], []
+        old, own = have[-1], self._free.pop()
+        self.table[lane, need - 1] = own
+        self._let_go([old])
+        have[-1] = own
+        return [old], [own]
 
     def fork(self, src: int, dst: int, length: int) -> tuple[list[int], list[int]]:
         """Lane `dst`, which holds nothing, continues after the first `length` positions of lane `src`: it

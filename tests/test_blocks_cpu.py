@@ -126,6 +126,85 @@ def test_any_order_keeps_every_lanes_positions() -> None:
                 assert k[rows, 0, 0].tolist() == want and v[rows // 16, 0, 1, rows % 16].tolist() == [-x for x in want]
 
 
+def test_trim_inside_a_shared_block_takes_one_of_its_own() -> None:
+    """Lanes that share a block, one of them cut back into it: its next positions are its own."""
+    for grown, keep in ((64, 40), (64, 63), (48, 40), (33, 7)):  # the last one with blocks between, and none let go
+        t = _tables()
+        t.grow(0, grown)
+        assert t.fork(0, 1, grown // 16 * 16) == ([], [])
+        before = list(t.host[0])
+        src, dst = t.trim(1, keep)
+        last = keep // 16
+        assert src == [before[last]] and dst == [t.host[1][last]] and dst[0] not in before
+        assert t.host[0] == before and t.host[1][:last] == before[:last]
+        _invariants(t)
+        t.grow(1, keep + 1)
+        rows = t.physical_rows(torch.tensor([0, 1]), torch.tensor([[keep], [keep]]))
+        assert int(rows[0, 0]) != int(rows[1, 0])
+        assert t.trim(1, keep) == ([], [])  # its own by now
+        assert t.trim(0, keep) == ([], [])  # the source holds it alone
+        _invariants(t)
+    t = _tables()
+    t.grow(0, 32)
+    t.fork(0, 1, 32)
+    assert t.trim(1, 16) == ([], []) and t.host[1] == t.host[0][:1]  # whole blocks stay shared
+    _invariants(t)
+
+
+def test_trim_inside_a_shared_block_without_a_free_one() -> None:
+    t = _tables(lanes=3, max_seq=64)
+    t.grow(0, 48)
+    t.fork(0, 1, 48)
+    t._free.clear()
+    before, table = [list(h) for h in t.host], t.table.clone()
+    with pytest.raises(ValueError):
+        t.trim(1, 20)
+    assert t.host == before and torch.equal(t.table, table) and len(t._holders) == 3
+    t = _tables(lanes=3, max_seq=64)
+    t.grow(0, 48)
+    t.fork(0, 1, 32)
+    t.grow(1, 48)  # a third block of its own, which the cut gives back before it needs one
+    t._free.clear()
+    own = t.host[1][2]
+    assert t.trim(1, 20) == ([t.host[0][1]], [own]) and t.host[1] == [t.host[0][0], own]
+
+
+def test_any_order_with_cuts_inside_blocks_keeps_every_lanes_positions() -> None:
+    """As above, with cuts at any position: what a lane writes after one is read by no other lane."""
+    for seed in range(4):
+        rng = random.Random(seed)
+        t = _tables(lanes=6, seed=seed)
+        k, v = torch.zeros(t.rows, 1, 2), torch.zeros(t.n_blocks, 1, 2, 16)
+        kept = [[] for _ in range(6)]
+        stamp = 0
+        for _ in range(400):
+            lane, other = rng.randrange(6), rng.randrange(6)
+            act = rng.choice(("write", "write", "fork", "trim", "trim", "compact"))
+            if act == "write" and len(kept[lane]) < 150:
+                n = rng.randint(1, 9)
+                t.grow(lane, len(kept[lane]) + n)
+                for _ in range(n):
+                    stamp += 1
+                    row = int(t.physical_rows(torch.tensor([lane]), torch.tensor([[len(kept[lane])]]))[0, 0])
+                    k[row], v[row // 16, :, :, row % 16] = stamp, -stamp
+                    kept[lane].append(stamp)
+            elif act == "fork" and lane != other:
+                t.release(other)
+                n = rng.randint(0, len(kept[lane]))
+                attention.copy_blocks([k, v], *t.fork(lane, other, n))
+                kept[other] = kept[lane][:n]
+            elif act == "trim":
+                n = rng.randint(0, len(kept[lane]))
+                attention.copy_blocks([k, v], *t.trim(lane, n))
+                kept[lane] = kept[lane][:n]
+            elif act == "compact":
+                attention.copy_blocks([k, v], *t.compact())
+            _invariants(t)
+            for j, want in enumerate(kept):
+                rows = t.physical_rows(torch.tensor([j]), torch.arange(len(want))[None])[0]
+                assert k[rows, 0, 0].tolist() == want and v[rows // 16, 0, 1, rows % 16].tolist() == [-x for x in want]
+
+
 def test_model_fork_and_compact_on_the_cpu() -> None:
     """A forked slot steps as its source does; a compaction in between changes nothing."""
     import dataclasses
