@@ -708,14 +708,18 @@ class Model:
         self.hidden_cache[lane].zero_()
 
     def caches(self, *more: dict) -> list[torch.Tensor]:
-        """The K and V pools of the attention layers, and of `more` (an MTP head's `pool`)."""
+        """The K and V pools of the attention layers, of the attached MTP head, and of `more`, each once."""
         own = [p for ty, p in zip(self.cfg.layer_types, self.pool) if ty == ATTN]
-        return [p[name] for p in (*own, *more) for name in ("k", "v")]
+        if self.mtp is not None:
+            own.append(self.mtp.pool)
+        held = {id(p[name]): p[name] for p in (*own, *more) for name in ("k", "v")}
+        return list(held.values())
 
     def fork(self, src: int, dst: int, length: int, *more: dict) -> None:
         """Slot `dst`, which is reset, becomes a second continuation of slot `src` after its `length`
         committed positions: blocks shared (`BlockTables.fork`), its last block, DeltaNet state and cached
-        hidden copied. `more`: pools beside the layers' that are read through the same tables."""
+        hidden copied. `more`: pools beside the layers' and the attached MTP head's that are read through the
+        same tables (the `pool` of a head that only a runner knows)."""
         pairs = self.blocks.fork(src, dst, length)
         if pairs[0]:
             attention.copy_blocks(self.caches(*more), *pairs, self.cfg.block_size)
@@ -726,7 +730,8 @@ class Model:
         self.hidden_cache[dst].copy_(self.hidden_cache[src])
 
     def compact(self, *more: dict) -> int:
-        """Move the held cache blocks to the pools' front (`BlockTables.compact`); returns how many moved."""
+        """Move the held cache blocks to the pools' front (`BlockTables.compact`); returns how many moved.
+        `more` as in `fork`."""
         src, dst = self.blocks.compact()
         if src:
             attention.copy_blocks(self.caches(*more), src, dst, self.cfg.block_size)

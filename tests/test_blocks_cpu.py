@@ -11,6 +11,7 @@ import torch
 import _mtpk
 import attention
 import verify_model as vm
+from tests import model_helpers
 
 
 def _tables(lanes=5, max_seq=160, seed=0):
@@ -229,6 +230,42 @@ def test_model_fork_and_compact_on_the_cpu() -> None:
     b = step(1, torch.tensor([[7, 1]]), 6)
     assert torch.equal(a, b)
     assert not torch.equal(step(0, torch.tensor([[4]]), 8), step(1, torch.tensor([[6]]), 8))
+
+
+def _slot_equal(model, a, b, length):
+    return all(torch.equal(x, y) for x, y in zip(model_helpers.slot_state(model, a, length),
+                                                 model_helpers.slot_state(model, b, length), strict=True))
+
+
+def test_model_fork_and_compact_take_the_attached_heads_cache() -> None:
+    """A fork inside a block and a compaction, with an MTP head attached: the head's rows and the next rounds'
+    tokens are the source's."""
+    import mtp
+
+    model = model_helpers.build(k=2, lanes=4)
+    ids = model_helpers.prompts(1, 21)[0]
+    model.prefill(2, model_helpers.prompts(1, 40, seed=6)[0])  # blocks that the compaction finds free
+    token = int(model.argmax(model.prefill(0, ids)[None])[0])
+    model.fork(0, 1, 21)
+    assert _slot_equal(model, 0, 1, 21)
+    model.reset(2)
+    before = [x.clone() for x in model_helpers.slot_state(model, 0, 21)]
+    assert model.compact() > 0
+    assert all(torch.equal(x, y) for x, y in zip(before, model_helpers.slot_state(model, 0, 21), strict=True))
+    assert _slot_equal(model, 0, 1, 21)
+    drafts = [mtp.draft(model, model.mtp, model.hidden_cache[[lane]], [token], [lane], [21]) for lane in (0, 1)]
+    assert drafts[0] == drafts[1]
+    rounds = [mtp.speculative_decode(model, [lane], [token], [21]) for lane in (0, 1)]
+    assert rounds[0] == rounds[1] and _slot_equal(model, 0, 1, 21 + len(rounds[0][0]))
+
+
+def test_caches_name_each_pool_once() -> None:
+    model = model_helpers.build()
+    pools = model.caches()
+    assert any(p is model.mtp.pool["k"] for p in pools) and any(p is model.mtp.pool["v"] for p in pools)
+    other = {"k": torch.zeros(1), "v": torch.zeros(1)}
+    assert [id(p) for p in model.caches(model.mtp.pool, other)] == [id(p) for p in (*pools, other["k"], other["v"])]
+    assert len({p.data_ptr() for p in pools}) == len(pools) == 2 * (1 + model.cfg.layer_types.count(vm.ATTN))
 
 
 def test_copy_blocks_on_the_cpu_and_its_refusals() -> None:

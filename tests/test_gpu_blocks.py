@@ -9,6 +9,7 @@ import torch
 import _mtpk
 import attention
 import verify_model as vm
+from tests import model_helpers
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +142,21 @@ def test_a_forked_slot_steps_as_its_source(dev) -> None:
     assert model.compact() > 0
     assert torch.equal(step(2, [7, 1], 21), a)
     assert not torch.equal(step(0, [4], 23), step(2, [6], 23))
+
+
+def test_a_forked_slot_takes_the_attached_heads_cache(dev) -> None:
+    """A fork inside a block and a compaction, with an MTP head attached: its rows and the next round's tokens
+    are the source's."""
+    import mtp
+
+    model = model_helpers.build(dev, k=2, lanes=4)
+    token = int(model.argmax(model.prefill(0, model_helpers.prompts(1, 21)[0])[None])[0])
+    model.prefill(2, model_helpers.prompts(1, 40, seed=6)[0])
+    model.fork(0, 1, 21)
+    model.reset(2)
+    before = [x.clone() for x in model_helpers.slot_state(model, 0, 21)]
+    assert model.compact() > 0
+    for lane in (0, 1):
+        assert all(torch.equal(x, y) for x, y in zip(before, model_helpers.slot_state(model, lane, 21), strict=True))
+    rounds = [mtp.speculative_decode(model, [lane], [token], [21]) for lane in (0, 1)]
+    assert rounds[0] == rounds[1]
