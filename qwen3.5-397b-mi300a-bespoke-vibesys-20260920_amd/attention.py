@@ -200,6 +200,24 @@ def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
                                                  slopes, prefix, first, gate, _mtpk.stream_for(q))
 
 
+def _not_captured(device: torch.device) -> None:
+    if device.type == "cuda":
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("host ids cannot be part of a graph: give src and dst on the device")
+
+
+def check_pools(pools: list[torch.Tensor], block: int = BLOCK) -> int:
+    """Number of blocks of the pools, after every check that `copy_blocks` makes of them and of the moment when
+    it is called with host ids (`ValueError`): for callers that change block tables before the copies."""
+    n_blocks = _mtpk.native().pool_blocks(pools, block)
+    _not_captured(pools[0].device)
+    for p in pools:
+        if p.is_cuda and (p.numel() // n_blocks * p.element_size() % 16 or p.data_ptr() % 16):
+            raise ValueError("blocks must be of a multiple of 16 bytes, and pools start on 16 bytes")
+    return n_blocks
+
+
 def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None:
     """Block `dst[i]` of every pool becomes block `src[i]` of it, in one launch (`mtpk_copy_blocks`): K pools
     `[rows, kv_heads, hd]` and V pools `[rows / block, kv_heads, hd, block]` of one cache's layers.
@@ -222,8 +240,7 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
         raise ValueError("src and dst must be of one length")
     if src.numel() == 0:
         return
-    if pools[0].is_cuda and torch.cuda.is_current_stream_capturing():
-        raise ValueError("host ids cannot be part of a graph: give src and dst on the device")
+    _not_captured(pools[0].device)
     if int(min(src.min(), dst.min())) < 0 or int(max(src.max(), dst.max())) >= n_blocks:
         raise ValueError(f"block ids must lie in [0, {n_blocks})")
     taken = torch.bincount(dst, minlength=n_blocks)

@@ -498,37 +498,40 @@ class BlockTables:
         if part and not self._free:
             raise ValueError("no free block for the fork's last one")
         mine = self.host[src][:whole]
-        pairs: tuple[list[int], list[int]] = ([], [])
-        for block in mine:
-            self._holders[block] = self._holders.get(block, 1) + 1
-        if part:
-            pairs[0].append(self.host[src][whole])
-            pairs[1].append(self._free.pop())
-            mine.append(pairs[1][0])
-        self.host[dst] = mine
-        self.held_positions[dst] = need * self.block_size
+        pairs = ([self.host[src][whole]], [self._free[-1]]) if part else ([], [])
         if whole:
             self.table[dst, :whole] = self.table[src, :whole]
         if part:
             self.table[dst, whole] = pairs[1][0]
+        for block in mine:
+            self._holders[block] = self._holders.get(block, 1) + 1
+        if part:
+            mine.append(self._free.pop())
+        self.host[dst] = mine
+        self.held_positions[dst] = need * self.block_size
         return pairs
+
+    def moves(self) -> tuple[list[int], list[int]]:
+        """The moves that `compact` would make, as `(src, dst)` lists."""
+        held = sorted({block for have in self.host for block in have})
+        low = set(range(1, len(held) + 1))
+        return [block for block in held if block not in low], sorted(low.difference(held))
 
     def compact(self) -> tuple[list[int], list[int]]:
         """Move every held block to the lowest ids, `1 ..` their count, so that the free ones are the pools'
         tail: returns the moves as `(src, dst)` lists (no block is in both) and writes the tables."""
-        held = sorted({block for have in self.host for block in have})
-        low = set(range(1, len(held) + 1))
-        src = [block for block in held if block not in low]
-        dst = sorted(low.difference(held))
+        src, dst = self.moves()
         to = dict(zip(src, dst, strict=True))
-        self.host = [[to.get(block, block) for block in have] for have in self.host]
-        self._holders = {to.get(block, block): n for block, n in self._holders.items()}
-        self._free = list(range(self.n_blocks - 1, len(held), -1))  # the lowest is handed out first
+        host = [[to.get(block, block) for block in have] for have in self.host]
         if src:
             table = torch.zeros(self.lanes, self.max_blocks, dtype=torch.int32)
-            for lane, have in enumerate(self.host):
+            for lane, have in enumerate(host):
                 table[lane, : len(have)] = torch.tensor(have, dtype=torch.int32)
             self.table.copy_(table)
+        self.host = host
+        self._holders = {to.get(block, block): n for block, n in self._holders.items()}
+        held = len({block for have in host for block in have})
+        self._free = list(range(self.n_blocks - 1, held, -1))  # the lowest is handed out first
         return src, dst
 
     def physical_rows(self, lanes: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
@@ -720,9 +723,10 @@ class Model:
         committed positions: blocks shared (`BlockTables.fork`), its last block, DeltaNet state and cached
         hidden copied. `more`: pools beside the layers' and the attached MTP head's that are read through the
         same tables (the `pool` of a head that only a runner knows)."""
+        pools = self._copied(more) if length % self.cfg.block_size else []
         pairs = self.blocks.fork(src, dst, length)
-        if pairs[0]:
-            attention.copy_blocks(self.caches(*more), *pairs, self.cfg.block_size)
+        if pools:
+            attention.copy_blocks(pools, *pairs, self.cfg.block_size)
         for ty, p in zip(self.cfg.layer_types, self.pool):
             if ty != ATTN:
                 p["conv"][dst].copy_(p["conv"][src])
@@ -732,10 +736,21 @@ class Model:
     def compact(self, *more: dict) -> int:
         """Move the held cache blocks to the pools' front (`BlockTables.compact`); returns how many moved.
         `more` as in `fork`."""
+        pools = self._copied(more) if self.blocks.moves()[0] else []
         src, dst = self.blocks.compact()
-        if src:
-            attention.copy_blocks(self.caches(*more), src, dst, self.cfg.block_size)
+        if pools:
+            attention.copy_blocks(pools, src, dst, self.cfg.block_size)
         return len(src)
+
+    def _copied(self, more: tuple[dict, ...]) -> list[torch.Tensor]:
+        """`caches`, with what `attention.copy_blocks` would refuse refused here, before a table says that the
+        blocks are copied."""
+        pools = self.caches(*more)
+        if pools:
+            n = attention.check_pools(pools, self.cfg.block_size)
+            if n != self.blocks.n_blocks:
+                raise ValueError(f"the pools have {n} blocks, the tables {self.blocks.n_blocks}")
+        return pools
 
     # ------------------------------------------------------------ sublayers
 

@@ -268,6 +268,37 @@ def test_caches_name_each_pool_once() -> None:
     assert len({p.data_ptr() for p in pools}) == len(pools) == 2 * (1 + model.cfg.layer_types.count(vm.ATTN))
 
 
+def test_a_refused_copy_leaves_the_tables_as_they_were() -> None:
+    """Pools that the copy cannot take: neither a fork nor a compaction writes a table first."""
+    model = model_helpers.build(lanes=3)
+    model.prefill(2, model_helpers.prompts(1, 40, seed=6)[0])
+    model.prefill(0, model_helpers.prompts(1, 21)[0])
+    model.reset(2)
+    t = model.blocks
+    assert t.moves()[0]
+    was = [list(h) for h in t.host], list(t.held_positions), dict(t._holders), list(t._free), t.table.clone()
+    kept = [x.clone() for x in model_helpers.slot_state(model, 0, 21)]
+    good = model.mtp.pool["k"], model.mtp.pool["v"]
+    for bad in ({"k": good[0][:-16].clone(), "v": good[1]}, {"k": good[0][:-16].clone(), "v": good[1][:-1].clone()},
+                {"k": good[0].view(-1), "v": good[1]}, {"k": good[0].transpose(1, 2), "v": good[1]}):
+        for call in (lambda: model.fork(0, 1, 21, bad), lambda: model.compact(bad)):
+            with pytest.raises(ValueError):
+                call()
+            assert (t.host, t.held_positions, t._holders, t._free) == was[:4] and torch.equal(t.table, was[4])
+    short = {name: p[: p.shape[0] // 2].clone() for name, p in model.mtp.pool.items()}
+    only, model.mtp = model.mtp, None
+    own = model.pool
+    model.pool = [short if ty == vm.ATTN else p for ty, p in zip(model.cfg.layer_types, own)]
+    for call in (lambda: model.fork(0, 1, 21), lambda: model.compact()):  # pools of one number, but not the tables'
+        with pytest.raises(ValueError):
+            call()
+        assert (t.host, t.held_positions, t._holders, t._free) == was[:4] and torch.equal(t.table, was[4])
+    model.pool, model.mtp = own, only
+    assert all(torch.equal(x, y) for x, y in zip(kept, model_helpers.slot_state(model, 0, 21), strict=True))
+    model.fork(0, 1, 21)
+    assert _slot_equal(model, 0, 1, 21) and model.compact() > 0
+
+
 def test_copy_blocks_on_the_cpu_and_its_refusals() -> None:
     k, v = torch.arange(64.0).view(64, 1, 1).expand(64, 1, 4).contiguous(), torch.arange(4.0).view(4, 1, 1, 1).expand(4, 1, 4, 16).contiguous()
     attention.copy_blocks([k, v], [2, 2], [0, 3])

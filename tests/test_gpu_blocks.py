@@ -160,3 +160,24 @@ def test_a_forked_slot_takes_the_attached_heads_cache(dev) -> None:
         assert all(torch.equal(x, y) for x, y in zip(before, model_helpers.slot_state(model, lane, 21), strict=True))
     rounds = [mtp.speculative_decode(model, [lane], [token], [21]) for lane in (0, 1)]
     assert rounds[0] == rounds[1]
+
+
+def test_a_fork_or_compaction_in_a_capture_changes_no_table(dev) -> None:
+    model = vm.Model(vm.tiny_cfg(), device=dev, dtype=torch.float32, lanes=3, max_seq=64)
+    model.blocks.grow(1, 40)
+    model.blocks.grow(0, 21)
+    model.reset(1)
+    t = model.blocks
+    was = [list(h) for h in t.host], list(t._free), t.table.clone()
+    graph = torch.cuda.CUDAGraph()
+    x = torch.zeros(4, device=dev)
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        for call in (lambda: model.fork(0, 2, 21), lambda: model.compact()):
+            with pytest.raises(ValueError):
+                call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (t.host, t._free) == was[:2] and torch.equal(t.table, was[2])
+    model.fork(0, 2, 21)
+    assert model.compact() > 0
