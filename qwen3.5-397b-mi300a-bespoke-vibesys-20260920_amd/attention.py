@@ -207,10 +207,26 @@ def _not_captured(device: torch.device) -> None:
                 raise ValueError("host ids cannot be part of a graph: give src and dst on the device")
 
 
+def _pool_blocks(pools: list[torch.Tensor], block: int) -> int:
+    """Blocks of the pools, one number for all of them; the library is asked about device pools alone."""
+    if any(p.is_cuda for p in pools):
+        return _mtpk.native().pool_blocks(pools, block)
+    if not pools or block < 1:
+        raise ValueError("copy_blocks takes at least one pool, and a block has at least one row")
+    first = pools[0]
+    n = first.shape[0] // (1 if first.dim() == 4 else block) if first.dim() else 0
+    for p in pools:
+        rows = {3: n * block, 4: n}.get(p.dim())
+        if rows is None or p.shape[0] != rows or p.numel() == 0 or not p.is_contiguous() or p.device != first.device:
+            raise ValueError(f"pools must be contiguous K caches [rows, kv_heads, hd] and V caches [blocks, kv_heads, hd, "
+                             f"{block}] of one number of blocks on one device, got {tuple(p.shape)} on {p.device}")
+    return n
+
+
 def check_pools(pools: list[torch.Tensor], block: int = BLOCK) -> int:
     """Number of blocks of the pools, after every check that `copy_blocks` makes of them and of the moment when
     it is called with host ids (`ValueError`): for callers that change block tables before the copies."""
-    n_blocks = _mtpk.native().pool_blocks(pools, block)
+    n_blocks = _pool_blocks(pools, block)
     _not_captured(pools[0].device)
     for p in pools:
         if p.is_cuda and (p.numel() // n_blocks * p.element_size() % 16 or p.data_ptr() % 16):
@@ -227,14 +243,13 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
     `ValueError`) and copied to the device, or int32 / int64 device tensors, which are taken as they are:
     a pair with an id outside the pools is skipped, and the rest of the rule is the caller's; a captured call
     takes device ids alone. CPU pools take the torch spelling."""
-    native = _mtpk.native()
     held = [torch.is_tensor(x) and x.is_cuda for x in (src, dst)]
     if all(held):
-        native.copy_blocks(pools, src, dst, block, _mtpk.stream_for(src))
+        _mtpk.native().copy_blocks(pools, src, dst, block, _mtpk.stream_for(src))
         return
     if any(held):
         raise ValueError("src and dst must both be on the host or both on the device")
-    n_blocks = native.pool_blocks(pools, block)
+    n_blocks = _pool_blocks(pools, block)
     src, dst = (torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in (src, dst))
     if src.shape != dst.shape:
         raise ValueError("src and dst must be of one length")
@@ -253,4 +268,4 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
             blocks[dst] = blocks[src]
         return
     pairs = torch.stack((src, dst)).pin_memory().to(device, non_blocking=True)
-    native.copy_blocks(pools, pairs[0], pairs[1], block, _mtpk.stream_for(pairs))
+    _mtpk.native().copy_blocks(pools, pairs[0], pairs[1], block, _mtpk.stream_for(pairs))

@@ -313,6 +313,21 @@ def test_copy_blocks_on_the_cpu_and_its_refusals() -> None:
     assert torch.equal(k, before[0]) and torch.equal(v, before[1])
 
 
+def test_cpu_pools_take_no_library(monkeypatch) -> None:
+    """The torch spelling alone: copies, refusals, a model's fork and compaction without a built library."""
+    def missing():
+        raise RuntimeError("not built")
+
+    monkeypatch.setattr(_mtpk, "native", missing)
+    monkeypatch.setattr(_mtpk, "lib", missing)
+    test_copy_blocks_on_the_cpu_and_its_refusals()
+    test_model_fork_and_compact_take_the_attached_heads_cache()
+    with pytest.raises(ValueError):
+        attention.copy_blocks([torch.zeros(())], [0], [0])
+    with pytest.raises(ValueError):
+        attention.copy_blocks([torch.zeros(32, 1, 1)], [0], [1], 0)
+
+
 P = 1 << 20  # an address that no refused call follows
 
 
