@@ -234,6 +234,13 @@ def check_pools(pools: list[torch.Tensor], block: int = BLOCK) -> int:
     return n_blocks
 
 
+def _host_ids(ids) -> torch.Tensor:
+    ids = torch.as_tensor(ids).reshape(-1)
+    if ids.numel() and (ids.dtype == torch.bool or ids.is_floating_point() or ids.is_complex()):
+        raise ValueError(f"block ids must be integers, got {ids.dtype}")
+    return ids.to(torch.int64)
+
+
 def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None:
     """Block `dst[i]` of every pool becomes block `src[i]` of it, in one launch (`mtpk_copy_blocks`): K pools
     `[rows, kv_heads, hd]` and V pools `[rows / block, kv_heads, hd, block]` of one cache's layers.
@@ -250,7 +257,7 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
     if any(held):
         raise ValueError("src and dst must both be on the host or both on the device")
     n_blocks = _pool_blocks(pools, block)
-    src, dst = (torch.as_tensor(x, dtype=torch.int64).reshape(-1) for x in (src, dst))
+    src, dst = _host_ids(src), _host_ids(dst)
     if src.shape != dst.shape:
         raise ValueError("src and dst must be of one length")
     if src.numel() == 0:

@@ -313,6 +313,18 @@ def test_copy_blocks_on_the_cpu_and_its_refusals() -> None:
     assert torch.equal(k, before[0]) and torch.equal(v, before[1])
 
 
+def test_host_ids_that_are_not_integers_are_refused() -> None:
+    k = torch.arange(64.0).view(64, 1, 1)
+    before = k.clone()
+    for src, dst in (([0.7], [1]), ([0], [1.5]), (torch.tensor([0.0]), torch.tensor([1.0])), ([True], [False]), ([0j], [1])):
+        with pytest.raises(ValueError):
+            attention.copy_blocks([k], src, dst)
+    assert torch.equal(k, before)
+    attention.copy_blocks([k], torch.tensor([2], dtype=torch.uint8), torch.tensor([[1]], dtype=torch.int32))
+    attention.copy_blocks([k], [], torch.empty(0))
+    assert torch.equal(k[16:32], before[32:48]) and torch.equal(k[:16], before[:16])
+
+
 def test_cpu_pools_take_no_library(monkeypatch) -> None:
     """The torch spelling alone: copies, refusals, a model's fork and compaction without a built library."""
     def missing():
