@@ -355,7 +355,10 @@ def row_stride(x: torch.Tensor) -> int | None:
 
 def stream_of(device: torch.device) -> int:
     """Handle of torch's current stream on `device` (what the kernels launch on): the handle alone, without
-    the Stream object around it (0.1 against 2.1 us a call)."""
+    the Stream object around it (0.1 against 2.1 us a call). `ValueError` for a device that has no streams:
+    some calls check their tensors' device by this alone."""
+    if device.type != "cuda":
+        raise ValueError(f"libmtpk entry points take device tensors, got {device}")
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 

@@ -340,6 +340,18 @@ def test_cpu_pools_take_no_library(monkeypatch) -> None:
         attention.copy_blocks([torch.zeros(32, 1, 1)], [0], [1], 0)
 
 
+def test_a_cpu_tensor_has_no_stream(monkeypatch) -> None:
+    """Not the current device's either: the kernel would be handed a host address."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    for device in (torch.device("cpu"), torch.device("cpu", 0), torch.device("meta")):
+        with pytest.raises(ValueError):
+            _mtpk.stream_of(device)
+    with pytest.raises(ValueError):
+        _mtpk.stream_for(torch.empty(1))
+    assert _mtpk.stream_of(torch.device("cuda")) == 0
+
+
 P = 1 << 20  # an address that no refused call follows
 
 
