@@ -62,6 +62,8 @@ struct MaskedArgs {
   // cap2 * tanh(s scale / cap) as s (c0 + c1 s^2) up to |s| = cubic_max, s (d0 + d1 s^2 + d2 s^4) up to
   // quintic_max; s c0 without a cap
   float cubic_max, quintic_max, c0, c1, d0, d1, d2;
+  // the same quintic of any cap: s (e0 + e1 u + e2 u^2), u = (s cap_k)^2, up to |s cap_k| = 0.25
+  float cap_k, e0, e1, e2;
   float* part_o;
   float* part_ml;
 };
@@ -214,6 +216,13 @@ __device__ inline float cap_exact(const MaskedArgs& a, float s) {
   return fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.cap_in) + 1.f), -2.f * a.cap2, a.cap2);
 }
 
+// The cap of a score, however wide: cap_exact is off by 2^-23 of the cap, which is more than a whole score where the
+// cap is far above it, so it takes over only where scores are of the cap's own size.
+__device__ inline float cap_any(const MaskedArgs& a, float s) {
+  const float x = s * a.cap_k, u = x * x;
+  return u <= 0.0625f ? s * fmaf(u, fmaf(u, a.e2, a.e1), a.e0) : cap_exact(a, s);
+}
+
 // The larger of a value and of the other half's (lane ^ 32).
 __device__ inline float halves_max(float v) {
   const uint32_t u = f32_bits(v);
@@ -251,7 +260,7 @@ struct TileSoftmax {
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = cap_exact(a, s[i]);
+        for (int i = 0; i < 16; ++i) s[i] = CAP ? cap_exact(a, s[i]) : cap_any(a, s[i]);
       }
       if (SLOPES) {
         const float away = (float)(row.pos - key0 - 8 * h);
@@ -380,7 +389,7 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
         for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
       }
     }
-    s = a.cap2 > 0.f ? cap_exact(a, s) : s * a.c0;  // c0 without a cap: the scale
+    s = a.cap2 > 0.f ? cap_any(a, s) : s * a.c0;  // c0 without a cap: the scale
     s = live ? fmaf(fabsf((float)(row.pos - key)), -slope2, s) : -INFINITY;
     const float mn = fmaxf(m, wave_max(s)), ms = mn == -INFINITY ? 0.f : mn;
     const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn), p = live ? __builtin_amdgcn_exp2f(s - ms) : 0.f;
@@ -1204,10 +1213,14 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
     // tanh(u) / u by polynomials in u^2 of least relative error: 8.4e-6 on |u| <= 0.15, which is 9e-5 of an exponent
     // at cap 50 (a rounded probability is off by up to 2^-8), and 4e-7 on |u| <= 0.25
     const double k = (double)scale / softcap, c = (double)softcap * 1.4426950408889634;
-    a.cap2 = (float)c;
+    a.cap2 = (float)std::min(c, 1.7e38);  // twice it stays finite
     a.cap_in = (float)(2. * 1.4426950408889634 * k);
     a.cubic_max = (float)(0.15 / k);
     a.quintic_max = (float)(0.25 / k);
+    a.cap_k = (float)k;
+    a.e0 = (float)(c * k * 0.99999961);
+    a.e1 = (float)(c * k * -0.33321928);
+    a.e2 = (float)(c * k * 0.12841935);
     if (c <= kCapMost) {
       a.c0 = (float)(c * k * 0.99999165);
       a.c1 = (float)(c * k * k * k * -0.33035765);

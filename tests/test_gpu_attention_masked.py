@@ -141,6 +141,30 @@ def test_wide_caps(dev, heads, kvh, hd, t, base, softcap) -> None:
     check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap, slopes=torch.linspace(0.0, 2.0, heads))
 
 
+@pytest.mark.parametrize("softcap", [1e4, 1e5, 1e8, 1e30, 3e38])
+@pytest.mark.parametrize("heads,kvh,hd,t,base", [(32, 2, 256, 1, [500]), (32, 2, 256, 40, [9]), (16, 4, 128, 12, [3000])])
+def test_caps_far_above_the_scores(dev, heads, kvh, hd, t, base, softcap) -> None:
+    """A cap that is as good as none leaves the scores' own digits. So do the rows that are done again one by one:
+    an infinite value that another row sees."""
+    for q_std in (2.0, 8.0):
+        q, k, v, table, b0 = case(1, 1, t, heads, kvh, hd, base, q_std=q_std)
+        check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap)
+    check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap, slopes=torch.linspace(0.0, 2.0, heads))
+    if t > 1:
+        at = base[0] + t - 1
+        v[int(table[0, at // 16]) * 16 + at % 16] = float("inf")
+        want, spread = ref.paged_attention_masked(q[:, :-1], k, v.nan_to_num(0, 0, 0), table, b0, hd**-0.5, softcap=softcap)
+        got = run(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap).double().cpu()[:, :-1]
+        assert float(((got - want).abs() / bars(want, spread)).max()) <= 1.0
+
+
+def test_scores_of_a_wide_caps_size(dev) -> None:
+    """Scores around and above a quarter of caps of some hundreds, where the cap's two forms meet."""
+    for softcap in (100.0, 400.0):
+        q, k, v, table, b0 = case(1, 1, 9, 16, 4, 128, [90], q_std=softcap / 8)
+        check(dev, q, k, v, table, b0, 128**-0.5, softcap=softcap)
+
+
 @pytest.mark.parametrize("heads,kvh,hd,t,base", [(32, 2, 256, 1, [500]), (32, 2, 256, 40, [9]), (16, 4, 128, 12, [3000])])
 @pytest.mark.parametrize("softcap", [0.0, 30.0, 50.0, 69.0])
 def test_scores_far_from_zero(dev, heads, kvh, hd, t, base, softcap) -> None:
