@@ -670,9 +670,11 @@ int mtpk_rotate_to_cache(const uint16_t* q, const int64_t* q_strides, const uint
  * seen iff j >= first[b * t + s] (int32 | int64 [batch, t], may be NULL: the row's document), p - j <
  * window (0: none), and j <= p or both p and j below prefix[b] (int32 | int64 [batch], may be NULL); keys
  * at or past base_pos[b] + t, or past the table, are never seen. out = the softmax's sum over the seen
- * keys, 0 for a row that sees none, times sigmoid(gate) when gate is given, rounded once. Keys that no row
- * sees may hold anything, and one row's keys do not touch another row. Query, gate and output strides
- * multiples of 8, rows 16-byte aligned. Pools of any size; table_stride <= 2^26.
+ * keys, 0 for a row that sees none, times sigmoid(gate) when gate is given, rounded once. Keys that a row does
+ * not see may hold anything: they are no part of its sum. Finite keys that no row of the call sees leave every
+ * bit as it is; a row's last bits may differ with what the other rows of its call see, as the rows of a tile share
+ * the form in which their scores are capped, and where a value is not finite are done again in fp32 alone. Query,
+ * gate and output strides multiples of 8, rows 16-byte aligned. Pools of any size; table_stride <= 2^26.
  * n_split from mtpk_attention_masked_splits (0 for a shape that is not taken; max_ctx a bound on
  * base_pos + t), at most 64; n_split > 1 needs mtpk_attention_masked_workspace_bytes of workspace
  * (16-byte aligned). No reference counterpart. */

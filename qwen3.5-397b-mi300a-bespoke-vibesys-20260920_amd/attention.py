@@ -193,8 +193,9 @@ def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     `slopes[h] * |p - j|`. The row sees j iff `j <= p`, or p and j are both below `prefix[b]` (integers
     `[B]`; at most `base_pos[b] + t` counts); and `p - j < window` (0: no window); and `j >= first[b, s]`
     (integers `[B, t]`: the first position of the row's document). A row that sees nothing is zeros.
-    `gate` of q's shape multiplies the output by its sigmoid. Keys that a row does not see never reach its
-    output, whatever they hold. `ctx_len` is a host bound on `max(base_pos) + t`; it sizes the key splits
+    `gate` of q's shape multiplies the output by its sigmoid. Keys that a row does not see are no part of its
+    sum, whatever they hold (finite ones that no row sees leave every bit; the other rows' may move its last bits,
+    within the rounding). `ctx_len` is a host bound on `max(base_pos) + t`; it sizes the key splits
     alone. bf16 with fp32 scores, statistics and sums; the output is rounded once."""
     return _mtpk.native().paged_attention_masked(q, k_pool, v_pool, block_table, base_pos, ctx_len, scale, softcap, window,
                                                  slopes, prefix, first, gate, _mtpk.stream_for(q))

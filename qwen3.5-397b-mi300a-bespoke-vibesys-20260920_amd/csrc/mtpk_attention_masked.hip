@@ -21,8 +21,11 @@
 // rounded once.
 //
 // Keys that a row does not see may hold anything: their scores are replaced, and V is zeroed where no row of
-// the workgroup sees the key. A value that is not finite and that some of the rows sharing a tile see
-// makes all of them NaN (0 times infinity): such rows are found at the end and done again one by one.
+// the workgroup sees the key. Nor do finite ones that no row sees choose the form in which a tile's scores are capped;
+// the rows of a tile share it (each score's form by that score alone took two forms and a selection for every one of
+// a tile past the cubic: 8000 rows of 16 heads of 128, scores of std 4 under a cap of 30, 390 -> 597 us). A value that
+// is not finite and that some of the rows sharing a tile see makes all of them NaN (0 times infinity): such rows are
+// found at the end and done again one by one.
 
 #include <algorithm>
 #include <cmath>
@@ -59,11 +62,9 @@ struct MaskedArgs {
   int n_split, row_groups;
   float cap2;                   // cap * log2(e), 0: none
   float cap_in;                 // 2 * log2(e) * scale / cap
-  // cap2 * tanh(s scale / cap) as s (c0 + c1 s^2) up to |s| = cubic_max, s (d0 + d1 s^2 + d2 s^4) up to
-  // quintic_max; s c0 without a cap
-  float cubic_max, quintic_max, c0, c1, d0, d1, d2;
-  // the same quintic of any cap: s (e0 + e1 u + e2 u^2), u = (s cap_k)^2, up to |s cap_k| = 0.25
-  float cap_k, e0, e1, e2;
+  // cap2 * tanh(s scale / cap) as s (c0 + c1 s^2) up to |s| = cubic_max (s c0 without a cap), and as
+  // s (e0 + e1 u + e2 u^2), u = (s cap_k)^2, up to |s cap_k| = 0.25
+  float cubic_max, c0, c1, cap_k, e0, e1, e2;
   float* part_o;
   float* part_ml;
 };
@@ -216,11 +217,13 @@ __device__ inline float cap_exact(const MaskedArgs& a, float s) {
   return fmaf(__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.cap_in) + 1.f), -2.f * a.cap2, a.cap2);
 }
 
+__device__ inline float cap_quintic(const MaskedArgs& a, float s, float u) { return s * fmaf(u, fmaf(u, a.e2, a.e1), a.e0); }
+
 // The cap of a score, however wide: cap_exact is off by 2^-23 of the cap, which is more than a whole score where the
 // cap is far above it, so it takes over only where scores are of the cap's own size.
 __device__ inline float cap_any(const MaskedArgs& a, float s) {
   const float x = s * a.cap_k, u = x * x;
-  return u <= 0.0625f ? s * fmaf(u, fmaf(u, a.e2, a.e1), a.e0) : cap_exact(a, s);
+  return u <= 0.0625f ? cap_quintic(a, s, u) : cap_exact(a, s);
 }
 
 // The larger of a value and of the other half's (lane ^ 32).
@@ -243,20 +246,33 @@ struct TileSoftmax {
 
   // Scores to where `exponent` takes them from there, and without a cap the row's new maximum. Returns what the
   // row's sums are multiplied by, 1 for the whole wave in most tiles.
-  __device__ inline float finish(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
+  // Inlined by force, as the steps around it in k_masked_rows are: a call would keep the wave's sums in memory.
+  __device__ __forceinline__ float finish(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
                                  int h, RowSoft& r) {
     c0 = a.c0;
     c1 = a.c1;
-    const bool bent = CAP ? __ballot(!(top <= a.cubic_max)) != 0ull : a.cap2 > 0.f;  // past the cap's cubic part
+    const int lo = row.lo - key0 - 8 * h, n = max(row.hi - row.lo, 0);  // seen: 0 <= i - lo < n, in one comparison
+    auto seen = [&](int i) { return (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)n; };
+    auto past = [&]() { return __ballot(!(top <= a.cubic_max)) != 0ull; };
+    bool bent = CAP ? past() : a.cap2 > 0.f;  // past the cap's cubic part
+    if (CAP && bent && !whole) {  // keys that no row sees have no part in the choice of the form
+      begin();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = seen(i) ? s[i] : 0.f;
+        scan(s[i]);
+      }
+      bent = past();
+    }
     if (SLOPES || !whole || bent) {  // uniform over the wave: in full here, and the exponent is the score
       if (!bent) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = CAP ? s[i] * fmaf(s[i] * s[i], c1, c0) : s[i] * c0;
-      } else if (CAP && __ballot(!(top <= a.quintic_max)) == 0ull) {
+      } else if (CAP && __ballot(!(top * a.cap_k <= 0.25f)) == 0ull) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float u = s[i] * s[i];
-          s[i] = s[i] * fmaf(u, fmaf(u, a.d2, a.d1), a.d0);
+          const float x = s[i] * a.cap_k;
+          s[i] = cap_quintic(a, s[i], x * x);
         }
       } else {
 #pragma unroll
@@ -268,10 +284,8 @@ struct TileSoftmax {
         for (int i = 0; i < 16; ++i) s[i] = fmaf(fabsf(away - (float)(16 * (i >> 3) + (i & 7))), -slope2, s[i]);
       }
       if (!whole) {
-        const int lo = row.lo - key0 - 8 * h, n = max(row.hi - row.lo, 0);  // seen: 0 <= i - lo < n, in one comparison
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[i] = (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)n ? s[i] : kUnseen;
+        for (int i = 0; i < 16; ++i) s[i] = seen(i) ? s[i] : kUnseen;
       }
       c0 = 1.f;
       c1 = 0.f;
@@ -288,7 +302,7 @@ struct TileSoftmax {
     r.l *= alpha;
     return alpha;
   }
-  __device__ inline float prepare(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
+  __device__ __forceinline__ float prepare(const MaskedArgs& a, f32x16_t& s, const RowKeys& row, float slope2, bool whole, int key0,
                                   int h, RowSoft& r) {
     begin();
 #pragma unroll
@@ -603,7 +617,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     }
     ring_fence();
   };
-  auto finish = [&](f32x16_t& s, int key) {
+  auto finish = [&](f32x16_t& s, int key) __attribute__((always_inline)) {
     return soft_tile.finish(a, s, row, slope2, set.whole(key), key, h, soft);
   };
   // Exponents [from, to) of a tile's 16.
@@ -612,7 +626,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   };
   // S^T of the tile at k into sn and O^T of the one at v with the scores sc. `next` (or null): where the K after that
   // is; `to` (or null): where the next stage goes.
-  auto tile = [&](const uint8_t* k, const uint8_t* v, auto next, const f32x16_t& sc, f32x16_t& sn, auto to) {
+  auto tile = [&](const uint8_t* k, const uint8_t* v, auto next, const f32x16_t& sc, f32x16_t& sn, auto to) __attribute__((always_inline)) {
     constexpr bool kNext = !std::is_same_v<decltype(next), std::nullptr_t>;
     constexpr bool kStage = !std::is_same_v<decltype(to), std::nullptr_t>;
     constexpr int kSlots = G::kS + G::kT;  // products beside which the exponents stand, two thirds before O^T begins
@@ -648,7 +662,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   };
   // The stage in `at`; the next one's loads go to `to`.
   f32x16_t s0, s1;
-  auto stage = [&](uint8_t* at, uint8_t* to) {
+  auto stage = [&](uint8_t* at, uint8_t* to) __attribute__((always_inline)) {
     ring_fence();
     vmcnt_wait<0>();  // this stage, loaded during the last one, which has been the last to read `to`
     __builtin_amdgcn_s_barrier();
@@ -1216,7 +1230,6 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
     a.cap2 = (float)std::min(c, 1.7e38);  // twice it stays finite
     a.cap_in = (float)(2. * 1.4426950408889634 * k);
     a.cubic_max = (float)(0.15 / k);
-    a.quintic_max = (float)(0.25 / k);
     a.cap_k = (float)k;
     a.e0 = (float)(c * k * 0.99999961);
     a.e1 = (float)(c * k * -0.33321928);
@@ -1224,9 +1237,6 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
     if (c <= kCapMost) {
       a.c0 = (float)(c * k * 0.99999165);
       a.c1 = (float)(c * k * k * k * -0.33035765);
-      a.d0 = (float)(c * k * 0.99999961);
-      a.d1 = (float)(c * k * k * k * -0.33321928);
-      a.d2 = (float)(c * k * k * k * k * k * 0.12841935);
     }
   }
   a.part_o = (float*)workspace;

@@ -243,6 +243,25 @@ def test_unseen_keys_may_hold_anything(dev, heads, kvh, hd, t, base, value) -> N
         assert worst <= 1.0  # and no NaN
 
 
+@pytest.mark.parametrize("heads,kvh,hd,t,base", [(32, 2, 256, 1, [40]), (16, 4, 128, 9, [40]), (32, 2, 256, 40, [40]), (8, 2, 64, 3, [4000]),
+                                                 (16, 4, 128, 60, [90])])
+@pytest.mark.parametrize("softcap,slope", [(30.0, 0.0), (50.0, 0.01), (300.0, 0.0), (1e6, 0.0)])
+def test_unseen_keys_leave_capped_rows_bit_for_bit(dev, heads, kvh, hd, t, base, softcap, slope) -> None:
+    """Finite keys that no row sees, before the document and behind the last row, whose scores lie in the middle of the
+    cap's range or at its end: the form in which a tile's scores are capped does not go by them."""
+    q, k, v, table, b0 = case(6, 1, t, heads, kvh, hd, base)
+    first = torch.full((1, t), base[0] - 9)
+    kw = dict(first=first, softcap=softcap, **({"slopes": torch.full((heads,), slope)} if slope else {}))
+    clean = check(dev, q, k, v, table, b0, hd**-0.5, **kw)
+    at = torch.arange(table.shape[1] * 16)
+    unseen = table[0].long()[at // 16] * 16 + at % 16
+    unseen = unseen[(at < base[0] - 9) | (at >= base[0] + t)]
+    for value in (0.0, 3.0, 8.0, 30.0, 1e4, 1e30):
+        k2, v2 = k.clone(), v.clone()
+        k2[unseen], v2[unseen] = (k[unseen].float() * value).bfloat16(), 7.0
+        assert torch.equal(run(dev, q, k2, v2, table, b0, hd**-0.5, **kw).double().cpu(), clean)
+
+
 @pytest.mark.parametrize("heads,kvh,hd,t,base", [(8, 2, 64, 3, [40]), (32, 2, 256, 6, [100]), (16, 4, 128, 60, [7]), (8, 2, 128, 1, [5000])])
 def test_seen_infinities_and_nan(dev, heads, kvh, hd, t, base) -> None:
     """What a row sees reaches it: an infinite value its channel alone, a NaN key every channel; the rows
