@@ -42,7 +42,7 @@ def paged_attention_masked(q, k_pool, v_pool, table, base, scale, *, softcap=0.0
             if softcap:
                 x = softcap * torch.tanh(x / softcap)
             if slopes is not None:
-                x = x - float(slopes[h]) * (p - j).abs()
+                x = x - float(slopes[h]) * (p - j).abs().double()
             x = x.masked_fill(~seen, -torch.inf)
             any_ = seen.any(-1)
             w = torch.softmax(x[any_], -1)

@@ -62,3 +62,14 @@ def test_unseen_values_stay_out() -> None:
     v[table[0][0] * 16 + 11] = float("nan")  # position 11 of lane 0: rows 2.. see it
     out, _ = masked_attention_ref.paged_attention_masked(q, k, v, table, base, 0.3)
     assert torch.equal(out[0, :2], clean[0, :2]) and out[0, 2:].isnan().all() and torch.equal(out[1], clean[1])
+
+
+def test_a_bias_goes_by_the_distances_differences() -> None:
+    """A row far behind its keys weighs them as the nearest row that sees them all: one distance more for every key
+    is no change, to the digits of 64 bits."""
+    q, k, v, table, _ = _case(3, b=1, t=1, base=(0,))
+    slopes = torch.tensor([0.01, 0.1, 0.3, 1.0])
+    near, _ = masked_attention_ref.paged_attention_masked(q, k, v, table, torch.tensor([48]), 0.5, slopes=slopes)
+    for past in (1, 2**20, 2**31):
+        far, _ = masked_attention_ref.paged_attention_masked(q, k, v, table, torch.tensor([48 + past]), 0.5, slopes=slopes)
+        torch.testing.assert_close(far, near, rtol=1e-6, atol=1e-7)
