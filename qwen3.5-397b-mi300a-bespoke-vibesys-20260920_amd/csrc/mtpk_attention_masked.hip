@@ -69,7 +69,7 @@ struct MaskedArgs {
   float* part_ml;
 };
 
-// The keys [lo, hi) that a row sees, and its position.
+// The keys [lo, hi) that a row sees, and its position (for distances).
 struct RowKeys {
   int pos, lo, hi;
 };
@@ -84,9 +84,12 @@ __device__ inline RowKeys masked_row(const MaskedArgs& a, int b, int s) {
   if (a.window > 0) lo = max(lo, pos - a.window + 1);
   if (a.first) lo = max(lo, load_index(a.first, a.first_dt, (int64_t)b * a.t + s));
   // never past the rows of this call, nor past the lane's table
-  hi = max(min(min(hi, base + a.t), a.table_stride * kAttnBlock), (int64_t)0);
+  const int64_t end = a.table_stride * kAttnBlock;
+  hi = max(min(min(hi, base + a.t), end), (int64_t)0);
   lo = min(lo, (int64_t)INT32_MAX);
-  return RowKeys{(int)pos, (int)lo, (int)hi};
+  // A row past the table is as if at its end: one distance more or less for all of its keys is no change, and
+  // int and float hold the others' differences.
+  return RowKeys{(int)min(pos, end), (int)lo, (int)hi};
 }
 
 // Over the 16 lanes of a row by DPP, then the two rows of a half.

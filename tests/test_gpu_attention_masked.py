@@ -312,6 +312,20 @@ def test_lanes_that_hold_nothing(dev) -> None:
     assert torch.all((got[[0, 3]] - want).abs() <= bars(want, spread))
 
 
+@pytest.mark.parametrize("heads,kvh,hd,t", [(8, 2, 64, 2), (16, 4, 128, 20), (32, 2, 256, 5)])
+@pytest.mark.parametrize("past", [1, 2**20, 2**30, 2**31 + 5, 2**40])
+def test_a_bias_of_rows_past_the_table(dev, heads, kvh, hd, t, past) -> None:
+    """Rows of positions far behind the table's last key: their keys' distances differ as those of near rows do."""
+    q, k, v, table, b0 = case(14, 2, t, heads, kvh, hd, [60, 60])
+    b0[1] = table.shape[1] * 16 + past
+    slopes = torch.linspace(0.01, 0.3, heads)
+    q, k, v = q.to(dev), k.to(dev), attention.v_blocks(v).to(dev)
+    for kw in ({}, {"softcap": 30.0}):
+        got = attention.paged_attention_masked(q, k, v, table.to(dev), b0.to(dev), 80, hd**-0.5, slopes=slopes.to(dev), **kw)
+        want, spread = ref.paged_attention_masked(q.cpu(), k.cpu(), attention.v_rows(v).cpu(), table, b0, hd**-0.5, slopes=slopes, **kw)
+        assert float(((got.double().cpu() - want).abs() / bars(want, spread)).max()) <= 1.0
+
+
 def test_strides_and_index_types(dev) -> None:
     q, k, v, table, b0 = case(11, 2, 6, 16, 4, 128, [30, 200])
     kw = dict(prefix=b0 + 3, first=torch.randint(0, 30, (2, 6)))
