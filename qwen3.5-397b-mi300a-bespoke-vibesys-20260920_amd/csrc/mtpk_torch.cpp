@@ -207,8 +207,9 @@ Tensor rotate_to_cache(const Tensor& q_in, const Tensor& k_in, const Tensor& v_i
     need(flags && keep->dim() == 2 && keep->size(0) == b && keep->size(1) == t, "keep must be bool [", b, ", ", t, "]");
     on(device, *keep);
   }
+  need(heads > 0 && kvh > 0, "q and k must have heads, got ", q_in.sizes(), " and ", k_in.sizes());
   const Tensor out = at::empty_like(q_in, q_in.options(), at::MemoryFormat::Contiguous);
-  if (out.numel() == 0) return out;
+  if (out.numel() == 0) return out;  // no rows
   const Tensor q = on16(q_in), k = on16(k_in), v = on16(v_in);
   const Strides qs(q), ks(k), vs(v), os(out);
   const c10::DeviceGuard guard(device);

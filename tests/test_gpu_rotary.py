@@ -260,3 +260,15 @@ def test_rotate_to_cache_refuses(dev) -> None:
         with pytest.raises(ValueError):
             call(**kw)
     assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+
+
+def test_rotate_to_cache_of_no_rows_and_of_no_heads(dev) -> None:
+    """No rows are no work; k and v beside a q without heads are not left unwritten in silence."""
+    q, k, v, (kp, vp), table, base = _round(dev, 2, 3, 8, 2, 64, 64, [4, 30], 5, 6)
+    rates, _ = rotary.frequencies(64, 1e4, device=dev)
+    before = kp.clone(), vp.clone()
+    assert rotary.rotate_to_cache(q[:, :0], k[:, :0], v[:, :0], rates, kp, vp, table, base).shape == (2, 0, 8, 64)
+    assert rotary.rotate_to_cache(q[:0], k[:0], v[:0], rates, kp, vp, table[:0], base[:0]).shape == (0, 3, 8, 64)
+    with pytest.raises(ValueError):
+        rotary.rotate_to_cache(q[:, :, :0], k, v, rates, kp, vp, table, base)
+    assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
