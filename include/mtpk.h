@@ -637,7 +637,8 @@ int mtpk_kv_write(const uint16_t* k, int64_t k_row_stride, const uint16_t* v, in
  * with interleaved, (2 i, 2 i + 1), and pair i is turned by pos * rates[i] radians (f64 [rot_dim / 2],
  * the angle reduced in 64 bits) and multiplied by magnitude. out: x's type, strides like x's; it may be x
  * itself. fp32 arithmetic, one rounding. dim a multiple of 8 up to 512, rot_dim even, 2 .. dim; 16-byte
- * aligned rows. The rates of a scaled context are the caller's (rotary.frequencies). No reference
+ * aligned rows; fewer than 2^32 threads, one for 8 channels of a token's head lanes (tokens times dim / 8 rounded
+ * up to a power of two). The rates of a scaled context are the caller's (rotary.frequencies). No reference
  * counterpart in this form (`apply_rope`, model.py:631-635, takes fp32 tables: mtpk_rownorm). */
 int mtpk_rotate(const void* x, int dtype, const int64_t* x_strides, int64_t tokens, int64_t heads,
                 int64_t dim, const void* w, int w_dtype, float eps, const int64_t* pos,
@@ -651,7 +652,7 @@ int mtpk_rotate(const void* x, int dtype, const int64_t* x_strides, int64_t toke
  * [head_dim], each may be NULL: no norm). Step s of lane b is at base_pos[b] + s, rotated at
  * positions[b * t + s] when positions is given (int64 [batch, t]); its k and v go where
  * mtpk_kv_write puts them, with its keep (rows with 0, and positions outside the lane's table or the
- * pool, are not written; their q rows are). out [batch, t, heads, head_dim]. head_dim as dim above. */
+ * pool, are not written; their q rows are). A call of 2^32 threads or more is refused. out [batch, t, heads, head_dim]. head_dim as dim above. */
 int mtpk_rotate_to_cache(const uint16_t* q, const int64_t* q_strides, const uint16_t* k,
                          const int64_t* k_strides, const uint16_t* v, const int64_t* v_strides,
                          const void* q_norm, const void* k_norm, int norm_dtype, float eps,
@@ -674,7 +675,8 @@ int mtpk_rotate_to_cache(const uint16_t* q, const int64_t* q_strides, const uint
  * not see may hold anything: they are no part of its sum. Finite keys that no row of the call sees leave every
  * bit as it is; a row's last bits may differ with what the other rows of its call see, as the rows of a tile share
  * the form in which their scores are capped, and where a value is not finite are done again in fp32 alone. Query,
- * gate and output strides multiples of 8, rows 16-byte aligned. Pools of any size; table_stride <= 2^26.
+ * gate and output strides multiples of 8, rows 16-byte aligned. Pools of any size; table_stride <= 2^26;
+ * batch * t * heads < 2^25, in fewer than 2^24 groups of up to 128 rows of a kv head.
  * n_split from mtpk_attention_masked_splits (0 for a shape that is not taken; max_ctx a bound on
  * base_pos + t), at most 64; n_split > 1 needs mtpk_attention_masked_workspace_bytes of workspace
  * (16-byte aligned). No reference counterpart. */
@@ -694,8 +696,9 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
 
 /* ---------------------------------------------------------------- copies of cache blocks
  * Block dst[i] = block src[i] (int32 | int64 [pairs], on the device) in each of n_pools pools, in one
- * launch per 64 pools: forked lanes' last blocks, blocks that a compaction moves. pools and block_bytes
- * are host arrays; pool p holds n_blocks blocks of block_bytes[p] bytes (a multiple of 16; pools 16-byte
+ * launch per 64 pools and 2^24 pieces of up to 16 KB: forked lanes' last blocks, blocks that a compaction
+ * moves. pools and block_bytes are host arrays (pairs < 2^31); pool p holds n_blocks blocks of block_bytes[p]
+ * bytes (a multiple of 16; pools 16-byte
  * aligned). A pair with an id outside [0, n_blocks) is skipped. A block may be the source of several
  * pairs; no block may be the destination of two, nor source of one and destination of another. No
  * reference counterpart (`block_pool.py` hands out blocks and never moves them). */

@@ -1146,7 +1146,7 @@ int masked_flags(const MaskedArgs& a, int64_t batch, hipStream_t st) {
 bool masked_shape(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim) {
   return batch > 0 && t > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
          (head_dim == 64 || head_dim == 128 || head_dim == 256) && batch <= INT32_MAX / 64 / t &&
-         heads <= INT32_MAX / 64 / (batch * t);
+         heads <= INT32_MAX / 64 / (batch * t) && batch * kv_heads * masked_row_groups(heads / kv_heads * t) <= kMaxGroups;
 }
 
 }  // namespace

@@ -25,7 +25,7 @@ struct CopyArgs {
 __global__ __launch_bounds__(256) void k_copy_blocks(CopyArgs a) {
   constexpr int N = kCopyPiece / 256 / 16;
   const int64_t per = (int64_t)a.pools * a.pieces;
-  const int64_t pair = blockIdx.x / per;
+  const int64_t pair = blockIdx.x / per;  // of this launch
   const int rest = (int)(blockIdx.x - pair * per), i = rest / a.pieces, piece = rest % a.pieces;
   const int64_t from = load_index(a.src, a.index_dt, pair), to = load_index(a.dst, a.index_dt, pair);
   if (from < 0 || from >= a.n_blocks || to < 0 || to >= a.n_blocks || from == to) return;
@@ -52,7 +52,7 @@ using namespace mtpk;
 extern "C" int mtpk_copy_blocks(void* const* pools, const int64_t* block_bytes, int n_pools,
                                 int64_t n_blocks, const void* src, const void* dst, int index_dtype,
                                 int64_t pairs, void* stream) {
-  if (!pools || !block_bytes || n_pools < 1 || n_blocks < 1 || pairs < 0) return MTPK_EINVAL;
+  if (!pools || !block_bytes || n_pools < 1 || n_blocks < 1 || pairs < 0 || pairs > INT32_MAX) return MTPK_EINVAL;
   if (index_dtype != MTPK_I32 && index_dtype != MTPK_I64) return MTPK_EINVAL;
   for (int i = 0; i < n_pools; ++i)
     if (!pools[i] || !aligned16(pools[i]) || block_bytes[i] < 16 || block_bytes[i] % 16) return MTPK_EINVAL;
@@ -68,15 +68,19 @@ extern "C" int mtpk_copy_blocks(void* const* pools, const int64_t* block_bytes, 
       most = a.bytes[i] > most ? a.bytes[i] : most;
     }
     const int64_t pieces = (most + kCopyPiece - 1) / kCopyPiece;
-    if (pieces * a.pools > INT32_MAX / pairs) return MTPK_EINVAL;
-    a.src = src;
-    a.dst = dst;
+    if (pieces > kMaxGroups / a.pools) return MTPK_EINVAL;
     a.index_dt = index_dtype;
     a.n_blocks = n_blocks;
     a.pieces = (int)pieces;
-    hipLaunchKernelGGL(k_copy_blocks, dim3((unsigned)(pairs * a.pools * pieces)), dim3(256), 0, (hipStream_t)stream, a);
-    const int rc = status_of(hipGetLastError());
-    if (rc) return rc;
+    const int64_t most_pairs = kMaxGroups / (a.pools * pieces), index_bytes = index_dtype == MTPK_I64 ? 8 : 4;
+    for (int64_t at = 0; at < pairs; at += most_pairs) {
+      const int64_t n = pairs - at < most_pairs ? pairs - at : most_pairs;
+      a.src = static_cast<const uint8_t*>(src) + at * index_bytes;
+      a.dst = static_cast<const uint8_t*>(dst) + at * index_bytes;
+      hipLaunchKernelGGL(k_copy_blocks, dim3((unsigned)(n * a.pools * pieces)), dim3(256), 0, (hipStream_t)stream, a);
+      const int rc = status_of(hipGetLastError());
+      if (rc) return rc;
+    }
   }
   return 0;
 }

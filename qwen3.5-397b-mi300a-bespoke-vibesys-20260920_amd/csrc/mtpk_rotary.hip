@@ -336,7 +336,7 @@ int rotate_launch(RotArgs& a, int64_t tokens, int interleaved, hipStream_t st) {
     a.v_groups = (int)v_groups;
     grid += v_groups;
   }
-  if (grid > INT32_MAX) return MTPK_EINVAL;
+  if (grid > kMaxGroups) return MTPK_EINVAL;
   if (interleaved) return rotate_g<T, kAdjacent, CACHE>(a, (unsigned)grid, st);
   if (a.rot % 16 == 0) return rotate_g<T, kHalvesOf8, CACHE>(a, (unsigned)grid, st);
   return rotate_g<T, kHalves, CACHE>(a, (unsigned)grid, st);

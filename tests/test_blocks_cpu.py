@@ -405,3 +405,15 @@ def test_masked_attention_sizes(lib) -> None:
                 == lib.mtpk_attention_masked_splits(1, 1, 32, 2, 256, ctx, 0))
     assert lib.mtpk_attention_masked_workspace_bytes(2, 1, 8, 2, 64, 1) == 0
     assert lib.mtpk_attention_masked_workspace_bytes(2, 1, 8, 2, 64, 3) >= 2 * 2 * 4 * 3 * 66 * 4
+
+
+def test_launches_stay_within_a_grid(lib) -> None:
+    """More workgroups than a launch's 2^32 threads hold: refused before the launch."""
+    assert lib.mtpk_attention_masked_splits(1 << 24, 1, 1, 1, 64, 100, 0) == 0
+    assert lib.mtpk_attention_masked_splits((1 << 24) - 1, 1, 1, 1, 64, 100, 0) == 1
+    strides = (ctypes.c_int64 * 2)(512, 512)
+    st = ctypes.addressof(strides)
+    assert lib.mtpk_rotate(P, _mtpk.BF16, st, 1 << 26, 1, 512, None, 0, 1e-6, P, P, 64, 0, 1.0, P, st,
+                           None) == _mtpk.EINVAL
+    pools, sizes = (ctypes.c_void_p * 1)(P), (ctypes.c_int64 * 1)(1 << 40)
+    assert lib.mtpk_copy_blocks(ctypes.addressof(pools), ctypes.addressof(sizes), 1, 8, P, P, 2, 3, None) == _mtpk.EINVAL

@@ -181,3 +181,23 @@ def test_a_fork_or_compaction_in_a_capture_changes_no_table(dev) -> None:
     assert (t.host, t._free) == was[:2] and torch.equal(t.table, was[2])
     model.fork(0, 2, 21)
     assert model.compact() > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_more_pieces_than_a_launch_takes(dev, dtype) -> None:
+    """Blocks of 16 bytes in 64 pools and two more, 2^24 pieces and some: the copies go on in a second launch."""
+    n, pairs = 540000, 2**18 + 77
+    pools = [torch.randint(0, 2**40, (n, 1, 2), device=dev).view(torch.int64) for _ in range(66)]
+    order = torch.randperm(n, device=dev).to(dtype)
+    src, dst = order[:pairs].contiguous(), order[pairs : 2 * pairs].contiguous()
+    src[5], dst[pairs - 3] = -1, n  # skipped
+    live = torch.ones(pairs, dtype=torch.bool, device=dev)
+    live[5] = live[pairs - 3] = False
+    want = []
+    for p in (pools[0], pools[40], pools[63], pools[64], pools[65]):
+        w = p.clone()
+        w[dst[live].long()] = p[src[live].long()]
+        want.append(w)
+    attention.copy_blocks(pools, src, dst, 1)
+    for p, w in zip((pools[0], pools[40], pools[63], pools[64], pools[65]), want, strict=True):
+        assert torch.equal(p, w)
