@@ -1,5 +1,7 @@
 """Builds `libmtpk.so` (gfx950) in this directory with hipcc, one object per translation unit, and
-`_mtpk_torch.so`, the C++ calls on torch tensors in front of some of its entry points, with g++.
+`_mtpk_torch.so`, the C++ calls on torch tensors in front of some of its entry points, with g++. The library
+needs hipcc alone: where g++, torch or their headers are missing, it is built and the calls are left out
+with a warning.
 
 `python build_lib.py` or `build_lib.build()`; `__graft_entry__.build()` calls it. Rebuilds every
 time it is called (the build is the compile check), in parallel across translation units.
@@ -7,10 +9,13 @@ time it is called (the build is the compile check), in parallel across translati
 
 from __future__ import annotations
 
+import importlib.util
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -56,7 +61,22 @@ def _compile(src: str) -> Path:
     return obj
 
 
-def _build_torch_calls() -> None:
+def _torch_calls_need() -> str | None:
+    """What `build_torch_calls` lacks here, or None."""
+    if shutil.which("g++") is None:
+        return "g++"
+    if importlib.util.find_spec("torch") is None:
+        return "torch"
+    import torch
+
+    for header in (Path(torch.__file__).resolve().parent / "include" / "torch" / "csrc" / "utils" / "pybind.h",
+                   Path(sysconfig.get_paths()["include"]) / "Python.h"):
+        if not header.exists():
+            return str(header)
+    return None
+
+
+def build_torch_calls() -> None:
     """`_mtpk_torch.so`: host C++ against the installed torch, no device code and no link to libmtpk (its
     entry points' addresses are handed over when it is loaded)."""
     import torch
@@ -77,17 +97,21 @@ def _build_torch_calls() -> None:
 def build(verbose: bool = False) -> Path:
     OBJ_DIR.mkdir(exist_ok=True)
     with ThreadPoolExecutor(max_workers=min(7, len(SOURCES))) as pool:
-        calls = pool.submit(_build_torch_calls)
+        lacks = _torch_calls_need()
+        calls = None if lacks else pool.submit(build_torch_calls)
         objs = list(pool.map(_compile, SOURCES))
-        calls.result()
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB)
+    if calls is None:
+        warnings.warn(f"{TORCH_LIB.name} is not built: {lacks} is missing", stacklevel=2)
+    else:
+        calls.result()
     if verbose:
-        print(f"built {LIB} and {TORCH_LIB.name}")
+        print(f"built {LIB}" + ("" if calls is None else f" and {TORCH_LIB.name}"))
     return LIB
 
 
