@@ -38,6 +38,7 @@ namespace mtpk {
 
 constexpr int kTileKeys = 32;
 constexpr int kMaskedSplits = 64;       // key splits the merge takes
+constexpr int kMergeOne = 8;            // up to these, with a wave a row; beyond, a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct MaskedArgs {
@@ -1129,7 +1130,7 @@ int masked_launch(const MaskedArgs& a, int64_t batch, hipStream_t st) {
   int rc = status_of(hipGetLastError());
   if (rc || a.n_split == 1) return rc;
   const int out_rows = (int)(batch * a.heads * a.t), group_rows = (int)masked_group_rows(rows);
-  if (a.n_split <= 8)
+  if (a.n_split <= kMergeOne)
     hipLaunchKernelGGL((k_masked_merge<HD, 1>), dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, a, out_rows, group_rows);
   else
     hipLaunchKernelGGL((k_masked_merge<HD, 4>), dim3((unsigned)out_rows), dim3(256), 0, st, a, out_rows, group_rows);
@@ -1189,6 +1190,7 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
       kv_heads > 4096) return MTPK_EINVAL;
   if (!(scale > 0.f) || !(softcap >= 0.f) || !(scale < INFINITY) || !(softcap < INFINITY)) return MTPK_EINVAL;
   if (window < 0 || n_split < 1 || n_split > kMaskedSplits) return MTPK_EINVAL;
+  if (n_split > kMergeOne && batch * t * heads > kMaxGroups) return MTPK_EINVAL;  // the merge's workgroups
   if (prefix && prefix_dtype != MTPK_I32 && prefix_dtype != MTPK_I64) return MTPK_EINVAL;
   if (first && first_dtype != MTPK_I32 && first_dtype != MTPK_I64) return MTPK_EINVAL;
   // 16-byte accesses to query, gate and output rows and to the pools

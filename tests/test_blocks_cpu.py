@@ -417,3 +417,14 @@ def test_launches_stay_within_a_grid(lib) -> None:
                            None) == _mtpk.EINVAL
     pools, sizes = (ctypes.c_void_p * 1)(P), (ctypes.c_int64 * 1)(1 << 40)
     assert lib.mtpk_copy_blocks(ctypes.addressof(pools), ctypes.addressof(sizes), 1, 8, P, P, 2, 3, None) == _mtpk.EINVAL
+
+
+def test_a_merge_stays_within_a_grid(lib) -> None:
+    """Splits that the caller chose, beyond what the sizes ask for."""
+    strides = (ctypes.c_int64 * 3)(1 << 30, 64, 128)
+    st = ctypes.addressof(strides)
+    for n, t in ((9, 1 << 24), (64, (1 << 25) - 1)):
+        size = lib.mtpk_attention_masked_workspace_bytes(1, t, 1, 1, 64, n)
+        assert size > 0
+        assert lib.mtpk_paged_attention_masked(P, st, None, st, 1, t, 1, 1, 64, P, P, 160, P, 5, P, 0.1, 0.0, 0, None, None, 0, None, 0, n,
+                                               P, size, P, st, None) == _mtpk.EINVAL
