@@ -743,13 +743,12 @@ class Model:
         return len(src)
 
     def _copied(self, more: tuple[dict, ...]) -> list[torch.Tensor]:
-        """`caches`, with what `attention.copy_blocks` would refuse refused here, before a table says that the
-        blocks are copied."""
-        pools = self.caches(*more)
-        if pools:
-            n = attention.check_pools(pools, self.cfg.block_size)
-            if n != self.blocks.n_blocks:
-                raise ValueError(f"the pools have {n} blocks, the tables {self.blocks.n_blocks}")
+        """The tables' blocks of `caches` (a head's pool may hold more), with what `attention.copy_blocks` would
+        refuse refused here, before a table says that the blocks are copied."""
+        size, n = self.cfg.block_size, self.blocks.n_blocks
+        pools = [p[: n * (size if p.dim() == 3 else 1)] for p in self.caches(*more)]
+        if pools and attention.check_pools(pools, size) != n:
+            raise ValueError(f"the pools hold fewer than the tables' {n} blocks")
         return pools
 
     # ------------------------------------------------------------ sublayers

@@ -259,6 +259,21 @@ def test_model_fork_and_compact_take_the_attached_heads_cache() -> None:
     assert rounds[0] == rounds[1] and _slot_equal(model, 0, 1, 21 + len(rounds[0][0]))
 
 
+def test_a_head_with_a_longer_cache_than_the_layers() -> None:
+    model = model_helpers.build(lanes=4)
+    for name, rows in (("k", 48), ("v", 3)):
+        p = model.mtp.pool[name]
+        model.mtp.pool[name] = torch.cat([p, torch.full((rows, *p.shape[1:]), 7.0)])
+    model.prefill(2, model_helpers.prompts(1, 40, seed=6)[0])
+    model.prefill(0, model_helpers.prompts(1, 21)[0])
+    model.fork(0, 1, 21)
+    model.reset(2)
+    before = [x.clone() for x in model_helpers.slot_state(model, 0, 21)]
+    assert _slot_equal(model, 0, 1, 21) and model.compact() > 0
+    assert all(torch.equal(x, y) for x, y in zip(before, model_helpers.slot_state(model, 1, 21), strict=True))
+    assert bool((model.mtp.pool["k"][-48:] == 7.0).all()) and bool((model.mtp.pool["v"][-3:] == 7.0).all())
+
+
 def test_caches_name_each_pool_once() -> None:
     model = model_helpers.build()
     pools = model.caches()
