@@ -18,7 +18,9 @@
 //
 // Sums and statistics are fp32. P is rounded to bf16 for the second product, and the row sum adds the
 // rounded values, so that a row's weights sum to 1 as they are used. The output, with its gate, is
-// rounded once.
+// rounded once: 1.9e-3 to 2.4e-3 of the 2-norm from 64 bits, where the output's rounding alone makes 1.7e-3. P in two
+// bf16 parts, a second product for the rest, comes down to that; it took 5 % more for a short context of one lane, 1 %
+// for 48 lanes in a window, 2 to 8 % for verify rows, and prompts, half products as they are, would pay most.
 //
 // Keys that a row does not see may hold anything: their scores are replaced, and V is zeroed where no row of
 // the workgroup sees the key. Nor do finite ones that no row sees choose the form in which a tile's scores are capped;
@@ -449,9 +451,10 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
 // O^T of tile t stand the exponents of tile t, spread evenly, between the others the scan of tile t + 1. Heads
 // of 256, whose sums fill the registers, have half of a tile's exponents between its own O^T's products.
 //
-// 8000 rows of 16 heads of 128: 314-335 us by box, 0.93 PFLOP/s of visible products, at 1.9 GHz: the card's power bounds
-// it (work that took 9 % of the cycles away made it 3 % faster), 42 % of the cycles being products. 4095 rows of 32
-// heads of 256 in documents of 700, gated: 89 us, 46 us of which the rows, gates and outputs take from memory at the copy
+// 8000 rows of 16 heads of 128: 306-335 us by box, 0.93 PFLOP/s of visible products, at 1.9 GHz, 45 % of the cycles being
+// products: 70 cycles a product, of which the same mix of instructions alone takes 50 at 1.77 GHz (the card's power), and
+// the rest are stalls, bank conflicts in a third of the LDS cycles among them. 4095 rows of 32
+// heads of 256 in documents of 700, gated: 84-90 us, 46 us of which the rows, gates and outputs take from memory at the copy
 // rate; a workgroup spends 7 us on its rows, 19 on 12 tiles, 11 on gates and outputs, and the card holds just two
 // rounds of them. Left out: two sets of 32 rows a wave, which read each operand once for both but leave one wave a
 // SIMD (heads of 128: 317 -> 361 us); three waves a SIMD there (453 -> 477, an earlier form).
