@@ -1234,7 +1234,8 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
   if (softcap > 0.f) {
     // tanh(u) / u by polynomials in u^2 of least relative error: 8.4e-6 on |u| <= 0.15, which is 9e-5 of an exponent
     // at cap 50 (a rounded probability is off by up to 2^-8), and 4e-7 on |u| <= 0.25
-    const double k = (double)scale / softcap, c = (double)softcap * 1.4426950408889634;
+    // (scores of 1e-30 caps are as good as infinite ones: the constants, and a score of 0 times them, stay finite)
+    const double k = std::min((double)scale / softcap, 1e30), c = (double)softcap * 1.4426950408889634;
     a.cap2 = (float)std::min(c, 1.7e38);  // twice it stays finite
     a.cap_in = (float)(2. * 1.4426950408889634 * k);
     a.cubic_max = (float)(0.15 / k);
@@ -1244,7 +1245,7 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
     a.e2 = (float)(c * k * 0.12841935);
     if (c <= kCapMost) {
       a.c0 = (float)(c * k * 0.99999165);
-      a.c1 = (float)(c * k * k * k * -0.33035765);
+      a.c1 = (float)std::max(c * k * k * k * -0.33035765, -3e38);
     }
   }
   a.part_o = (float*)workspace;

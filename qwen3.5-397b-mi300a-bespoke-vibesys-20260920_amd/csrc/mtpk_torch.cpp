@@ -248,6 +248,7 @@ Tensor paged_attention_masked(const Tensor& q_in, const Tensor& k_pool, const Te
        cache.table.size(1), " blocks");
   need(scale > 0 && std::isfinite(scale) && softcap >= 0 && std::isfinite(softcap) && window >= 0,
        "scale must be positive, softcap and window not negative, got ", scale, ", ", softcap, " and ", window);
+  need(softcap == 0 || (float)softcap > 0, "softcap ", softcap, " is below float32's range, where 0 means none");
   std::optional<Tensor> gate, slopes;
   if (gate_in) {
     need(gate_in->sizes() == q_in.sizes() && gate_in->scalar_type() == at::kBFloat16, "gate must be bf16 of q's shape");

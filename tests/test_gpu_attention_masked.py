@@ -158,6 +158,18 @@ def test_caps_far_above_the_scores(dev, heads, kvh, hd, t, base, softcap) -> Non
         assert float(((got - want).abs() / bars(want, spread)).max()) <= 1.0
 
 
+@pytest.mark.parametrize("heads,kvh,hd,t,base", [(8, 2, 64, 1, [40]), (16, 4, 128, 9, [40]), (32, 2, 256, 40, [9])])
+def test_caps_far_below_the_scores(dev, heads, kvh, hd, t, base) -> None:
+    """All weights equal, those of scores of 0 among them; a cap that float32 does not hold is refused."""
+    q, k, v, table, b0 = case(1, 1, t, heads, kvh, hd, base)
+    q[:, :, 1] = 0
+    k[::3] = 0
+    for softcap in (1e-6, 1e-13, 1e-20, 1e-30, 1e-38, 1e-42):
+        check(dev, q, k, v, table, b0, hd**-0.5, softcap=softcap)
+    with pytest.raises(ValueError):
+        run(dev, q, k, v, table, b0, hd**-0.5, softcap=1e-50)
+
+
 def test_scores_of_a_wide_caps_size(dev) -> None:
     """Scores around and above a quarter of caps of some hundreds, where the cap's two forms meet."""
     for softcap in (100.0, 400.0):
