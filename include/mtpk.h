@@ -705,6 +705,78 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
 int mtpk_copy_blocks(void* const* pools, const int64_t* block_bytes, int n_pools, int64_t n_blocks,
                      const void* src, const void* dst, int index_dtype, int64_t pairs, void* stream);
 
+/* ---------------------------------------------------------------- trees of drafts
+ * A verify round whose drafts branch. Every entry point takes a tree as parents (parents_dtype int32 | int64):
+ * node s of lane b at parents[b * parents_strides[0] + s * parents_strides[1]] (host array of two element strides;
+ * 0 for lanes that share a tree), t <= 64 nodes. A parent is an earlier node (0 <= parent < s) or -1, the committed
+ * context; any other value marks an absent node, and what hangs below an absent node is absent. Absent nodes' outputs are
+ * zeros. No reference counterpart (its drafts are chains).
+ *
+ * Attention: mtpk_paged_attention_gated's operands. Node s of lane b has its key and value at cache position
+ * base_pos[b] + s; it sees every position below base_pos[b], and of the nodes itself and its ancestors. Sums and statistics
+ * fp32, probabilities bf16, the output (times sigmoid(gate) when gate is given) rounded once. What a node does not see may
+ * hold anything. n_split from mtpk_attention_tree_splits (0: a shape that is not taken; max_ctx a bound on base_pos + t), at
+ * most 64; n_split > 1 needs mtpk_attention_tree_workspace_bytes of workspace (16-byte aligned). Limits as
+ * mtpk_paged_attention_masked's. */
+int mtpk_attention_tree_splits(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_ctx);
+int64_t mtpk_attention_tree_workspace_bytes(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                            int n_split);
+int mtpk_paged_attention_tree(const uint16_t* q, const int64_t* q_strides, const uint16_t* gate, const int64_t* gate_strides,
+                              int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim, const uint16_t* k_pool,
+                              const uint16_t* v_pool, int64_t pool_rows, const int32_t* block_table, int64_t table_stride,
+                              const int64_t* base_pos, float scale, const void* parents, int parents_dtype,
+                              const int64_t* parents_strides, int n_split, void* workspace, int64_t workspace_bytes, uint16_t* out,
+                              const int64_t* out_strides, void* stream);
+
+/* mtpk_deltanet_prep for a tree's rows: the convolution's columns before a node are its ancestors', then the stored
+ * window's. Same operands and outputs; k_dim, v_dim <= 256, conv_k 2..9. bf16 rows' convolution is rounded to bf16 as its
+ * exact value is, next to a border too (mtpk_deltanet_prep: as its fp32 value is). A slot outside the pool reads a zero window. */
+int mtpk_deltanet_prep_tree(const void* proj, int dtype, int64_t proj_stride, const void* conv_state, const int64_t* slot,
+                            int64_t slots_total, const void* conv_w, const float* a_log, const float* dt_bias, const void* parents,
+                            int parents_dtype, const int64_t* parents_strides, int64_t batch, int64_t t, int64_t k_heads,
+                            int64_t k_dim, int64_t v_heads, int64_t v_dim, int64_t conv_k, float eps, float q_scale, float* q,
+                            float* k, float* v, float* g, float* beta, void* stream);
+
+/* mtpk_delta_rule's verify mode for a tree: node s runs one step on its parent's state (-1: its slot's stored one),
+ * out [rows, t, heads, v_dim] holds every node's output; the stored states are read alone. slot may be NULL (row j: slot j);
+ * rows of a slot outside the pool give zeros. */
+int mtpk_delta_rule_tree(const float* state, int64_t slots_total, const int64_t* slot, int64_t rows, int64_t t, int64_t heads,
+                         int64_t qk_heads, int64_t k_dim, int64_t v_dim, const float* q, const float* k, const float* v,
+                         const float* g, const float* beta, const void* parents, int parents_dtype, const int64_t* parents_strides,
+                         float* out, void* stream);
+
+/* mtpk_deltanet_commit along a path: slot[j]'s state runs the rows path[j * t + i], i < lengths[j], of the call, and its
+ * conv window becomes the last k1 columns of [stored window | those rows' first `channels` of proj]. path int64 [rows, t],
+ * t <= 64; an entry outside [0, t) ends the path. A slot outside the pool is skipped; slots must be distinct. */
+int mtpk_deltanet_commit_path(float* state, int64_t slots_total, const int64_t* slot, int64_t rows, int64_t t, int64_t heads,
+                              int64_t qk_heads, int64_t k_dim, int64_t v_dim, const float* k, const float* v, const float* g,
+                              const float* beta, const int64_t* path, const int64_t* lengths, void* conv_state, int conv_dtype,
+                              int64_t conv_slots_total, const void* proj, int64_t proj_stride, int64_t channels, int64_t k1,
+                              void* stream);
+
+/* Greedy acceptance of a path (mtpk_greedy_accept for a tree): from node 0, the lane's own token, to the lowest child
+ * whose token is step_argmax of the node it hangs below, and so on while there is one, that argmax is none of the lane's
+ * stop ids and fewer than budget - 1 drafts are accepted. step_argmax, tokens int64 [batch, t] (row strides given, unit
+ * column stride); stops int64 [batch, n_stops], -1 padded. Outputs, contiguous: path int64 [batch, t] (node 0, then the
+ * accepted ones; the last repeated behind them), accept_len int64 [batch] (accepted drafts), lengths (accept_len + 1, 1
+ * on inactive lanes), keep u8 [batch, t] (active and i <= accept_len), bonus (step_argmax of the last accepted node),
+ * next_pos = pos + accept_len + 1, budget_left = budget - accept_len - 1, live u8 (bonus is no stop and budget_left > 0),
+ * hidden_src = b * t + the last accepted node. */
+int mtpk_tree_accept(const int64_t* step_argmax, int64_t sa_stride, const int64_t* tokens, int64_t tokens_stride,
+                     const void* parents, int parents_dtype, const int64_t* parents_strides, const uint8_t* active,
+                     const int64_t* pos, const int64_t* budget, const int64_t* stops, int64_t n_stops, int64_t batch, int64_t t,
+                     int64_t* path, int64_t* accept_len, int64_t* lengths, uint8_t* keep, int64_t* bonus, int64_t* next_pos,
+                     int64_t* budget_left, uint8_t* live, int64_t* hidden_src, void* stream);
+
+/* The accepted rows together: cache row base_pos[b] + path[b * t + i] becomes row base_pos[b] + i, for i < lengths[b],
+ * in each of n_pools pools (host arrays: addresses, 16-byte aligned; channels = kv_heads * head_dim; element bytes, 2 or 4;
+ * transposed 0: a K pool [n_blocks * 16, channels], its rows a multiple of 16 bytes, 1: a V pool [n_blocks, channels, 16]).
+ * A path rises (int64 [batch, t], t <= 64); an entry outside [0, t) ends it, and a row whose position lies outside the
+ * lane's table or whose block lies outside the pools is left. */
+int mtpk_keep_path(void* const* pools, const int64_t* channels, const int* element_bytes, const int* transposed, int n_pools,
+                   int64_t n_blocks, const int32_t* block_table, int64_t table_stride, const int64_t* base_pos,
+                   const int64_t* path, const int64_t* lengths, int64_t batch, int64_t t, void* stream);
+
 /* Streaming-read probe (no reference counterpart: a measurement of the HBM read ceiling the MoE
  * weight streams are compared with). Reads bytes [0, bytes) of `base` with 16-byte loads,
  * `loads_in_flight` (4, 8 or 16) per thread per iteration, over `grid` workgroups of 256

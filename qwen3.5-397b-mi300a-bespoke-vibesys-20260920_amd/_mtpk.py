@@ -242,6 +242,42 @@ _SIGNATURES: dict[str, tuple[object, list]] = {
          c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
     ),
     "mtpk_copy_blocks": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p]),
+    "mtpk_attention_tree_splits": (c_int, [c_int64] * 6),
+    "mtpk_attention_tree_workspace_bytes": (c_int64, [c_int64] * 5 + [c_int]),
+    "mtpk_paged_attention_tree": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+         c_void_p, c_int64, c_void_p, c_int64, c_void_p, ctypes.c_float, c_void_p, c_int, c_void_p, c_int,
+         c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
+    ),
+    "mtpk_deltanet_prep_tree": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+         c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, ctypes.c_float, ctypes.c_float, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "mtpk_delta_rule_tree": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
+    ),
+    "mtpk_deltanet_commit_path": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64,
+         c_int64, c_int64, c_void_p],
+    ),
+    "mtpk_tree_accept": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "mtpk_keep_path": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+         c_void_p, c_int64, c_int64, c_void_p],
+    ),
     "mtpk_probe_stream": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),
     "mtpk_delta_rule": (
         c_int,
@@ -298,7 +334,10 @@ def lib() -> ctypes.CDLL:
 
 _native = None
 _NATIVE_ENTRIES = ("mtpk_status_string", "mtpk_rotate", "mtpk_rotate_to_cache", "mtpk_attention_masked_splits",
-                   "mtpk_attention_masked_workspace_bytes", "mtpk_paged_attention_masked", "mtpk_copy_blocks")
+                   "mtpk_attention_masked_workspace_bytes", "mtpk_paged_attention_masked", "mtpk_copy_blocks",
+                   "mtpk_attention_tree_splits", "mtpk_attention_tree_workspace_bytes", "mtpk_paged_attention_tree",
+                   "mtpk_deltanet_prep_tree", "mtpk_delta_rule_tree", "mtpk_deltanet_commit_path", "mtpk_tree_accept",
+                   "mtpk_keep_path")
 
 
 def native():

@@ -201,6 +201,22 @@ def paged_attention_masked(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
                                                  slopes, prefix, first, gate, _mtpk.stream_for(q))
 
 
+def paged_attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                         base_pos: torch.Tensor, ctx_len: int, scale: float, parents: torch.Tensor, *,
+                         gate: torch.Tensor | None = None) -> torch.Tensor:
+    """`paged_attention_gated` of a tree of up to 64 drafts per lane (`mtpk_paged_attention_tree`). q `[B, t, heads,
+    hd]`, any strides; returns `[B, t, heads, hd]` contiguous.
+
+    `parents` int32 or int64 `[B, t]`, any strides (one tree for all lanes: expanded): node s hangs below the earlier node
+    `parents[b, s]`, or below the committed context at -1. Any other value marks an absent node, and what hangs below
+    one is absent: such rows are zeros. Node s of lane b has its key and value at cache position `base_pos[b] + s`, whatever its
+    depth. It sees every position below `base_pos[b]`, itself and its ancestors; other keys may hold anything.
+    `gate` of q's shape multiplies the output by its sigmoid. `ctx_len` is a host bound on `max(base_pos) + t`; it sizes the key
+    splits alone. bf16 with fp32 scores, statistics and sums; the output is rounded once."""
+    return _mtpk.native().paged_attention_tree(q, k_pool, v_pool, block_table, base_pos, ctx_len, scale, parents, gate,
+                                               _mtpk.stream_for(q))
+
+
 def _not_captured(device: torch.device) -> None:
     if device.type == "cuda":
         with torch.cuda.device(device):
@@ -277,3 +293,48 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
         return
     pairs = torch.stack((src, dst)).pin_memory().to(device, non_blocking=True)
     _mtpk.native().copy_blocks(pools, pairs[0], pairs[1], block, _mtpk.stream_for(pairs))
+
+
+def keep_path(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: torch.Tensor, path: torch.Tensor,
+              lengths: torch.Tensor) -> None:
+    """The accepted rows of verified trees, moved together: of lane b, cache position `base_pos[b] + path[b, i]` becomes
+    position `base_pos[b] + i` for `i < lengths[b]`, in every pool in one launch (`mtpk_keep_path`): K pools `[rows, kv_heads,
+    hd]` and V pools `[rows / 16, kv_heads, hd, 16]` of one cache's layers, read through the lanes' `block_table` `[B, blocks]`.
+
+    `path` int32 or int64 `[B, t]`, t up to 64, rises in its first `lengths[b]` entries (`graph_mtp.tree_accept`); an entry
+    that is no node of `[0, t)` ends it. Rows outside the lane's table, and blocks outside the pools, are left.
+    CPU pools take the torch spelling."""
+    if pools and not pools[0].is_cuda:
+        _keep_path_torch(pools, block_table, base_pos, path, lengths)
+        return
+    if not pools:
+        raise ValueError("keep_path takes at least one pool")
+    _mtpk.native().keep_path(pools, block_table, base_pos, path, lengths, _mtpk.stream_for(pools[0]))
+
+
+def _keep_path_torch(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: torch.Tensor, path: torch.Tensor,
+                     lengths: torch.Tensor) -> None:
+    n_blocks = _pool_blocks(pools, BLOCK)
+    if path.dim() != 2 or not 1 <= path.shape[1] <= 64:
+        raise ValueError(f"path must be [B, 1 to 64], got {tuple(path.shape)}")
+    b, t = path.shape
+    if block_table.dim() != 2 or block_table.shape[0] != b or tuple(base_pos.shape) != (b,) or tuple(lengths.shape) != (b,):
+        raise ValueError(f"block_table must be [{b}, blocks], base_pos and lengths [{b}]")
+    for name, x in (("block_table", block_table), ("base_pos", base_pos), ("path", path), ("lengths", lengths)):
+        if x.dtype not in (torch.int32, torch.int64) or x.is_cuda:
+            raise ValueError(f"{name} must be int32 or int64 beside the pools, got {x.dtype} on {x.device}")
+    node = torch.arange(t)
+    path, base, table = path.long(), base_pos.long()[:, None], block_table.long()
+    on = ((path >= 0) & (path < t)).int().cumprod(1).bool() & (node < lengths[:, None])
+    src, dst = (base + x for x in (path, node.expand(b, t)))
+    end = table.shape[1] * BLOCK
+    on &= (src >= 0) & (src < end) & (dst >= 0) & (dst < end)
+    at = [(table.gather(1, x.clamp(0, end - 1) // BLOCK), x % BLOCK) for x in (src, dst)]
+    for blocks, _ in at:
+        on &= (blocks >= 0) & (blocks < n_blocks)
+    (sb, sr), (db, dr) = ((blocks[on], rows[on]) for blocks, rows in at)
+    for p in pools:
+        if p.dim() == 3:
+            p[db * BLOCK + dr] = p[sb * BLOCK + sr]
+        else:
+            p[db, :, :, dr] = p[sb, :, :, sr]

@@ -35,6 +35,7 @@
 
 #include "mtpk_attention_common.h"
 #include "mtpk_host.h"
+#include "mtpk_tree.h"
 
 namespace mtpk {
 
@@ -70,11 +71,14 @@ struct MaskedArgs {
   float cubic_max, c0, c1, cap_k, e0, e1, e2;
   float* part_o;
   float* part_ml;
+  TreeParents tree;  // the TREE form alone
 };
 
-// The keys [lo, hi) that a row sees, and its position (for distances).
+// The keys [lo, hi) that a row sees, and its position (for distances); in a tree of the keys from `pos` on, the lane's
+// first node, only those whose bits are set.
 struct RowKeys {
   int pos, lo, hi;
+  uint64_t nodes;
 };
 
 __device__ inline RowKeys masked_row(const MaskedArgs& a, int b, int s) {
@@ -92,7 +96,21 @@ __device__ inline RowKeys masked_row(const MaskedArgs& a, int b, int s) {
   lo = min(lo, (int64_t)INT32_MAX);
   // A row past the table is as if at its end: one distance more or less for all of its keys is no change, and
   // int and float hold the others' differences.
-  return RowKeys{(int)min(pos, end), (int)lo, (int)hi};
+  return RowKeys{(int)min(pos, end), (int)lo, (int)hi, 0ull};
+}
+
+// A tree's row: the lane's whole context, then nodes by their bits. (An absent node's row, without bits, goes along as if it
+// saw the context, and is done again in the end, which makes it zeros.)
+__device__ inline RowKeys tree_row(const MaskedArgs& a, int b) {
+  const int64_t base = a.base[b], end = a.table_stride * kAttnBlock;
+  return RowKeys{(int)min(max(base, (int64_t)0), end), 0, (int)max(min(base + a.t, end), (int64_t)0), 0ull};
+}
+
+// Bit i: whether the row sees key key0 + i, for keys below `end`.
+__device__ inline uint32_t tree_seen(const RowKeys& row, int key0) {
+  const int at = key0 - row.pos, left = row.hi - key0;
+  uint64_t w = at >= kTreeNodes ? 0ull : at >= 0 ? row.nodes >> at : at <= -32 ? ~0ull : row.nodes << -at | ((1ull << -at) - 1ull);
+  return left >= 32 ? (uint32_t)w : left <= 0 ? 0u : (uint32_t)w & ((1u << left) - 1u);
 }
 
 // Over the 16 lanes of a row by DPP, then the two rows of a half.
@@ -241,7 +259,7 @@ __device__ inline float halves_max(float v) {
 
 // One tile of scores on its way to P, in steps that the caller puts between its products: scan (every value once),
 // finish, and each value's exponent.
-template <bool CAP, bool SLOPES>
+template <bool CAP, bool SLOPES, bool TREE = false>
 struct TileSoftmax {
   float c0, c1, ms;  // exponent of a score s: s (c0 + c1 s^2) with a cap, s c0 - ms without one
   float top;         // the largest score, with a cap the largest magnitude
@@ -258,7 +276,13 @@ struct TileSoftmax {
     c0 = a.c0;
     c1 = a.c1;
     const int lo = row.lo - key0 - 8 * h, n = max(row.hi - row.lo, 0);  // seen: 0 <= i - lo < n, in one comparison
-    auto seen = [&](int i) { return (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)n; };
+    const uint32_t bits = TREE && !whole ? tree_seen(row, key0 + 8 * h) : 0u;
+    auto seen = [&](int i) {
+      if constexpr (TREE)
+        return (bits >> (16 * (i >> 3) + (i & 7)) & 1u) != 0u;
+      else
+        return (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)n;
+    };
     auto past = [&]() { return __ballot(!(top <= a.cubic_max)) != 0ull; };
     bool bent = CAP ? past() : a.cap2 > 0.f;  // past the cap's cubic part
     if (CAP && bent && !whole) {  // keys that no row sees have no part in the choice of the form
@@ -380,10 +404,14 @@ __device__ inline void store_out8(const MaskedArgs& a, int b, int hq, int st, in
 // One row by one wave, key by key in fp32 straight from memory: for the rows whose result above is not
 // finite (a value or score that is not, seen by this row or by another one that shares its tiles), or
 // whose keys all weigh too little. What the row does not see is not read.
-template <int HD>
+template <int HD, bool TREE = false>
 __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, int lane) {
   constexpr int NV = HD / kWave;
-  const RowKeys row = masked_row(a, b, step);
+  RowKeys row = TREE ? tree_row(a, b) : masked_row(a, b, step);
+  if (TREE) {
+    row.nodes = lane_bits(tree_ancestors(a.tree.at(b, lane, a.t), lane), step);
+    if (row.nodes == 0ull) row.hi = row.lo;
+  }
   const int kh = hq / (a.heads / a.kvh);
   const uint16_t* const q = a.q + a.qr.at(b, hq, step);
   const int32_t* const trow = a.table + (int64_t)b * a.table_stride;
@@ -394,7 +422,8 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
 #pragma unroll 1
   for (int key0 = row.lo; key0 < row.hi; key0 += kWave) {
     const int key = key0 + lane;
-    const bool live = key < row.hi;
+    bool live = key < row.hi;
+    if (TREE && key >= row.pos) live = live && (row.nodes >> (key - row.pos & 63) & 1ull);
     const int id = live ? trow[key / kAttnBlock] : -1;
     const bool held = (uint32_t)id < a.pool_blocks;  // else the block reads as zeros
     float s = 0.f;
@@ -440,6 +469,7 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
   for (int e = 0; e < NV; ++e) {
     const float y = acc[e] * inv + odd[e];
     to[e] = f32_to_bf16(gate ? y * sigmoid_of(gate[e]) : y);
+    if (TREE && row.hi <= row.lo) to[e] = 0;  // an absent node, whatever its gate holds
   }
 }
 
@@ -458,7 +488,7 @@ __device__ void masked_row_slow(const MaskedArgs& a, int b, int hq, int step, in
 // rate; a workgroup spends 7 us on its rows, 19 on 12 tiles, 11 on gates and outputs, and the card holds just two
 // rounds of them. Left out: two sets of 32 rows a wave, which read each operand once for both but leave one wave a
 // SIMD (heads of 128: 317 -> 361 us); three waves a SIMD there (453 -> 477, an earlier form).
-template <int HD, int W, bool CAP, bool SLOPES>
+template <int HD, int W, bool CAP, bool SLOPES, bool TREE = false>
 __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
   using G = TileGeom<HD>;
   constexpr bool AHEAD = HD <= 128;
@@ -491,21 +521,32 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
 #pragma unroll
     for (int s = 0; s < G::kS; ++s) qd[s] = ld16(qrow + 16 * s);
   }
-  RowKeys row = masked_row(a, b, step);
-  RowSet set = row_set(row);
-  if (lane == 0) {
-    wg_lo[wave] = set.lo_min;
-    wg_hi[wave] = set.hi_max;
-  }
-  __syncthreads();
-  int lo = wg_lo[0], hi = wg_hi[0];
+  RowKeys row;
+  RowSet set;
+  int lo, hi;
+  if constexpr (TREE) {  // the same keys for all rows
+    row = tree_row(a, b);
+    lo = 0;
+    hi = uniform(row.hi);
+    set = RowSet{0, 0, min(uniform(row.pos), hi), hi};
+  } else {
+    row = masked_row(a, b, step);
+    set = row_set(row);
+    if (lane == 0) {
+      wg_lo[wave] = set.lo_min;
+      wg_hi[wave] = set.hi_max;
+    }
+    __syncthreads();
+    lo = wg_lo[0];
+    hi = wg_hi[0];
 #pragma unroll
-  for (int w = 1; w < W; ++w) {
-    lo = min(lo, wg_lo[w]);
-    hi = max(hi, wg_hi[w]);
+    for (int w = 1; w < W; ++w) {
+      lo = min(lo, wg_lo[w]);
+      hi = max(hi, wg_hi[w]);
+    }
+    lo = uniform(lo);
+    hi = uniform(hi);
   }
-  lo = uniform(lo);
-  hi = uniform(hi);
   int tile0, tiles;
   masked_split(lo, hi, a.n_split, sp, tile0, tiles);
   tile0 = uniform(tile0);
@@ -589,6 +630,10 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     static_for<2 * kMine>([&](auto j) { load(buf0, key0, j); });
     blocks(key0 + kStageKeys);
   }
+  if constexpr (TREE) {
+    const uint64_t nodes = tree_ancestors(a.tree.at(b, lane, a.t), lane);
+    row.nodes = (uint64_t)(uint32_t)__shfl((int)(nodes >> 32), step, kWave) << 32 | (uint32_t)__shfl((int)nodes, step, kWave);
+  }
   bf16x8_t q[G::kS - QL];
 #pragma unroll
   for (int s = 0; s < G::kS; ++s) {
@@ -599,7 +644,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
       lds16_store(q_mine + s * 1024, qd[s]);
   }
 
-  TileSoftmax<CAP, SLOPES> soft_tile;
+  TileSoftmax<CAP, SLOPES, TREE> soft_tile;
   u32x4_t p[2], f[RD];
   const f32x16_t zero = {};
   auto kfrag = [&](const uint8_t* k, int i) { return lds16(k + (kat ^ (32u * (i & 3))) + 128 * (i >> 2)); };
@@ -737,7 +782,8 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     if (key0 >= end) break;
     stage(buf1, buf0);
   }
-  const float l = soft.l + __shfl_xor(soft.l, 32, kWave);
+  float l = soft.l + __shfl_xor(soft.l, 32, kWave);
+  if (TREE && row.nodes == 0ull) l = 0.f;
   const bool real = row0 + c < R;
   // o[dt][4 i + e] is channel 32 dt + 8 i + 4 h + e of the row
   if (a.n_split == 1) {
@@ -792,7 +838,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
     while (again != 0ull) {
       const int rl = uniform(__builtin_ctzll(again)), ro = row0 + rl;
       again &= again - 1ull;
-      masked_row_slow<HD>(a, b, kh * group + ro % group, ro / group, lane);
+      masked_row_slow<HD, TREE>(a, b, kh * group + ro % group, ro / group, lane);
     }
   } else {
     if (!real) return;
@@ -819,7 +865,7 @@ __global__ __launch_bounds__(W* kWave, 2) void k_masked_rows(MaskedArgs a) {
 // all of the rows, and stage it for themselves alone: no barrier until their results are merged. K's
 // place is loaded again as soon as the first product has read it, V's after the second. 48 lanes of 2 kv heads of 256,
 // windows of 4096: 81 us with the merge, 5.2 TB/s in this kernel; 65,000 and 31,000 keys of 4 kv heads of 128: 50 us.
-template <int HD, int W, bool CAP, bool SLOPES>
+template <int HD, int W, bool CAP, bool SLOPES, bool TREE = false>
 __global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
   using G = TileGeom<HD>;
   __shared__ __attribute__((aligned(16))) uint8_t smem[W][G::kKTile + G::kTile];  // a wave's K and V tile
@@ -837,8 +883,8 @@ __global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
 #pragma unroll
     for (int s = 0; s < G::kS; ++s) qd[s] = ld16(qrow + 16 * s);
   }
-  const RowKeys row = masked_row(a, b, step);
-  const RowSet set = row_set(row);
+  RowKeys row = TREE ? tree_row(a, b) : masked_row(a, b, step);
+  const RowSet set = TREE ? RowSet{0, 0, min(uniform(row.pos), uniform(row.hi)), uniform(row.hi)} : row_set(row);
   const int lo = set.lo_min, hi = set.hi_max;
   const float slope2 = SLOPES ? a.slopes[hq] * kLog2e : 0.f;
   int tile0, tiles;
@@ -894,6 +940,10 @@ __global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
     b0 = block(key0 + kStep, 0);
     b1 = block(key0 + kStep, 1);
   }
+  if constexpr (TREE) {
+    const uint64_t nodes = tree_ancestors(a.tree.at(b, lane, a.t), lane);
+    row.nodes = (uint64_t)(uint32_t)__shfl((int)(nodes >> 32), step, kWave) << 32 | (uint32_t)__shfl((int)nodes, step, kWave);
+  }
   bf16x8_t q[G::kS];
 #pragma unroll
   for (int s = 0; s < G::kS; ++s) {
@@ -922,7 +972,7 @@ __global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
     }
     if (more) stage_k(key0 + kStep, b0, b1);  // every read of K went into a product above
     ring_fence();
-    TileSoftmax<CAP, SLOPES> soft_tile;
+    TileSoftmax<CAP, SLOPES, TREE> soft_tile;
     u32x4_t p[2];
     const float alpha = soft_tile.prepare(a, s, row, slope2, set.whole(key0), key0, h, soft);
     static_for<16>([&](auto i) { soft_tile.template exponent<i>(s, p, soft); });
@@ -960,7 +1010,8 @@ __global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
     }
   }
   // The waves' results through their own tiles' LDS: 32 rows of HD floats.
-  const float l = soft.l + __shfl_xor(soft.l, 32, kWave);
+  float l = soft.l + __shfl_xor(soft.l, 32, kWave);
+  if (TREE && row.nodes == 0ull) l = 0.f;
   constexpr int kRow = HD * 4, kFlip = HD / 4 - 1;
 #pragma unroll
   for (int dt = 0; dt < G::kT; ++dt)
@@ -1020,14 +1071,14 @@ __global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
   if (a.n_split > 1) return;
   __syncthreads();
   for (int rl = wave; rl < min(R, 32); rl += W) {
-    if (uniform(again[rl]) != 0) masked_row_slow<HD>(a, b, kh * group + rl % group, rl / group, lane);
+    if (uniform(again[rl]) != 0) masked_row_slow<HD, TREE>(a, b, kh * group + rl % group, rl / group, lane);
   }
 }
 
 // Merge of the key splits: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M = max_s m_s. W waves a
 // row: each weighs all splits at once (lane s split s), then takes every W-th split, four of them in
 // flight; the waves' sums are added in order.
-template <int HD, int W>
+template <int HD, int W, bool TREE = false>
 __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, int group_rows) {
   constexpr int NV = HD / kWave;
   typedef float vec_t __attribute__((ext_vector_type(NV)));
@@ -1075,7 +1126,7 @@ __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, in
     odd = fmaf(y, 0.f, odd);
     orow[e] = f32_to_bf16(grow ? y * sigmoid_of(grow[e]) : y);
   }
-  if (__ballot(odd != 0.f) != 0ull) masked_row_slow<HD>(a, b, hq, st, lane);
+  if (__ballot(odd != 0.f) != 0ull) masked_row_slow<HD, TREE>(a, b, hq, st, lane);
 }
 
 namespace {
@@ -1109,34 +1160,34 @@ int masked_splits(int64_t batch, int64_t kvh, int64_t rows, int64_t hd, int64_t 
   return n < 1 ? 1 : (int)n;
 }
 
-template <int HD, bool CAP, bool SLOPES>
+template <int HD, bool CAP, bool SLOPES, bool TREE>
 void masked_few_launch(const MaskedArgs& a, dim3 grid, hipStream_t st) {
   if constexpr (HD < 256) {
     if (masked_eight(a.lanes_kvh, HD)) {
-      hipLaunchKernelGGL((k_masked_few<HD, 8, CAP, SLOPES>), grid, dim3(512), 0, st, a);
+      hipLaunchKernelGGL((k_masked_few<HD, 8, CAP, SLOPES, TREE>), grid, dim3(512), 0, st, a);
       return;
     }
   }
-  hipLaunchKernelGGL((k_masked_few<HD, 4, CAP, SLOPES>), grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_masked_few<HD, 4, CAP, SLOPES, TREE>), grid, dim3(256), 0, st, a);
 }
 
-template <int HD, bool CAP, bool SLOPES>
+template <int HD, bool CAP, bool SLOPES, bool TREE = false>
 int masked_launch(const MaskedArgs& a, int64_t batch, hipStream_t st) {
   const int64_t rows = (int64_t)(a.heads / a.kvh) * a.t;
   const dim3 grid((unsigned)(batch * a.kvh * a.row_groups), (unsigned)a.n_split);
   if (rows <= 32)
-    masked_few_launch<HD, CAP, SLOPES>(a, grid, st);
+    masked_few_launch<HD, CAP, SLOPES, TREE>(a, grid, st);
   else if (rows <= 64)
-    hipLaunchKernelGGL((k_masked_rows<HD, 2, CAP, SLOPES>), grid, dim3(128), 0, st, a);
+    hipLaunchKernelGGL((k_masked_rows<HD, 2, CAP, SLOPES, TREE>), grid, dim3(128), 0, st, a);
   else
-    hipLaunchKernelGGL((k_masked_rows<HD, 4, CAP, SLOPES>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_masked_rows<HD, 4, CAP, SLOPES, TREE>), grid, dim3(256), 0, st, a);
   int rc = status_of(hipGetLastError());
   if (rc || a.n_split == 1) return rc;
   const int out_rows = (int)(batch * a.heads * a.t), group_rows = (int)masked_group_rows(rows);
   if (a.n_split <= kMergeOne)
-    hipLaunchKernelGGL((k_masked_merge<HD, 1>), dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, a, out_rows, group_rows);
+    hipLaunchKernelGGL((k_masked_merge<HD, 1, TREE>), dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, a, out_rows, group_rows);
   else
-    hipLaunchKernelGGL((k_masked_merge<HD, 4>), dim3((unsigned)out_rows), dim3(256), 0, st, a, out_rows, group_rows);
+    hipLaunchKernelGGL((k_masked_merge<HD, 4, TREE>), dim3((unsigned)out_rows), dim3(256), 0, st, a, out_rows, group_rows);
   return status_of(hipGetLastError());
 }
 
@@ -1151,6 +1202,55 @@ bool masked_shape(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int
   return batch > 0 && t > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
          (head_dim == 64 || head_dim == 128 || head_dim == 256) && batch <= INT32_MAX / 64 / t &&
          heads <= INT32_MAX / 64 / (batch * t) && batch * kv_heads * masked_row_groups(heads / kv_heads * t) <= kMaxGroups;
+}
+
+int64_t masked_workspace(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim, int n_split) {
+  if (!masked_shape(batch, t, heads, kv_heads, head_dim) || n_split <= 1) return 0;
+  const int64_t rows = heads / kv_heads * t;
+  return batch * kv_heads * masked_row_groups(rows) * masked_group_rows(rows) * n_split * (head_dim + 2) * 4;
+}
+
+// The operands that every call has, checked and taken down. False: refused.
+bool masked_operands(MaskedArgs& a, const uint16_t* q, const int64_t* q_strides, const uint16_t* gate, const int64_t* gate_strides,
+                     int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim, const uint16_t* k_pool,
+                     const uint16_t* v_pool, int64_t pool_rows, const int32_t* block_table, int64_t table_stride,
+                     const int64_t* base_pos, float scale, int n_split, void* workspace, int64_t workspace_bytes, uint16_t* out,
+                     const int64_t* out_strides) {
+  if (!masked_shape(batch, t, heads, kv_heads, head_dim)) return false;
+  if (pool_rows <= 0 || pool_rows % kAttnBlock || table_stride <= 0 || table_stride > (1 << 26) || kv_heads > 4096) return false;
+  if (!(scale > 0.f) || !(scale < INFINITY)) return false;
+  if (n_split < 1 || n_split > kMaskedSplits) return false;
+  if (n_split > kMergeOne && batch * t * heads > kMaxGroups) return false;  // the merge's workgroups
+  // 16-byte accesses to query, gate and output rows and to the pools
+  if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (gate && !aligned16(gate))) return false;
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] % 8 || out_strides[i] % 8 || (gate && gate_strides[i] % 8)) return false;
+  if (n_split > 1 && (!workspace || !aligned16(workspace) ||
+                      workspace_bytes < masked_workspace(batch, t, heads, kv_heads, head_dim, n_split)))
+    return false;
+  const int64_t rows = heads / kv_heads * t;
+  a.q = q;
+  a.qr = {q_strides[0], q_strides[1], q_strides[2]};
+  a.out = out;
+  a.orow = {out_strides[0], out_strides[1], out_strides[2]};
+  a.gate = gate;
+  if (gate) a.gr = {gate_strides[0], gate_strides[1], gate_strides[2]};
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.pool_blocks = (uint32_t)std::min<int64_t>(pool_rows / kAttnBlock, (int64_t)1 << 31);
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.base = base_pos;
+  a.t = (int)t;
+  a.heads = (int)heads;
+  a.kvh = (int)kv_heads;
+  a.lanes_kvh = (int)(batch * kv_heads);
+  a.n_split = n_split;
+  a.row_groups = (int)masked_row_groups(rows);
+  a.c0 = scale * kLog2e;
+  a.part_o = (float*)workspace;
+  a.part_ml = a.part_o ? a.part_o + batch * kv_heads * a.row_groups * masked_group_rows(rows) * n_split * head_dim : nullptr;
+  return true;
 }
 
 }  // namespace
@@ -1171,9 +1271,7 @@ int mtpk_attention_masked_splits(int64_t batch, int64_t t, int64_t heads, int64_
 
 int64_t mtpk_attention_masked_workspace_bytes(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads,
                                               int64_t head_dim, int n_split) {
-  if (!masked_shape(batch, t, heads, kv_heads, head_dim) || n_split <= 1) return 0;
-  const int64_t rows = heads / kv_heads * t;
-  return batch * kv_heads * masked_row_groups(rows) * masked_group_rows(rows) * n_split * (head_dim + 2) * 4;
+  return masked_workspace(batch, t, heads, kv_heads, head_dim, n_split);
 }
 
 int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, const uint16_t* gate,
@@ -1188,49 +1286,19 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
   if (!q || !k_pool || !v_pool || !block_table || !base_pos || !out || !q_strides || !out_strides) return MTPK_EINVAL;
   if (gate && !gate_strides) return MTPK_EINVAL;
   if (batch == 0 && t > 0) return 0;
-  if (!masked_shape(batch, t, heads, kv_heads, head_dim)) return MTPK_EINVAL;
-  if (pool_rows <= 0 || pool_rows % kAttnBlock || table_stride <= 0 || table_stride > (1 << 26) ||
-      kv_heads > 4096) return MTPK_EINVAL;
-  if (!(scale > 0.f) || !(softcap >= 0.f) || !(scale < INFINITY) || !(softcap < INFINITY)) return MTPK_EINVAL;
-  if (window < 0 || n_split < 1 || n_split > kMaskedSplits) return MTPK_EINVAL;
-  if (n_split > kMergeOne && batch * t * heads > kMaxGroups) return MTPK_EINVAL;  // the merge's workgroups
+  MaskedArgs a{};
+  if (!masked_operands(a, q, q_strides, gate, gate_strides, batch, t, heads, kv_heads, head_dim, k_pool, v_pool, pool_rows,
+                       block_table, table_stride, base_pos, scale, n_split, workspace, workspace_bytes, out, out_strides))
+    return MTPK_EINVAL;
+  if (!(softcap >= 0.f) || !(softcap < INFINITY) || window < 0) return MTPK_EINVAL;
   if (prefix && prefix_dtype != MTPK_I32 && prefix_dtype != MTPK_I64) return MTPK_EINVAL;
   if (first && first_dtype != MTPK_I32 && first_dtype != MTPK_I64) return MTPK_EINVAL;
-  // 16-byte accesses to query, gate and output rows and to the pools
-  if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (gate && !aligned16(gate)))
-    return MTPK_EINVAL;
-  for (int i = 0; i < 3; ++i)
-    if (q_strides[i] % 8 || out_strides[i] % 8 || (gate && gate_strides[i] % 8)) return MTPK_EINVAL;
-  if (n_split > 1 && (!workspace || !aligned16(workspace) ||
-                      workspace_bytes < mtpk_attention_masked_workspace_bytes(batch, t, heads, kv_heads, head_dim, n_split)))
-    return MTPK_EINVAL;
-  const int64_t rows = heads / kv_heads * t;
-  MaskedArgs a{};
-  a.q = q;
-  a.qr = {q_strides[0], q_strides[1], q_strides[2]};
-  a.out = out;
-  a.orow = {out_strides[0], out_strides[1], out_strides[2]};
-  a.gate = gate;
-  if (gate) a.gr = {gate_strides[0], gate_strides[1], gate_strides[2]};
-  a.k_pool = k_pool;
-  a.v_pool = v_pool;
-  a.pool_blocks = (uint32_t)std::min<int64_t>(pool_rows / kAttnBlock, (int64_t)1 << 31);
-  a.table = block_table;
-  a.table_stride = table_stride;
-  a.base = base_pos;
   a.slopes = slopes;
   a.prefix = prefix;
   a.prefix_dt = prefix_dtype;
   a.first = first;
   a.first_dt = first_dtype;
   a.window = (int)std::min<int64_t>(window, INT32_MAX);
-  a.t = (int)t;
-  a.heads = (int)heads;
-  a.kvh = (int)kv_heads;
-  a.lanes_kvh = (int)(batch * kv_heads);
-  a.n_split = n_split;
-  a.row_groups = (int)masked_row_groups(rows);
-  a.c0 = scale * kLog2e;
   if (softcap > 0.f) {
     // tanh(u) / u by polynomials in u^2 of least relative error: 8.4e-6 on |u| <= 0.15, which is 9e-5 of an exponent
     // at cap 50 (a rounded probability is off by up to 2^-8), and 4e-7 on |u| <= 0.25
@@ -1248,13 +1316,45 @@ int mtpk_paged_attention_masked(const uint16_t* q, const int64_t* q_strides, con
       a.c1 = (float)std::max(c * k * k * k * -0.33035765, -3e38);
     }
   }
-  a.part_o = (float*)workspace;
-  a.part_ml = a.part_o ? a.part_o + batch * kv_heads * a.row_groups * masked_group_rows(rows) * n_split * head_dim : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   switch (head_dim) {
     case 64: return masked_flags<64>(a, batch, st);
     case 128: return masked_flags<128>(a, batch, st);
     default: return masked_flags<256>(a, batch, st);
+  }
+}
+
+int mtpk_attention_tree_splits(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_ctx) {
+  if (t > kTreeNodes || !masked_shape(batch, t, heads, kv_heads, head_dim) || max_ctx < 0) return 0;
+  return masked_splits(batch, kv_heads, heads / kv_heads * t, head_dim, max_ctx);
+}
+
+int64_t mtpk_attention_tree_workspace_bytes(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                            int n_split) {
+  return t > kTreeNodes ? 0 : mtpk_attention_masked_workspace_bytes(batch, t, heads, kv_heads, head_dim, n_split);
+}
+
+int mtpk_paged_attention_tree(const uint16_t* q, const int64_t* q_strides, const uint16_t* gate, const int64_t* gate_strides,
+                              int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim, const uint16_t* k_pool,
+                              const uint16_t* v_pool, int64_t pool_rows, const int32_t* block_table, int64_t table_stride,
+                              const int64_t* base_pos, float scale, const void* parents, int parents_dtype,
+                              const int64_t* parents_strides, int n_split, void* workspace, int64_t workspace_bytes, uint16_t* out,
+                              const int64_t* out_strides, void* stream) {
+  if (!q || !k_pool || !v_pool || !block_table || !base_pos || !parents || !out || !q_strides || !out_strides || !parents_strides)
+    return MTPK_EINVAL;
+  if (gate && !gate_strides) return MTPK_EINVAL;
+  if (t < 1 || t > kTreeNodes || (parents_dtype != MTPK_I32 && parents_dtype != MTPK_I64)) return MTPK_EINVAL;
+  if (batch == 0) return 0;
+  MaskedArgs a{};
+  if (!masked_operands(a, q, q_strides, gate, gate_strides, batch, t, heads, kv_heads, head_dim, k_pool, v_pool, pool_rows,
+                       block_table, table_stride, base_pos, scale, n_split, workspace, workspace_bytes, out, out_strides))
+    return MTPK_EINVAL;
+  a.tree = {parents, parents_dtype, parents_strides[0], parents_strides[1]};
+  const hipStream_t st = (hipStream_t)stream;
+  switch (head_dim) {
+    case 64: return masked_launch<64, false, false, true>(a, batch, st);
+    case 128: return masked_launch<128, false, false, true>(a, batch, st);
+    default: return masked_launch<256, false, false, true>(a, batch, st);
   }
 }
 

@@ -1,0 +1,521 @@
+// The Gated DeltaNet rows of a tree of drafts (mtpk_tree.h): the delta rule's inputs, with the convolution along
+// each node's own path; the rule itself, each node from its parent's state; and the advance of the stored
+// state and convolution window along the accepted path.
+
+#include <algorithm>
+
+#include "mtpk_deltanet_step.h"
+#include "mtpk_host.h"
+#include "mtpk_tree.h"
+
+namespace mtpk {
+
+constexpr int kTreeConvMost = 8;  // conv_k - 1 at most
+constexpr int kTreeHeadMost = 256;  // widest head of the preparation
+
+// ---------------------------------------------------------------- inputs
+//
+// As mtpk_deltanet_prep, but the columns before a node are its ancestors' (then the stored window's), which are the
+// highest bits of its ancestors. A wave takes one head unit (the q heads, the k heads, the v heads, and one more for g
+// and beta) of up to kPrepNodes nodes of a lane: lane l holds channels 2 l, 2 l + 1 (+ 128), and the columns of all
+// nodes and taps are on their way at once.
+//
+// The convolution's output is a tensor of the model's type. Next to a rounding's border the order of the products decides
+// to which side a value goes, half a step of bf16 either way; bf16 rows are therefore summed in 64 bits (their products
+// are exact in 32), and the few outputs that 32 bits put within 2^-12 of a step of the border (1 in 2000) have their SiLU
+// done again in 64. Of f32 rows there is nothing to round, and the sums run as in mtpk_deltanet_prep.
+constexpr int kPrepNodes = 4;
+
+struct TreePrepArgs {
+  const void* proj;  // [B * t, proj_stride]: qkv (C), z, b (vh), a (vh)
+  int64_t proj_stride;
+  const void* conv;  // [slots, C, k1]
+  const int64_t* slot;
+  int64_t slots_total;
+  const void* conv_w;  // [C, conv_k]
+  const float* a_log;
+  const float* dt_bias;
+  TreeParents parents;
+  int B, t, kh, kd, vh, vd, conv_k;
+  float eps, q_scale;
+  float *q, *k, *v, *g, *beta;
+};
+
+template <typename T>
+__device__ inline float tree_float(const void* p, int64_t i) {
+  if constexpr (sizeof(T) == 2)
+    return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
+  else
+    return static_cast<const float*>(p)[i];
+}
+
+// Channels ch, ch + 1 of element i; `two`: both exist. PAIR: a dword of two bf16.
+template <typename T, bool PAIR>
+__device__ inline float2 tree_pair(const void* p, int64_t i, bool two) {
+  if constexpr (PAIR) {
+    const uint32_t d = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+    return make_float2(bits_f32(d << 16), bits_f32(d & 0xffff0000u));
+  } else {
+    return make_float2(tree_float<T>(p, i), two ? tree_float<T>(p, i + 1) : 0.f);
+  }
+}
+
+__device__ inline float tree_silu(float x) { return x / (1.f + expf(-x)); }
+
+// SiLU of the exact sum x, rounded to bf16.
+__device__ inline float tree_silu_bf16(double x) {
+  float y = tree_silu((float)x);
+  const uint32_t away = (f32_bits(y) + 0x8010u) & 0xffffu;  // 16 on the border between two bf16 values
+  if (away <= 32u) y = (float)(x / (1.0 + exp(-x)));
+  return bf16_to_f32(f32_to_bf16(y));
+}
+
+// K: conv_k, or 0 for any. NI: 128-channel parts of a head.
+template <typename T, int K, bool PAIR, int NI>
+__global__ __launch_bounds__(kWave) void k_tree_prep(TreePrepArgs a) {
+  constexpr int R = kPrepNodes, KM = K ? K : kTreeConvMost + 1;
+  const int lane = threadIdx.x;
+  const int conv_k = K ? K : a.conv_k, k1 = conv_k - 1;
+  const int units = 2 * a.kh + a.vh + 1, groups = (a.t + R - 1) / R;
+  const int u = blockIdx.x % units, br = blockIdx.x / units, b = br / groups, s0 = (br - b * groups) * R;
+  const int64_t row0 = (int64_t)b * a.t;
+  const int C = 2 * a.kh * a.kd + a.vh * a.vd;
+  const int parent = a.parents.at(b, lane, a.t);
+  if (u == units - 1) {
+    const uint64_t seen = tree_ancestors(parent, lane);
+    const uint64_t nodes = __ballot(seen != 0ull);
+    for (int i = lane; i < min(R, a.t - s0) * a.vh; i += kWave) {
+      const int s = s0 + i / a.vh, h = i % a.vh;
+      const int64_t at = (row0 + s) * a.proj_stride + C + a.vh * a.vd + h;
+      const bool present = nodes >> s & 1ull;
+      const float x = __fadd_rn(tree_float<T>(a.proj, at + a.vh), a.dt_bias[h]);
+      const float sp = x > 20.f ? x : log1pf(expf(x));
+      a.beta[(row0 + s) * a.vh + h] = present ? 1.f / (1.f + expf(-tree_float<T>(a.proj, at))) : 0.f;
+      a.g[(row0 + s) * a.vh + h] = present ? -expf(a.a_log[h]) * sp : 0.f;
+    }
+    return;
+  }
+  const bool is_v = u >= 2 * a.kh;
+  const int dim = is_v ? a.vd : a.kd;
+  const int c0 = is_v ? 2 * a.kh * a.kd + (u - 2 * a.kh) * a.vd : u * a.kd;
+  const int64_t slot = a.slot[b];
+  const bool slot_ok = slot >= 0 && slot < a.slots_total;
+  float2 w[NI][KM], stored[NI][KM - 1];
+#pragma unroll
+  for (int n = 0; n < NI; ++n) {
+    const int ch = 2 * lane + 128 * n, c = c0 + (ch < dim ? ch : 0);
+    const bool two = ch + 1 < dim;
+    if constexpr (PAIR && K == 4) {  // two channels of 4 taps, and of 3 columns
+      const u32x4_t d = ld16(static_cast<const uint16_t*>(a.conv_w) + (int64_t)c * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = d[j / 2], y = d[2 + j / 2];
+        w[n][j] = make_float2(bits_f32(j % 2 ? x & 0xffff0000u : x << 16), bits_f32(j % 2 ? y & 0xffff0000u : y << 16));
+      }
+      uint32_t e[3] = {0u, 0u, 0u};
+      if (slot_ok) {
+        const uint32_t* const p = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.conv) + (slot * C + c) * 3);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) e[j] = p[j];
+      }
+      stored[n][0] = make_float2(bits_f32(e[0] << 16), bits_f32(e[1] & 0xffff0000u));
+      stored[n][1] = make_float2(bits_f32(e[0] & 0xffff0000u), bits_f32(e[2] << 16));
+      stored[n][2] = make_float2(bits_f32(e[1] << 16), bits_f32(e[2] & 0xffff0000u));
+    } else {
+#pragma unroll
+      for (int j = 0; j < KM; ++j) {
+        w[n][j] = make_float2(0.f, 0.f);
+        if (j < conv_k) {
+          const int64_t i = (int64_t)c * conv_k + j;
+          w[n][j] = make_float2(tree_float<T>(a.conv_w, i), two ? tree_float<T>(a.conv_w, i + conv_k) : 0.f);
+        }
+        if (j == KM - 1) continue;
+        stored[n][j] = make_float2(0.f, 0.f);
+        if (j < k1 && slot_ok) {
+          const int64_t i = (slot * C + c) * k1 + j;
+          stored[n][j] = make_float2(tree_float<T>(a.conv, i), two ? tree_float<T>(a.conv, i + k1) : 0.f);
+        }
+      }
+    }
+  }
+  const uint64_t seen = tree_ancestors(parent, lane);
+  // tap j of node s0 + r: its ancestor conv_k - 1 - j generations up, or column `from` of the stored window
+  float2 x[R][NI][KM];
+  uint64_t way[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    way[r] = s0 + r < a.t ? lane_bits(seen, s0 + r) : 0ull;
+    uint64_t m = way[r];
+#pragma unroll
+    for (int j = KM - 1; j >= 0; --j) {
+      if (j >= conv_k) continue;
+      const bool raw = m != 0ull;
+      const int i = raw ? 63 - __builtin_clzll(m) : 0;  // else loaded for nothing: no branch around the loads
+      m &= ~(1ull << i);
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        const int ch = 2 * lane + 128 * n, c = c0 + (ch < dim ? ch : 0);
+        x[r][n][j] = tree_pair<T, PAIR>(a.proj, (row0 + i) * a.proj_stride + c, ch + 1 < dim);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (s0 + r >= a.t) continue;
+    const int above = __builtin_popcountll(way[r]);  // columns of the tree
+    float2 y[NI];
+    float ss = 0.f;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int ch = 2 * lane + 128 * n;
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float acc = 0.f;
+        double exact = 0.;
+#pragma unroll
+        for (int j = 0; j < KM; ++j) {
+          if (j >= conv_k) continue;
+          const int up = conv_k - 1 - j;  // generations
+          float col = e ? x[r][n][j].y : x[r][n][j].x;
+          if (up >= above) {  // uniform
+            col = 0.f;
+#pragma unroll
+            for (int i = 0; i < KM - 1; ++i)
+              if (i == k1 - 1 - (up - above)) col = e ? stored[n][i].y : stored[n][i].x;
+          }
+          const float prod = __fmul_rn(col, e ? w[n][j].y : w[n][j].x);
+          if constexpr (sizeof(T) == 2)
+            exact += (double)prod;
+          else
+            acc = j == 0 ? prod : __fadd_rn(acc, prod);
+        }
+        f[e] = ch + e < dim ? (sizeof(T) == 2 ? tree_silu_bf16(exact) : tree_silu(acc)) : 0.f;
+        ss += f[e] * f[e];
+      }
+      y[n] = make_float2(f[0], f[1]);
+    }
+    float scale = 1.f;
+    if (!is_v) scale = rsqrtf(wave_sum(ss) + a.eps);
+    const int64_t rs = row0 + s0 + r;
+    float* const to = is_v ? a.v + (rs * a.vh + (u - 2 * a.kh)) * a.vd
+                           : (u < a.kh ? a.q + (rs * a.kh + u) * a.kd : a.k + (rs * a.kh + (u - a.kh)) * a.kd);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      const int ch = 2 * lane + 128 * n;
+      float2 o = y[n];
+      if (!is_v) {
+        o = make_float2(o.x * scale, o.y * scale);
+        if (u < a.kh) o = make_float2(o.x * a.q_scale, o.y * a.q_scale);
+      }
+      if (above == 0) o = make_float2(0.f, 0.f);  // an absent node
+      if constexpr (PAIR) {
+        if (ch < dim) *reinterpret_cast<float2*>(to + ch) = o;
+      } else {
+        if (ch < dim) to[ch] = o.x;
+        if (ch + 1 < dim) to[ch + 1] = o.y;
+      }
+    }
+  }
+}
+
+template <typename T, int K, bool PAIR>
+int launch_tree_prep(const TreePrepArgs& a, hipStream_t st) {
+  const int64_t groups = (a.t + kPrepNodes - 1) / kPrepNodes, n = (int64_t)a.B * groups * (2 * a.kh + a.vh + 1);
+  if (n > 4 * kMaxGroups) return MTPK_EINVAL;  // one-wave workgroups
+  if (a.kd > 128 || a.vd > 128)
+    hipLaunchKernelGGL((k_tree_prep<T, K, PAIR, 2>), dim3((unsigned)n), dim3(kWave), 0, st, a);
+  else
+    hipLaunchKernelGGL((k_tree_prep<T, K, PAIR, 1>), dim3((unsigned)n), dim3(kWave), 0, st, a);
+  return status_of(hipGetLastError());
+}
+
+// ---------------------------------------------------------------- the rule, step by step
+//
+// A lane of the wave owns a column of the state, as in the chain's form, and takes the nodes in order. The state that it
+// holds is the last node's: a node that hangs below it goes on from there, any other one starts from the stored state
+// and walks its way from the root. So a chain costs a step a node, a tree its nodes' depths.
+template <int DK>
+__device__ __forceinline__ void tree_rule_column(const float* __restrict__ state, int64_t s_idx, int heads, int head, int row, int t,
+                                                 int rep, int dv, int col, const float* __restrict__ q, const float* __restrict__ k,
+                                                 const float* __restrict__ v, const float* __restrict__ g,
+                                                 const float* __restrict__ beta, float* __restrict__ out, uint64_t seen, int lane,
+                                                 float* kq) {
+  constexpr int kPer = (DK + kWave - 1) / kWave;
+  const bool live = col < dv;
+  const rsrc_t rsm = make_rsrc(state + ((s_idx * heads + head) * DK) * (int64_t)dv, (uint32_t)(DK * dv * 4));
+  const uint32_t vcol = live ? (uint32_t)col * 4u : kOutOfRange, drow = (uint32_t)dv * 4u;
+  const int qk_heads = heads / rep, kh = head / rep;
+  float s[DK];
+  uint64_t held = 0ull;  // the node whose state s is, with its ancestors
+  for (int node = 0; node < t; ++node) {
+    const uint64_t way = lane_bits(seen, node);
+    float* const to = out + (((int64_t)row * t + node) * heads + head) * dv + col;
+    if (way == 0ull) {
+      if (live) *to = 0.f;
+      continue;
+    }
+    uint64_t left = way;
+    if (held != 0ull && (held & ~way) == 0ull) {
+      left = way & ~held;
+    } else {
+#pragma unroll
+      for (int i = 0; i < DK; ++i)
+        s[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsm, (int)vcol, (int)(drow * i), 0));
+    }
+    held = way;
+    while (left != 0ull) {
+      const int at = __builtin_ctzll(left);
+      left &= left - 1ull;
+      const int64_t rs = (int64_t)row * t + at, hv = rs * heads + head;
+      float nk[kPer], nq[kPer];
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const int i = p * kWave + lane;
+        nk[p] = i < DK ? k[(rs * qk_heads + kh) * DK + i] : 0.f;
+        nq[p] = i < DK ? q[(rs * qk_heads + kh) * DK + i] : 0.f;
+      }
+      const float vv = live ? v[hv * dv + col] : 0.f, decay = __expf(g[hv]), bt = beta[hv];
+      __syncthreads();  // the last step's reads are over (a one-wave workgroup, or all waves alike)
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const int i = p * kWave + lane;
+        if (i < DK) {
+          kq[i] = nk[p];
+          kq[DK + i] = nq[p];
+        }
+      }
+      __syncthreads();
+      const float4* const kk = reinterpret_cast<const float4*>(kq);
+      const float4* const qq = reinterpret_cast<const float4*>(kq + DK);
+      float mem = 0.f, o = 0.f;
+#pragma unroll
+      for (int i4 = 0; i4 < DK / 4; ++i4) {
+        const float4 kv = kk[i4];
+        const float kr[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[4 * i4 + e] *= decay;
+          mem = fmaf(s[4 * i4 + e], kr[e], mem);
+        }
+      }
+      const float delta = (vv - mem) * bt;
+      asm volatile("" ::: "memory");  // k is read again rather than kept: the state takes DK registers
+#pragma unroll
+      for (int i4 = 0; i4 < DK / 4; ++i4) {
+        const float4 kv = kk[i4], qv = qq[i4];
+        const float kr[4] = {kv.x, kv.y, kv.z, kv.w}, qr[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[4 * i4 + e] = fmaf(kr[e], delta, s[4 * i4 + e]);
+          o = fmaf(s[4 * i4 + e], qr[e], o);
+        }
+      }
+      if (left == 0ull && live) *to = o;
+    }
+  }
+}
+
+template <int DK>
+__global__ __launch_bounds__(kWave) void k_tree_rule_steps(const float* __restrict__ state, int64_t slots_total,
+                                                           const int64_t* __restrict__ slot, int t, int heads, int rep, int dv,
+                                                           const float* __restrict__ q, const float* __restrict__ k,
+                                                           const float* __restrict__ v, const float* __restrict__ g,
+                                                           const float* __restrict__ beta, TreeParents parents,
+                                                           float* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) float kq[2 * DK];
+  const int nblk = (dv + kWave - 1) / kWave, bh = (int)blockIdx.x / nblk, row = bh / heads, head = bh - row * heads;
+  const int lane = threadIdx.x, col = ((int)blockIdx.x - bh * nblk) * kWave + lane;
+  const int64_t s_idx = slot ? slot[row] : row;
+  const int parent = parents.at(row, lane, t);
+  uint64_t seen = tree_ancestors(parent, lane);
+  if (s_idx < 0 || s_idx >= slots_total) {  // no such slot: zero outputs, no state access
+    if (col < dv)
+      for (int i = 0; i < t; ++i) out[(((int64_t)row * t + i) * heads + head) * dv + col] = 0.f;
+    return;
+  }
+  tree_rule_column<DK>(state, s_idx, heads, head, row, t, rep, dv, col, q, k, v, g, beta, out, seen, lane, kq);
+}
+
+// ---------------------------------------------------------------- the accepted path
+//
+// The chain's commit (mtpk_deltanet_step.h) over the rows that a path names, and behind its workgroups the
+// window's: its last conv_k - 1 columns after the path's.
+struct DnStepsOnPath {
+  const int64_t* path;
+  const int64_t* lengths;
+  int node = 0;
+  __device__ inline int begin(int row, int t) {
+    const TreePath p(path + (int64_t)row * t, lengths[row], t, threadIdx.x);
+    node = p.node;
+    return uniform(p.steps);
+  }
+  __device__ inline int64_t row(int r, int t, int st) const { return (int64_t)r * t + __builtin_amdgcn_readlane(node, st); }
+};
+
+struct PathWindow {
+  void* conv;
+  int dt;
+  const int64_t* slot;
+  int64_t slots_total;
+  const void* proj;
+  int64_t proj_stride;
+  const int64_t* path;
+  const int64_t* lengths;
+  int C, k1, t, per_row;  // per_row: waves of a lane
+};
+
+__device__ inline void path_window(const PathWindow& j, int id, int lane) {
+  const int b = id / j.per_row, c = (id - b * j.per_row) * kWave + lane;
+  const int64_t slot = j.slot[b];
+  if (slot < 0 || slot >= j.slots_total) return;  // uniform
+  const TreePath path(j.path + (int64_t)b * j.t, j.lengths[b], j.t, lane);
+  const int n = uniform(path.steps);
+  const bool on = c < j.C;
+  const int64_t base = (slot * j.C + (on ? c : 0)) * j.k1;
+  float v[kTreeConvMost];
+#pragma unroll
+  for (int w = 0; w < kTreeConvMost; ++w) {
+    if (w >= j.k1) continue;
+    const int p = n + w;  // of [the stored window | the path's columns]
+    const int at = p < j.k1 ? 0 : path.at(p - j.k1);
+    if (on) v[w] = p < j.k1 ? load_float(j.conv, j.dt, base + p) : load_float(j.proj, j.dt, ((int64_t)b * j.t + at) * j.proj_stride + c);
+  }
+#pragma unroll
+  for (int w = 0; w < kTreeConvMost; ++w)
+    if (w < j.k1 && on) store_float(j.conv, j.dt, base + w, v[w]);
+}
+
+__global__ __launch_bounds__(kWave, 3) void k_path_commit(float* __restrict__ state, int64_t slots_total,
+                                                          const int64_t* __restrict__ slot, int t, int heads, int rep, int dv,
+                                                          const float* __restrict__ k, const float* __restrict__ v,
+                                                          const float* __restrict__ g, const float* __restrict__ beta,
+                                                          const int64_t* __restrict__ path, const int64_t* __restrict__ lengths,
+                                                          int rule_blocks, PathWindow win) {
+  if ((int)blockIdx.x >= rule_blocks) {  // uniform over the one-wave workgroup
+    path_window(win, (int)blockIdx.x - rule_blocks, threadIdx.x);
+    return;
+  }
+  delta_rule_kg_body<4, false, true>((int)blockIdx.x, state, slots_total, slot, t, heads, rep, dv, k, k, v, g, beta, nullptr,
+                                     DnStepsOnPath{path, lengths});
+}
+
+template <int DK>
+__global__ __launch_bounds__(kWave) void k_path_commit_any(float* __restrict__ state, int64_t slots_total,
+                                                           const int64_t* __restrict__ slot, int t, int heads, int rep, int dv,
+                                                           const float* __restrict__ k, const float* __restrict__ v,
+                                                           const float* __restrict__ g, const float* __restrict__ beta,
+                                                           const int64_t* __restrict__ path, const int64_t* __restrict__ lengths,
+                                                           int rule_blocks, PathWindow win) {
+  if ((int)blockIdx.x >= rule_blocks) {
+    path_window(win, (int)blockIdx.x - rule_blocks, threadIdx.x);
+    return;
+  }
+  delta_rule_body<DK, false, true>((int)blockIdx.x, state, slots_total, slot, t, heads, rep, dv, k, k, v, g, beta, nullptr,
+                                   DnStepsOnPath{path, lengths});
+}
+
+namespace {
+
+bool tree_rule_shape(int64_t rows, int64_t t, int64_t heads, int64_t qk_heads, int64_t k_dim, int64_t v_dim, int64_t slots_total) {
+  return rows >= 0 && t >= 1 && t <= kTreeNodes && heads > 0 && qk_heads > 0 && heads % qk_heads == 0 &&
+         (k_dim == 16 || k_dim == 32 || k_dim == 64 || k_dim == 128) && v_dim > 0 && v_dim <= 4096 && slots_total > 0 &&
+         heads <= (1 << 20) && slots_total < (int64_t(1) << 40) / (heads * k_dim * v_dim) && rows <= INT32_MAX / heads;
+}
+
+}  // namespace
+}  // namespace mtpk
+
+using namespace mtpk;
+
+extern "C" {
+
+int mtpk_deltanet_prep_tree(const void* proj, int dtype, int64_t proj_stride, const void* conv_state, const int64_t* slot,
+                            int64_t slots_total, const void* conv_w, const float* a_log, const float* dt_bias, const void* parents,
+                            int parents_dtype, const int64_t* parents_strides, int64_t batch, int64_t t, int64_t k_heads,
+                            int64_t k_dim, int64_t v_heads, int64_t v_dim, int64_t conv_k, float eps, float q_scale, float* q,
+                            float* k, float* v, float* g, float* beta, void* stream) {
+  if (dtype != MTPK_F32 && dtype != MTPK_BF16) return MTPK_EINVAL;
+  if (parents_dtype != MTPK_I32 && parents_dtype != MTPK_I64) return MTPK_EINVAL;
+  if (batch < 0 || batch > INT32_MAX || t < 1 || t > kTreeNodes || k_heads < 1 || v_heads < 1 || k_heads > 65535 || v_heads > 65535 ||
+      conv_k < 2 || conv_k > kTreeConvMost + 1 || slots_total < 1)
+    return MTPK_EINVAL;
+  if (k_dim < 1 || k_dim > kTreeHeadMost || v_dim < 1 || v_dim > kTreeHeadMost) return MTPK_EINVAL;
+  const int64_t C = 2 * k_heads * k_dim + v_heads * v_dim;
+  if (proj_stride < C + v_heads * v_dim + 2 * v_heads) return MTPK_EINVAL;
+  if (batch == 0) return 0;
+  if (!proj || !conv_state || !slot || !conv_w || !a_log || !dt_bias || !parents || !parents_strides || !q || !k || !v || !g || !beta)
+    return MTPK_EINVAL;
+  const TreePrepArgs a{proj, proj_stride, conv_state, slot, slots_total, conv_w, a_log, dt_bias,
+                       {parents, parents_dtype, parents_strides[0], parents_strides[1]}, (int)batch, (int)t, (int)k_heads, (int)k_dim,
+                       (int)v_heads, (int)v_dim, (int)conv_k, eps, q_scale, q, k, v, g, beta};
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == MTPK_F32) return launch_tree_prep<float, 0, false>(a, st);
+  auto at = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  const bool pair = conv_k == 4 && proj_stride % 2 == 0 && k_dim % 2 == 0 && v_dim % 2 == 0 && at(proj, 4) && at(conv_state, 4) &&
+                    at(conv_w, 16) && at(q, 8) && at(k, 8) && at(v, 8);
+  return pair ? launch_tree_prep<uint16_t, 4, true>(a, st) : launch_tree_prep<uint16_t, 0, false>(a, st);
+}
+
+int mtpk_delta_rule_tree(const float* state, int64_t slots_total, const int64_t* slot, int64_t rows, int64_t t, int64_t heads,
+                         int64_t qk_heads, int64_t k_dim, int64_t v_dim, const float* q, const float* k, const float* v,
+                         const float* g, const float* beta, const void* parents, int parents_dtype, const int64_t* parents_strides,
+                         float* out, void* stream) {
+  if (!tree_rule_shape(rows, t, heads, qk_heads, k_dim, v_dim, slots_total) || (!slot && slots_total < rows)) return MTPK_EINVAL;
+  if (parents_dtype != MTPK_I32 && parents_dtype != MTPK_I64) return MTPK_EINVAL;
+  if (rows == 0) return 0;
+  if (!state || !q || !k || !v || !g || !beta || !parents || !parents_strides || !out) return MTPK_EINVAL;
+  const TreeParents tree{parents, parents_dtype, parents_strides[0], parents_strides[1]};
+  const hipStream_t st = (hipStream_t)stream;
+  const int rep = (int)(heads / qk_heads);
+  const int64_t grid = rows * heads * ((v_dim + kWave - 1) / kWave);
+  if (grid > 4 * kMaxGroups) return MTPK_EINVAL;
+#define MTPK_DNT(DK_)                                                                                                       \
+  hipLaunchKernelGGL((k_tree_rule_steps<DK_>), dim3((unsigned)grid), dim3(kWave), 0, st, state, slots_total, slot, (int)t,  \
+                     (int)heads, rep, (int)v_dim, q, k, v, g, beta, tree, out)
+  switch (k_dim) {
+    case 16: MTPK_DNT(16); break;
+    case 32: MTPK_DNT(32); break;
+    case 64: MTPK_DNT(64); break;
+    default: MTPK_DNT(128); break;
+  }
+#undef MTPK_DNT
+  return status_of(hipGetLastError());
+}
+
+int mtpk_deltanet_commit_path(float* state, int64_t slots_total, const int64_t* slot, int64_t rows, int64_t t, int64_t heads,
+                              int64_t qk_heads, int64_t k_dim, int64_t v_dim, const float* k, const float* v, const float* g,
+                              const float* beta, const int64_t* path, const int64_t* lengths, void* conv_state, int conv_dtype,
+                              int64_t conv_slots_total, const void* proj, int64_t proj_stride, int64_t channels, int64_t k1,
+                              void* stream) {
+  if (!tree_rule_shape(rows, t, heads, qk_heads, k_dim, v_dim, slots_total)) return MTPK_EINVAL;
+  if (conv_dtype != MTPK_F32 && conv_dtype != MTPK_BF16) return MTPK_EINVAL;
+  if (channels < 1 || channels > INT32_MAX / 2 || k1 < 1 || k1 > kTreeConvMost || proj_stride < channels || conv_slots_total < 1)
+    return MTPK_EINVAL;
+  if (rows == 0) return 0;
+  if (!state || !slot || !k || !v || !g || !beta || !path || !lengths || !conv_state || !proj) return MTPK_EINVAL;
+  const PathWindow win{conv_state, conv_dtype, slot, conv_slots_total, proj, proj_stride, path, lengths, (int)channels, (int)k1,
+                       (int)t, (int)((channels + kWave - 1) / kWave)};
+  const hipStream_t st = (hipStream_t)stream;
+  const int rep = (int)(heads / qk_heads);
+  const bool quads = k_dim == 128 && v_dim % kWave == 0 && aligned16(state) && aligned16(v);
+  const int64_t rule = rows * heads * ((v_dim + kWave - 1) / kWave), grid = rule + rows * win.per_row;
+  if (grid > 4 * kMaxGroups) return MTPK_EINVAL;
+#define MTPK_DNP(KERNEL_)                                                                                                    \
+  hipLaunchKernelGGL(KERNEL_, dim3((unsigned)grid), dim3(kWave), 0, st, state, slots_total, slot, (int)t, (int)heads, rep,   \
+                     (int)v_dim, k, v, g, beta, path, lengths, (int)rule, win)
+  if (quads) {
+    MTPK_DNP(k_path_commit);
+  } else {
+    switch (k_dim) {
+      case 16: MTPK_DNP(k_path_commit_any<16>); break;
+      case 32: MTPK_DNP(k_path_commit_any<32>); break;
+      case 64: MTPK_DNP(k_path_commit_any<64>); break;
+      default: MTPK_DNP(k_path_commit_any<128>); break;
+    }
+  }
+#undef MTPK_DNP
+  return status_of(hipGetLastError());
+}
+
+}  // extern "C"

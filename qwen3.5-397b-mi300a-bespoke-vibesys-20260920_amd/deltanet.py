@@ -176,3 +176,33 @@ def conv_commit(conv_state: torch.Tensor, slots: torch.Tensor, proj: torch.Tenso
         proj.data_ptr(),
         rs, ix.data_ptr(), b, channels, k1, t, _mtpk.stream_of(device)),
         "mtpk_conv_commit")  # fmt: skip
+
+
+def prep_tree(proj: torch.Tensor, conv_state: torch.Tensor, slots: torch.Tensor, conv_w: torch.Tensor,
+              a_log: torch.Tensor, dt_bias: torch.Tensor, k_heads: int, k_dim: int, v_heads: int, v_dim: int,
+              parents: torch.Tensor, eps: float = 1e-6) -> tuple[torch.Tensor, ...]:
+    """`prep` for the rows of trees of up to 64 drafts (`mtpk_deltanet_prep_tree`): the columns before a node are its
+    ancestors', then the stored window's. `parents` `[B, t]` as in `attention.paged_attention_tree`; absent nodes' rows are
+    zeros. bf16 rows' convolution is rounded to bf16 as its exact value is: beside `prep` on a chain, a value next to a
+    rounding's border may come out a step apart."""
+    return tuple(_mtpk.native().prep_tree(proj, conv_state, slots, conv_w, a_log, dt_bias, k_heads, k_dim, v_heads, v_dim,
+                                          parents, eps, _mtpk.stream_for(proj)))
+
+
+def delta_rule_tree(state: torch.Tensor, slots: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    g: torch.Tensor, beta: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
+    """`delta_rule`'s verify mode for trees of up to 64 drafts (`mtpk_delta_rule_tree`): node s of row j takes its step from
+    the state after its parent `parents[j, s]` (-1: the slot's stored state), so its output is that of a chain of its
+    ancestors and itself. `parents` `[B, t]` as in `attention.paged_attention_tree`; absent nodes give zeros. The states are
+    read and not written (`commit_path` advances them). Returns f32 `[B, t, heads, v_dim]`."""
+    return _mtpk.native().delta_rule_tree(state, slots, q, k, v, g, beta, parents, _mtpk.stream_for(state))
+
+
+def commit_path(state: torch.Tensor, conv_state: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                g: torch.Tensor, beta: torch.Tensor, path: torch.Tensor, lengths: torch.Tensor, proj: torch.Tensor,
+                channels: int) -> None:
+    """`commit` along a path of a tree, in one launch (`mtpk_deltanet_commit_path`): slot `slots[j]` takes the steps of rows
+    `path[j, i]`, `i < lengths[j]` (`graph_mtp.tree_accept`), and its conv window becomes the last columns of [stored
+    window | those rows' first `channels` of `proj` `[B, t, P]`]. A path entry that is no row of `[0, t)` ends the path; a slot
+    outside the pool (-1) commits nothing. `slots` distinct, t up to 64."""
+    _mtpk.native().commit_path(state, conv_state, slots, k, v, g, beta, path, lengths, proj, channels, _mtpk.stream_for(state))

@@ -207,6 +207,55 @@ def greedy_accept(step_argmax: torch.Tensor, draft: torch.Tensor, active: torch.
     return out
 
 
+@dataclass
+class TreeAccept:
+    """Outputs of one acceptance pass over trees: `path` int64 `[B, t]` holds node 0, the accepted nodes below it, and the
+    last of them repeated; `keep` bool `[B, t]` says which entries count (`i <= accept_len` on active lanes); the rest
+    `[B]` as in `AcceptResult`."""
+
+    path: torch.Tensor
+    accept_len: torch.Tensor
+    lengths: torch.Tensor
+    keep: torch.Tensor
+    bonus: torch.Tensor
+    next_pos: torch.Tensor
+    budget_left: torch.Tensor
+    live: torch.Tensor
+    hidden_src: torch.Tensor
+
+
+def tree_accept(step_argmax: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, active: torch.Tensor,
+                pos: torch.Tensor, budget: torch.Tensor, stops: torch.Tensor) -> TreeAccept:
+    """`greedy_accept` for trees of up to 64 drafts (`mtpk_tree_accept`): from node 0, the lane's own token, on to the lowest
+    child whose token is `step_argmax` of the node it hangs below, while there is one, that argmax is no stop id and the
+    budget lasts. step_argmax, tokens int64 `[B, t]`; parents `[B, t]` as in `attention.paged_attention_tree`; active bool
+    `[B]`; pos, budget int64 `[B]`; stops int64 `[B, S]`, -1 padded. CPU tensors take the torch spelling."""
+    if not step_argmax.is_cuda:
+        return tree_accept_torch(step_argmax, tokens, parents, active, pos, budget, stops)
+    return TreeAccept(*_mtpk.native().tree_accept(step_argmax, tokens, parents, active, pos, budget, stops,
+                                                  _mtpk.stream_for(step_argmax)))
+
+
+def tree_accept_torch(step_argmax: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, active: torch.Tensor,
+                      pos: torch.Tensor, budget: torch.Tensor, stops: torch.Tensor) -> TreeAccept:
+    """What `tree_accept` computes, in tensor ops."""
+    b, t = step_argmax.shape
+    lane, node = torch.arange(b, device=pos.device), torch.arange(t, device=pos.device)
+    at, n = torch.zeros_like(pos), torch.zeros_like(pos)
+    going = torch.ones_like(active)
+    path = [at]
+    for i in range(1, t):
+        best = step_argmax[lane, at]
+        fits = (parents == at[:, None]) & (tokens == best[:, None]) & (node > at[:, None])
+        going = going & fits.any(1) & ~(stops == best[:, None]).any(1) & (budget > i)
+        at = torch.where(going, fits.int().argmax(1), at)
+        n = n + going
+        path.append(at)
+    bonus, left = step_argmax[lane, at], budget - n - 1
+    return TreeAccept(torch.stack(path, 1), n, torch.where(active, n + 1, 1), active[:, None] & (node <= n[:, None]), bonus,
+                      pos + n + 1, left, ~(stops == bonus[:, None]).any(1) & (left > 0), lane * t + at)
+
+
 def kv_write_rows(pos: torch.Tensor, block_table: torch.Tensor, t: int, block_size: int) -> torch.Tensor:
     """Physical KV rows `block * bs + pos % bs` of a round's t positions (`graph_mtp.py:857-860`)."""
     grid = pos[:, None] + torch.arange(t, device=pos.device)[None, :]
