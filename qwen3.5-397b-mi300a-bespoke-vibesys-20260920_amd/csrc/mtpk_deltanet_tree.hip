@@ -337,6 +337,321 @@ __global__ __launch_bounds__(kWave) void k_tree_rule_steps(const float* __restri
   tree_rule_column<DK>(state, s_idx, heads, head, row, t, rep, dv, col, q, k, v, g, beta, out, seen, lane, kq);
 }
 
+// ---------------------------------------------------------------- the rule, all nodes at once
+//
+// With A(s) node s and its ancestors, G_s the sum of g over A(s), and S the stored state, the steps along every way are
+//   u_s = beta_s (v_s - e^(G_s) S^T k_s - sum over a in A(s), a != s, of e^(G_s - G_a) (k_a . k_s) u_a)
+//   out_s = e^(G_s) S^T q_s + sum over a in A(s) of e^(G_s - G_a) (k_a . q_s) u_a
+// which is the chunk form of a chain (mtpk_deltanet_chunk.h) with the ancestors in place of the earlier steps: parents come
+// first, so the system is unit lower triangular again. The state is read once, whatever the tree's depth, and passes
+// through two matrix products, K S and Q S; all products run on v_mfma_f32_16x16x4_f32. G is summed and differenced in
+// 64 bits.
+//
+// A wave takes 64 columns of a (row, head)'s state, as four column tiles of every fourth column, so that a lane's load of the
+// state is 16 bytes and a wave's 256 of a row. It streams through the products: 16 rows of it are multiplied with all
+// nodes' k and q, held in LDS, while the next ones are on their way. W waves to a workgroup, of the heads that share q
+// and k and their columns.
+//
+// A masked element is a product with zero, so that what is not finite at one node would reach nodes off its way. Where
+// a correction u comes out not finite, or the inputs are not the layer's (|k|^2 at most 1.01, g <= 0, beta in [0, 1]), the
+// wave does its columns again one by one, and adds a node's own ancestors alone.
+struct TreeRuleArgs {
+  const float* state;
+  int64_t slots_total;
+  const int64_t* slot;
+  int t, heads, qk_heads, rep, dv, slabs;  // slabs: of 64 columns
+  const float *q, *k, *v, *g, *beta;
+  TreeParents parents;
+  float* out;
+};
+
+template <int DK, int NT, int W>
+struct TreeRuleLds {
+  static constexpr int N = 16 * NT, kRow = DK + 4, kSq = N + 4, kDRow = 20, kDBlock = 16 * kDRow + 8;
+  float k[N][kRow], q[N][kRow];
+  float kk[N][kSq], qk[N][kSq];
+  struct Wave {
+    double g[N];
+    uint64_t seen[N];
+    float beta[N], eg[N];
+    float diag[NT][kDBlock];
+  } w[W];
+};
+
+// Node `lane`'s ancestors and itself, and the sum of x over them.
+__device__ inline uint64_t tree_sums(int parent, int lane, double& x) {
+  uint64_t m = parent >= -1 ? 1ull << lane : 0ull;
+  int up = parent;
+  while (__ballot(up >= 0) != 0ull) {
+    const int at = up < 0 ? lane : up;
+    const uint32_t lo = __shfl((uint32_t)m, at, kWave), hi = __shfl((uint32_t)(m >> 32), at, kWave);
+    const double above = __shfl(x, at, kWave);
+    const int next = __shfl(up, at, kWave);
+    if (up >= 0) {
+      m |= (uint64_t)hi << 32 | lo;
+      x += above;
+      up = next;
+    }
+  }
+  return up == -1 ? m : 0ull;
+}
+
+// Column col of the wave's (row, head), node by node: the corrections into `out`, then, from the last node back, each
+// one's output in its place, which no later one needs any more.
+template <int DK, int NT, int W>
+__device__ __forceinline__ void tree_rule_again(const TreeRuleArgs& a, const TreeRuleLds<DK, NT, W>& s, int wave, const float* state,
+                                                          int row, int head, int col) {
+  const auto& mine = s.w[wave];
+  if (col >= a.dv) return;
+  const int64_t hv = (int64_t)row * a.t * a.heads + head;
+  auto along = [&](const float* x, const float (*near)[TreeRuleLds<DK, NT, W>::kSq], int node, uint64_t others) {
+    float dot = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < DK; ++i) dot = fmaf(state[(int64_t)i * a.dv + col], x[i], dot);
+    float sum = mine.eg[node] * dot;
+#pragma unroll 1
+    while (others != 0ull) {
+      const int at = __builtin_ctzll(others);
+      others &= others - 1ull;
+      sum = fmaf(dn_exp(mine.g[node] - mine.g[at]) * near[node][at], a.out[(hv + (int64_t)at * a.heads) * a.dv + col], sum);
+    }
+    return sum;
+  };
+#pragma unroll 1
+  for (int node = 0; node < a.t; ++node) {
+    const uint64_t way = mine.seen[node];
+    const int64_t at = (hv + (int64_t)node * a.heads) * a.dv + col;
+    a.out[at] = way ? mine.beta[node] * (a.v[at] - along(s.k[node], s.kk, node, way & ~(1ull << node))) : 0.f;
+  }
+#pragma unroll 1
+  for (int node = a.t - 1; node >= 0; --node) {
+    const uint64_t way = mine.seen[node];
+    if (way) a.out[(hv + (int64_t)node * a.heads) * a.dv + col] = along(s.q[node], s.qk, node, way);
+  }
+}
+
+template <int DK, int NT, int W>
+__global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
+  using Lds = TreeRuleLds<DK, NT, W>;
+  constexpr int N = Lds::N, KT = DK / 16, RING = KT < 4 ? KT : 4;
+  __shared__ __attribute__((aligned(16))) Lds s;
+  const int units = a.rep * a.slabs, wgs = (units + W - 1) / W;
+  int id = blockIdx.x;
+  const int part = id % wgs;
+  id /= wgs;
+  const int kh = id % a.qk_heads, row = id / a.qk_heads;
+  const int tid = threadIdx.x, wave = uniform(tid / kWave), lane = tid & (kWave - 1), gq = lane >> 4, c = lane & 15;
+  const int unit = part * W + wave;
+  const bool on = unit < units;  // uniform over the wave
+  const int head = kh * a.rep + (on ? unit / a.slabs : 0), col = (on ? unit % a.slabs : 0) * kWave + 4 * c;
+  const bool live = on && col < a.dv;
+  const int64_t s_idx = a.slot ? a.slot[row] : row;
+  const int64_t hv0 = (int64_t)row * a.t * a.heads + head;
+  if (s_idx < 0 || s_idx >= a.slots_total) {  // no such slot: zero outputs, no state access; uniform over the workgroup
+    for (int i = gq; i < a.t; i += 4)
+      if (live) *reinterpret_cast<f32x4_t*>(a.out + (hv0 + (int64_t)i * a.heads) * a.dv + col) = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    return;
+  }
+  const float* const state = a.state + (s_idx * a.heads + head) * DK * (int64_t)a.dv;
+  const rsrc_t rs = make_rsrc(state, (uint32_t)(DK * a.dv * 4));
+  const uint32_t drow = (uint32_t)a.dv * 4u, voff = live ? (uint32_t)(4 * gq) * drow + (uint32_t)col * 4u : kOutOfRange;
+  f32x4_t st[RING][4];  // rows 16 kt + 4 gq + j, columns col .. col + 3
+  auto load_state = [&](int kt) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st[kt % RING][j] = __builtin_bit_cast(f32x4_t, buf16(rs, voff, drow * (uint32_t)(16 * kt + j)));
+  };
+  const int parent = a.parents.at(row, lane, a.t);
+  const bool node = lane < a.t;
+  const float gl = node ? a.g[hv0 + (int64_t)lane * a.heads] : 0.f, bl = node ? a.beta[hv0 + (int64_t)lane * a.heads] : 0.f;
+  constexpr int kPieces = N * DK / 4, kEach = (kPieces + W * kWave - 1) / (W * kWave);
+  u32x4_t kp[kEach], qp[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int p = tid + i * W * kWave, n = p / (DK / 4);
+    kp[i] = qp[i] = zero16();
+    if (n < a.t) {
+      const int64_t at = (((int64_t)row * a.t + n) * a.qk_heads + kh) * DK + p % (DK / 4) * 4;
+      kp[i] = ld16(a.k + at);
+      qp[i] = ld16(a.q + at);
+    }
+  }
+#pragma unroll
+  for (int kt = 0; kt < RING; ++kt) load_state(kt);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int p = tid + i * W * kWave, n = p / (DK / 4), d = p % (DK / 4) * 4;
+    if (kPieces % (W * kWave) && n >= N) continue;
+    *reinterpret_cast<u32x4_t*>(&s.k[n][d]) = kp[i];
+    *reinterpret_cast<u32x4_t*>(&s.q[n][d]) = qp[i];
+  }
+  // the lane's node, in this wave's head
+  auto& mine = s.w[wave];
+  double gs = gl < -1000.f ? -1000.f : gl;  // e^-1000 is 0 in fp32, and a finite sum keeps G_s - G_a defined
+  const uint64_t seen = tree_sums(parent, lane, gs);
+  if (lane < N) {
+    mine.g[lane] = seen ? gs : 0.;
+    mine.seen[lane] = seen;
+    mine.beta[lane] = seen ? bl : 0.f;
+    mine.eg[lane] = seen ? dn_exp(gs) : 0.f;
+  }
+  __syncthreads();
+  auto tile = [&](const float (*m)[Lds::kRow], int rt, int kt) {
+    return *reinterpret_cast<const f32x4_t*>(&m[16 * rt + c][16 * kt + 4 * gq]);
+  };
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+  // k . k and q . k of the node pairs, in turn over the waves
+  int turn = 0;
+#pragma unroll
+  for (int rt = 0; rt < NT; ++rt)
+#pragma unroll
+    for (int ct = 0; ct <= rt; ++ct)
+#pragma unroll
+      for (int of = 0; of < 2; ++of) {
+        if (turn++ % W != wave) continue;
+        f32x4_t acc[2] = {zero, zero};
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) acc[kt & 1] = dn_mma(tile(of ? s.q : s.k, rt, kt), tile(s.k, ct, kt), acc[kt & 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) (of ? s.qk : s.kk)[16 * rt + 4 * gq + i][16 * ct + c] = acc[0][i] + acc[1][i];
+      }
+  // K S and Q S: lane (gq, c) gets rows 4 gq + i of a tile, columns col + e
+  f32x4_t ks[NT][4], qs[NT][4];
+#pragma unroll
+  for (int rt = 0; rt < NT; ++rt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ks[rt][e] = qs[rt][e] = zero;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+    for (int rt = 0; rt < NT; ++rt) {
+      const f32x4_t ka = tile(s.k, rt, kt), qa = tile(s.q, rt, kt);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ks[rt][e] = mfma16x16x4(ka[j], st[kt % RING][j][e], ks[rt][e]);
+          qs[rt][e] = mfma16x16x4(qa[j], st[kt % RING][j][e], qs[rt][e]);
+        }
+    }
+    if (kt + RING < KT) load_state(kt + RING);
+  }
+  // v of a tile's nodes, in the products' layout
+  f32x4_t vv[2][4];
+  auto load_v = [&](int rt) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = 16 * rt + 4 * gq + i;
+      vv[rt & 1][i] = zero;
+      if (n < a.t && live) vv[rt & 1][i] = *reinterpret_cast<const f32x4_t*>(a.v + (hv0 + (int64_t)n * a.heads) * a.dv + col);
+    }
+  };
+  load_v(0);
+  __syncthreads();  // kk and qk are whole
+  if (!on) return;
+  const bool plain = !seen || (s.kk[lane < N ? lane : 0][lane < N ? lane : 0] <= 1.01f && gl <= 0.f && bl >= 0.f && bl <= 1.f);
+  bool odd = __ballot(!plain) != 0ull;
+  // A tile of the two masked matrices, -L and that of out: row 16 rt + c, columns 16 ct + 4 gq + e.
+  auto masked = [&](int rt, int ct, f32x4_t& l, f32x4_t& m) {
+    const int i = 16 * rt + c, j0 = 16 * ct + 4 * gq;
+    const double gi = mine.g[i];
+    const float bi = mine.beta[i];
+    const f32x4_t kv = *reinterpret_cast<const f32x4_t*>(&s.kk[i][j0]), qv = *reinterpret_cast<const f32x4_t*>(&s.qk[i][j0]);
+    const uint32_t bits = (uint32_t)(mine.seen[i] >> j0) & 15u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float d = dn_exp(fmin(gi - mine.g[j0 + e], 0.0));
+      const bool above = (bits >> e & 1u) != 0u;
+      l[e] = above && j0 + e != i ? -bi * d * kv[e] : 0.f;
+      m[e] = above ? d * qv[e] : 0.f;
+    }
+  };
+  f32x4_t am[NT];
+#pragma unroll
+  for (int rt = 0; rt < NT; ++rt) {
+    f32x4_t l;
+    masked(rt, rt, l, am[rt]);
+    *reinterpret_cast<f32x4_t*>(&mine.diag[rt][c * Lds::kDRow + 4 * gq]) = l;
+  }
+  auto own_lds = [&]() {  // the wave reads back only what it wrote
+    ring_fence();
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    ring_fence();
+  };
+  own_lds();
+  // the diagonal blocks' inverses, side by side: column c of block gq, D[i] = [i == c] + sum over m < i of -L[i][m] D[m]
+  {
+    const float* const block = mine.diag[gq < NT ? gq : 0];
+    float dc[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float acc = c == i ? 1.f : 0.f;
+#pragma unroll
+      for (int m4 = 0; m4 < (i + 3) / 4; ++m4) {
+        const f32x4_t lr = *reinterpret_cast<const f32x4_t*>(&block[i * Lds::kDRow + 4 * m4]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * m4 + e < i) acc = fmaf(lr[e], dc[4 * m4 + e], acc);
+      }
+      dc[i] = acc;
+    }
+    own_lds();
+    if (gq < NT) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine.diag[gq][i * Lds::kDRow + c] = dc[i];
+    }
+    own_lds();
+  }
+  uint32_t most = 0;  // bits of the largest |u|; infinity and NaN lie above every number
+#pragma unroll
+  for (int rt = 0; rt < NT; ++rt) {
+    const int n0 = 16 * rt + 4 * gq;
+    const f32x4_t bv = *reinterpret_cast<const f32x4_t*>(&mine.beta[n0]), ev = *reinterpret_cast<const f32x4_t*>(&mine.eg[n0]);
+    const f32x4_t inv = *reinterpret_cast<const f32x4_t*>(&mine.diag[rt][c * Lds::kDRow + 4 * gq]);
+    bool present[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) present[i] = mine.seen[n0 + i] != 0ull;
+    f32x4_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[e][i] = present[i] ? bv[i] * (vv[rt & 1][i][e] - ev[i] * ks[rt][e][i]) : 0.f;
+        qs[rt][e][i] *= ev[i];
+      }
+    if (rt + 1 < NT) load_v(rt + 1);
+#pragma unroll
+    for (int ct = 0; ct < rt; ++ct) {
+      f32x4_t l, m;
+      masked(rt, ct, l, m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[e] = dn_mma(l, ks[ct][e], y[e]);
+        qs[rt][e] = dn_mma(m, ks[ct][e], qs[rt][e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      ks[rt][e] = dn_mma(inv, y[e], zero);  // u, in the place of K S
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = max(most, f32_bits(ks[rt][e][i]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qs[rt][e] = dn_mma(am[rt], ks[rt][e], qs[rt][e]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + i;
+      if (n < a.t && live)
+        *reinterpret_cast<f32x4_t*>(a.out + (hv0 + (int64_t)n * a.heads) * a.dv + col) =
+            present[i] ? f32x4_t{qs[rt][0][i], qs[rt][1][i], qs[rt][2][i], qs[rt][3][i]} : zero;
+    }
+  }
+  odd |= __ballot(most >= 0x7f800000u) != 0ull;
+  if (odd) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above, before those of the same places
+    tree_rule_again<DK, NT, W>(a, s, wave, state, row, head, col - 4 * c + lane);
+  }
+}
+
 // ---------------------------------------------------------------- the accepted path
 //
 // The chain's commit (mtpk_deltanet_step.h) over the rows that a path names, and behind its workgroups the
@@ -423,6 +738,27 @@ bool tree_rule_shape(int64_t rows, int64_t t, int64_t heads, int64_t qk_heads, i
          heads <= (1 << 20) && slots_total < (int64_t(1) << 40) / (heads * k_dim * v_dim) && rows <= INT32_MAX / heads;
 }
 
+template <int DK, int NT, int W>
+int tree_rule_waves(const TreeRuleArgs& a, int64_t rows, hipStream_t st) {
+  const int64_t grid = rows * a.qk_heads * ((a.rep * a.slabs + W - 1) / W);
+  hipLaunchKernelGGL((k_tree_rule<DK, NT, W>), dim3((unsigned)grid), dim3(W * kWave), 0, st, a);
+  return status_of(hipGetLastError());
+}
+
+template <int DK, int NT>
+int tree_rule_tiles(const TreeRuleArgs& a, int64_t rows, hipStream_t st) {
+  const int64_t units = (int64_t)a.rep * a.slabs;
+  if (units >= 8 && rows * a.qk_heads * units >= 8 * device_cu_count()) return tree_rule_waves<DK, NT, 8>(a, rows, st);
+  return tree_rule_waves<DK, NT, 2>(a, rows, st);
+}
+
+template <int DK>
+int tree_rule_launch(const TreeRuleArgs& a, int64_t rows, hipStream_t st) {
+  if (a.t <= 16) return tree_rule_tiles<DK, 1>(a, rows, st);
+  if (a.t <= 32) return tree_rule_tiles<DK, 2>(a, rows, st);
+  return tree_rule_tiles<DK, 4>(a, rows, st);
+}
+
 }  // namespace
 }  // namespace mtpk
 
@@ -468,8 +804,17 @@ int mtpk_delta_rule_tree(const float* state, int64_t slots_total, const int64_t*
   const TreeParents tree{parents, parents_dtype, parents_strides[0], parents_strides[1]};
   const hipStream_t st = (hipStream_t)stream;
   const int rep = (int)(heads / qk_heads);
-  const int64_t grid = rows * heads * ((v_dim + kWave - 1) / kWave);
+  const int64_t slabs = (v_dim + kWave - 1) / kWave, grid = rows * heads * slabs;
   if (grid > 4 * kMaxGroups) return MTPK_EINVAL;
+  if (v_dim % 4 == 0 && aligned16(state) && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out)) {
+    const TreeRuleArgs a{state, slots_total, slot, (int)t, (int)heads, (int)qk_heads, rep, (int)v_dim, (int)slabs, q, k, v, g, beta, tree, out};
+    switch (k_dim) {
+      case 16: return tree_rule_launch<16>(a, rows, st);
+      case 32: return tree_rule_launch<32>(a, rows, st);
+      case 64: return tree_rule_launch<64>(a, rows, st);
+      default: return tree_rule_launch<128>(a, rows, st);
+    }
+  }
 #define MTPK_DNT(DK_)                                                                                                       \
   hipLaunchKernelGGL((k_tree_rule_steps<DK_>), dim3((unsigned)grid), dim3(kWave), 0, st, state, slots_total, slot, (int)t,  \
                      (int)heads, rep, (int)v_dim, q, k, v, g, beta, tree, out)

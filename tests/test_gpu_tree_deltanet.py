@@ -25,6 +25,7 @@ def _close(got, want):
 
 SHAPES = [  # heads, q/k heads, k_dim, v_dim
     (4, 2, 16, 16), (3, 3, 32, 96), (2, 1, 64, 64), (4, 1, 128, 128), (3, 1, 128, 64), (5, 5, 128, 192), (2, 2, 128, 40), (8, 2, 64, 128),
+    (2, 1, 16, 18), (2, 1, 128, 70), (1, 1, 64, 33), (3, 1, 32, 1),  # columns in no groups of four
 ]
 
 
