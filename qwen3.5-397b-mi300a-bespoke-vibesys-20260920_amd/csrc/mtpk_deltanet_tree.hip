@@ -344,13 +344,17 @@ __global__ __launch_bounds__(kWave) void k_tree_rule_steps(const float* __restri
 //   out_s = e^(G_s) S^T q_s + sum over a in A(s) of e^(G_s - G_a) (k_a . q_s) u_a
 // which is the chunk form of a chain (mtpk_deltanet_chunk.h) with the ancestors in place of the earlier steps: parents come
 // first, so the system is unit lower triangular again. The state is read once, whatever the tree's depth, and passes
-// through two matrix products, K S and Q S; all products run on v_mfma_f32_16x16x4_f32. G is summed and differenced in
-// 64 bits.
+// through two matrix products, K S and Q S.
+//
+// The products run on v_mfma_f32_16x16x32_bf16 at fp32's accuracy: each operand is three bf16 parts, 24 bits, each the rest of
+// the ones before it rounded, and of the nine products of parts the six largest are taken; what is left out is below
+// 2^-25 of the product. That is 96 cycles for 16 x 16 x 32 where v_mfma_f32_16x16x4_f32 takes 256. G is summed and
+// differenced in 64 bits, in units of log2.
 //
 // A wave takes 64 columns of a (row, head)'s state, as four column tiles of every fourth column, so that a lane's load of the
-// state is 16 bytes and a wave's 256 of a row. It streams through the products: 16 rows of it are multiplied with all
-// nodes' k and q, held in LDS, while the next ones are on their way. W waves to a workgroup, of the heads that share q
-// and k and their columns.
+// state is 16 bytes and a wave's 256 of a row. It streams through the products: 32 rows of it are multiplied with all
+// nodes' k and q, held in LDS in parts, while the next ones are on their way. W waves to a workgroup, of the heads that
+// share q and k and their columns.
 //
 // A masked element is a product with zero, so that what is not finite at one node would reach nodes off its way. Where
 // a correction u comes out not finite, or the inputs are not the layer's (|k|^2 at most 1.01, g <= 0, beta in [0, 1]), the
@@ -365,17 +369,60 @@ struct TreeRuleArgs {
   float* out;
 };
 
+// Three bf16 parts of four floats, in pairs.
+struct Parts4 {
+  uint32_t p[3][2];
+};
+__device__ inline Parts4 parts_of(f32x4_t x) {
+  Parts4 r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float a = x[2 * h], b = x[2 * h + 1];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const bf16x2_t y = {(__bf16)a, (__bf16)b};
+      const uint32_t u = __builtin_bit_cast(uint32_t, y);
+      r.p[i][h] = u;
+      a -= bits_f32(u << 16);
+      b -= bits_f32(u & 0xffff0000u);
+    }
+  }
+  return r;
+}
+
+// Part i of eight values.
+__device__ inline bf16x8_t part8(const Parts4& x, const Parts4& y, int i) {
+  return as_bf16x8(u32x4_t{x.p[i][0], x.p[i][1], y.p[i][0], y.p[i][1]});
+}
+
+// The products that are taken, the smallest first: parts of the left and of the right operand.
+constexpr int kPartProducts = 6;
+__device__ inline constexpr int left_part(int i) { return i == 0 ? 2 : i == 2 || i == 4 ? 1 : 0; }
+__device__ inline constexpr int right_part(int i) { return i == 1 ? 2 : i == 2 || i == 3 ? 1 : 0; }
+
+// K's and Q's parts lie in `both` until the products with the state are done (as they are, and taken apart by every wave for
+// itself, they were as fast for many lanes and slower for few: one lane of 7 nodes 10.3 against 11.9 us, of 30 14.5 against
+// 17.4). k . k, q . k and the diagonal blocks lie behind them, and at 64 nodes, where LDS does not hold both, in their place.
 template <int DK, int NT, int W>
 struct TreeRuleLds {
-  static constexpr int N = 16 * NT, kRow = DK + 4, kSq = N + 4, kDRow = 20, kDBlock = 16 * kDRow + 8;
-  float k[N][kRow], q[N][kRow];
-  float kk[N][kSq], qk[N][kSq];
+  static constexpr int N = 16 * NT, kRow = (DK < 32 ? 32 : DK) + 8, kSq = N + 4, kDRow = 20, kDBlock = 16 * kDRow + 8;
+  static constexpr bool OVER = NT == 4;
+  struct Pairs {
+    float kk[N][kSq], qk[N][kSq];
+    float diag[W][NT][kDBlock];
+  };
   struct Wave {
     double g[N];
     uint64_t seen[N];
     float beta[N], eg[N];
-    float diag[NT][kDBlock];
-  } w[W];
+  };
+  static constexpr int kPartBytes = 2 * 3 * N * kRow * 2, kPairBytes = (int)sizeof(Pairs);
+  static constexpr int kPairsAt = OVER ? 0 : kPartBytes;
+  static constexpr int kBytes = OVER ? (kPartBytes > kPairBytes ? kPartBytes : kPairBytes) : kPartBytes + kPairBytes;
+  Wave w[W];
+  __attribute__((aligned(16))) uint8_t both[kBytes];
+  __device__ inline uint16_t* part(int of, int p, int row) { return reinterpret_cast<uint16_t*>(both) + ((of * 3 + p) * N + row) * kRow; }
+  __device__ inline Pairs& pairs() { return *reinterpret_cast<Pairs*>(both + kPairsAt); }
 };
 
 // Node `lane`'s ancestors and itself, and the sum of x over them.
@@ -396,15 +443,19 @@ __device__ inline uint64_t tree_sums(int parent, int lane, double& x) {
   return up == -1 ? m : 0ull;
 }
 
+// e to the difference of two sums in log2 units; 2^-25 of 1 at most from the rounding of the exponent.
+__device__ inline float tree_decay(double x) { return __builtin_amdgcn_exp2f((float)x); }
+
 // Column col of the wave's (row, head), node by node: the corrections into `out`, then, from the last node back, each
 // one's output in its place, which no later one needs any more.
 template <int DK, int NT, int W>
-__device__ __forceinline__ void tree_rule_again(const TreeRuleArgs& a, const TreeRuleLds<DK, NT, W>& s, int wave, const float* state,
-                                                          int row, int head, int col) {
+__device__ __forceinline__ void tree_rule_again(const TreeRuleArgs& a, TreeRuleLds<DK, NT, W>& s, int wave, const float* state, int row,
+                                                int kh, int head, int col) {
   const auto& mine = s.w[wave];
   if (col >= a.dv) return;
   const int64_t hv = (int64_t)row * a.t * a.heads + head;
-  auto along = [&](const float* x, const float (*near)[TreeRuleLds<DK, NT, W>::kSq], int node, uint64_t others) {
+  auto along = [&](const float* xs, const float (*near)[TreeRuleLds<DK, NT, W>::kSq], int node, uint64_t others) {
+    const float* const x = xs + (((int64_t)row * a.t + node) * a.qk_heads + kh) * DK;
     float dot = 0.f;
 #pragma unroll 4
     for (int i = 0; i < DK; ++i) dot = fmaf(state[(int64_t)i * a.dv + col], x[i], dot);
@@ -413,7 +464,7 @@ __device__ __forceinline__ void tree_rule_again(const TreeRuleArgs& a, const Tre
     while (others != 0ull) {
       const int at = __builtin_ctzll(others);
       others &= others - 1ull;
-      sum = fmaf(dn_exp(mine.g[node] - mine.g[at]) * near[node][at], a.out[(hv + (int64_t)at * a.heads) * a.dv + col], sum);
+      sum = fmaf(tree_decay(mine.g[node] - mine.g[at]) * near[node][at], a.out[(hv + (int64_t)at * a.heads) * a.dv + col], sum);
     }
     return sum;
   };
@@ -421,19 +472,19 @@ __device__ __forceinline__ void tree_rule_again(const TreeRuleArgs& a, const Tre
   for (int node = 0; node < a.t; ++node) {
     const uint64_t way = mine.seen[node];
     const int64_t at = (hv + (int64_t)node * a.heads) * a.dv + col;
-    a.out[at] = way ? mine.beta[node] * (a.v[at] - along(s.k[node], s.kk, node, way & ~(1ull << node))) : 0.f;
+    a.out[at] = way ? mine.beta[node] * (a.v[at] - along(a.k, s.pairs().kk, node, way & ~(1ull << node))) : 0.f;
   }
 #pragma unroll 1
   for (int node = a.t - 1; node >= 0; --node) {
     const uint64_t way = mine.seen[node];
-    if (way) a.out[(hv + (int64_t)node * a.heads) * a.dv + col] = along(s.q[node], s.qk, node, way);
+    if (way) a.out[(hv + (int64_t)node * a.heads) * a.dv + col] = along(a.q, s.pairs().qk, node, way);
   }
 }
 
 template <int DK, int NT, int W>
-__global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
+__global__ __launch_bounds__(W* kWave, NT > 2 ? 2 : 3) void k_tree_rule(TreeRuleArgs a) {
   using Lds = TreeRuleLds<DK, NT, W>;
-  constexpr int N = Lds::N, KT = DK / 16, RING = KT < 4 ? KT : 4;
+  constexpr int N = Lds::N, DKP = DK < 32 ? 32 : DK, KB = DKP / 32, RING = NT < 4 && KB > 1 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) Lds s;
   const int units = a.rep * a.slabs, wgs = (units + W - 1) / W;
   int id = blockIdx.x;
@@ -454,66 +505,91 @@ __global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
   }
   const float* const state = a.state + (s_idx * a.heads + head) * DK * (int64_t)a.dv;
   const rsrc_t rs = make_rsrc(state, (uint32_t)(DK * a.dv * 4));
-  const uint32_t drow = (uint32_t)a.dv * 4u, voff = live ? (uint32_t)(4 * gq) * drow + (uint32_t)col * 4u : kOutOfRange;
-  f32x4_t st[RING][4];  // rows 16 kt + 4 gq + j, columns col .. col + 3
-  auto load_state = [&](int kt) {
+  const uint32_t drow = (uint32_t)a.dv * 4u;
+  const uint32_t voff = live && 8 * gq < DK ? (uint32_t)(8 * gq) * drow + (uint32_t)col * 4u : kOutOfRange;
+  f32x4_t st[RING][8];  // rows 32 kb + 8 gq + j, columns col .. col + 3
+  auto load_state = [&](int kb) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) st[kt % RING][j] = __builtin_bit_cast(f32x4_t, buf16(rs, voff, drow * (uint32_t)(16 * kt + j)));
+    for (int j = 0; j < 8; ++j) st[kb % RING][j] = __builtin_bit_cast(f32x4_t, buf16(rs, voff, drow * (uint32_t)(32 * kb + j)));
   };
   const int parent = a.parents.at(row, lane, a.t);
   const bool node = lane < a.t;
   const float gl = node ? a.g[hv0 + (int64_t)lane * a.heads] : 0.f, bl = node ? a.beta[hv0 + (int64_t)lane * a.heads] : 0.f;
-  constexpr int kPieces = N * DK / 4, kEach = (kPieces + W * kWave - 1) / (W * kWave);
-  u32x4_t kp[kEach], qp[kEach];
+  // K and Q, eight values of a node to a thread
+  constexpr int kPieces = 2 * N * DKP / 8, kEach = (kPieces + W * kWave - 1) / (W * kWave);
+  f32x4_t in[kEach][2];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int p = tid + i * W * kWave, n = p / (DK / 4);
-    kp[i] = qp[i] = zero16();
-    if (n < a.t) {
-      const int64_t at = (((int64_t)row * a.t + n) * a.qk_heads + kh) * DK + p % (DK / 4) * 4;
-      kp[i] = ld16(a.k + at);
-      qp[i] = ld16(a.q + at);
+    const int p = tid + i * W * kWave, of = p / (N * DKP / 8), n = p / (DKP / 8) % N, d = p % (DKP / 8) * 8;
+    in[i][0] = in[i][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (of < 2 && n < a.t && d < DK) {
+      const float* const at = (of ? a.q : a.k) + (((int64_t)row * a.t + n) * a.qk_heads + kh) * DK + d;
+      in[i][0] = *reinterpret_cast<const f32x4_t*>(at);
+      in[i][1] = *reinterpret_cast<const f32x4_t*>(at + 4);
     }
   }
 #pragma unroll
-  for (int kt = 0; kt < RING; ++kt) load_state(kt);
+  for (int kb = 0; kb < RING; ++kb) load_state(kb);
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int p = tid + i * W * kWave, n = p / (DK / 4), d = p % (DK / 4) * 4;
-    if (kPieces % (W * kWave) && n >= N) continue;
-    *reinterpret_cast<u32x4_t*>(&s.k[n][d]) = kp[i];
-    *reinterpret_cast<u32x4_t*>(&s.q[n][d]) = qp[i];
+    const int p = tid + i * W * kWave, of = p / (N * DKP / 8), n = p / (DKP / 8) % N, d = p % (DKP / 8) * 8;
+    if (kPieces % (W * kWave) && of > 1) continue;
+    const Parts4 x = parts_of(in[i][0]), y = parts_of(in[i][1]);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8_t*>(s.part(of, j, n) + d) = part8(x, y, j);
   }
   // the lane's node, in this wave's head
   auto& mine = s.w[wave];
-  double gs = gl < -1000.f ? -1000.f : gl;  // e^-1000 is 0 in fp32, and a finite sum keeps G_s - G_a defined
+  // e^-1000 is 0 in fp32, and a finite sum keeps G_s - G_a defined
+  double gs = (double)(gl < -1000.f ? -1000.f : gl) * 1.4426950408889634;
   const uint64_t seen = tree_sums(parent, lane, gs);
   if (lane < N) {
     mine.g[lane] = seen ? gs : 0.;
     mine.seen[lane] = seen;
     mine.beta[lane] = seen ? bl : 0.f;
-    mine.eg[lane] = seen ? dn_exp(gs) : 0.f;
+    mine.eg[lane] = seen ? tree_decay(gs) : 0.f;
   }
   __syncthreads();
-  auto tile = [&](const float (*m)[Lds::kRow], int rt, int kt) {
-    return *reinterpret_cast<const f32x4_t*>(&m[16 * rt + c][16 * kt + 4 * gq]);
-  };
   const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-  // k . k and q . k of the node pairs, in turn over the waves
-  int turn = 0;
+  auto piece = [&](int of, int rt, int kb, int p) {  // row 16 rt + c, k index 32 kb + 8 gq + j
+    return as_bf16x8(*reinterpret_cast<const u32x4_t*>(s.part(of, p, 16 * rt + c) + 32 * kb + 8 * gq));
+  };
+  // k . k and q . k of the node pairs, in turn over the waves: rows 16 rt + 4 gq + i, column 16 ct + c
+  constexpr int kTiles = NT * (NT + 1), kTurns = (kTiles + W - 1) / W;
+  f32x4_t pair[kTurns];
+  auto pairs = [&](auto f) {  // (index of this wave's tile, which matrix, row tile, column tile)
+    int at = 0;
 #pragma unroll
-  for (int rt = 0; rt < NT; ++rt)
+    for (int rt = 0; rt < NT; ++rt)
 #pragma unroll
-    for (int ct = 0; ct <= rt; ++ct)
+      for (int ct = 0; ct <= rt; ++ct)
 #pragma unroll
-      for (int of = 0; of < 2; ++of) {
-        if (turn++ % W != wave) continue;
-        f32x4_t acc[2] = {zero, zero};
+        for (int of = 0; of < 2; ++of, ++at)
+          if (at % W == wave) f(at / W, of, rt, ct);
+  };
+  auto store_pairs = [&]() {
+    pairs([&](int n, int of, int rt, int ct) {
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) acc[kt & 1] = dn_mma(tile(of ? s.q : s.k, rt, kt), tile(s.k, ct, kt), acc[kt & 1]);
+      for (int i = 0; i < 4; ++i) (of ? s.pairs().qk : s.pairs().kk)[16 * rt + 4 * gq + i][16 * ct + c] = pair[n][i];
+    });
+  };
+  pairs([&](int n, int of, int rt, int ct) {
+    f32x4_t acc[2] = {zero, zero};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) (of ? s.qk : s.kk)[16 * rt + 4 * gq + i][16 * ct + c] = acc[0][i] + acc[1][i];
-      }
+    for (int kb = 0; kb < KB; ++kb) {
+      bf16x8_t x[3], y[3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) x[p] = piece(of, rt, kb, p), y[p] = piece(0, ct, kb, p);
+#pragma unroll
+      for (int p = 0; p < kPartProducts; ++p) acc[kb & 1] = mfma16x16x32(x[left_part(p)], y[right_part(p)], acc[kb & 1]);
+    }
+    pair[n] = acc[0] + acc[1];
+  });
+  if (!Lds::OVER) {
+    store_pairs();
+    __syncthreads();  // kk and qk are whole, and no wave waits for another any more
+    if (!on) return;
+  }
   // K S and Q S: lane (gq, c) gets rows 4 gq + i of a tile, columns col + e
   f32x4_t ks[NT][4], qs[NT][4];
 #pragma unroll
@@ -521,19 +597,31 @@ __global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) ks[rt][e] = qs[rt][e] = zero;
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) {
+  for (int kb = 0; kb < KB; ++kb) {
+    bf16x8_t b[4][3];
+    {
+      const f32x4_t(&x)[8] = st[kb % RING];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const Parts4 lo = parts_of(f32x4_t{x[0][e], x[1][e], x[2][e], x[3][e]}), hi = parts_of(f32x4_t{x[4][e], x[5][e], x[6][e], x[7][e]});
+#pragma unroll
+        for (int p = 0; p < 3; ++p) b[e][p] = part8(lo, hi, p);
+      }
+    }
+    if (kb + RING < KB) load_state(kb + RING);
 #pragma unroll
     for (int rt = 0; rt < NT; ++rt) {
-      const f32x4_t ka = tile(s.k, rt, kt), qa = tile(s.q, rt, kt);
+      bf16x8_t ka[3], qa[3];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int p = 0; p < 3; ++p) ka[p] = piece(0, rt, kb, p), qa[p] = piece(1, rt, kb, p);
+#pragma unroll
+      for (int p = 0; p < kPartProducts; ++p)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          ks[rt][e] = mfma16x16x4(ka[j], st[kt % RING][j][e], ks[rt][e]);
-          qs[rt][e] = mfma16x16x4(qa[j], st[kt % RING][j][e], qs[rt][e]);
+          ks[rt][e] = mfma16x16x32(ka[left_part(p)], b[e][right_part(p)], ks[rt][e]);
+          qs[rt][e] = mfma16x16x32(qa[left_part(p)], b[e][right_part(p)], qs[rt][e]);
         }
     }
-    if (kt + RING < KT) load_state(kt + RING);
   }
   // v of a tile's nodes, in the products' layout
   f32x4_t vv[2][4];
@@ -546,31 +634,38 @@ __global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
     }
   };
   load_v(0);
-  __syncthreads();  // kk and qk are whole
-  if (!on) return;
-  const bool plain = !seen || (s.kk[lane < N ? lane : 0][lane < N ? lane : 0] <= 1.01f && gl <= 0.f && bl >= 0.f && bl <= 1.f);
+  if (Lds::OVER) {
+    __syncthreads();  // nobody reads the parts any more
+    store_pairs();
+    __syncthreads();  // kk and qk are whole
+    if (!on) return;
+  }
+  auto& sq = s.pairs();
+  const int own = lane < N ? lane : 0;
+  const bool plain = !seen || (sq.kk[own][own] <= 1.01f && gl <= 0.f && bl >= 0.f && bl <= 1.f);
   bool odd = __ballot(!plain) != 0ull;
   // A tile of the two masked matrices, -L and that of out: row 16 rt + c, columns 16 ct + 4 gq + e.
   auto masked = [&](int rt, int ct, f32x4_t& l, f32x4_t& m) {
     const int i = 16 * rt + c, j0 = 16 * ct + 4 * gq;
     const double gi = mine.g[i];
     const float bi = mine.beta[i];
-    const f32x4_t kv = *reinterpret_cast<const f32x4_t*>(&s.kk[i][j0]), qv = *reinterpret_cast<const f32x4_t*>(&s.qk[i][j0]);
+    const f32x4_t kv = *reinterpret_cast<const f32x4_t*>(&sq.kk[i][j0]), qv = *reinterpret_cast<const f32x4_t*>(&sq.qk[i][j0]);
     const uint32_t bits = (uint32_t)(mine.seen[i] >> j0) & 15u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float d = dn_exp(fmin(gi - mine.g[j0 + e], 0.0));
+      const float d = tree_decay(gi - mine.g[j0 + e]);
       const bool above = (bits >> e & 1u) != 0u;
       l[e] = above && j0 + e != i ? -bi * d * kv[e] : 0.f;
       m[e] = above ? d * qv[e] : 0.f;
     }
   };
+  float(*const diag)[Lds::kDBlock] = sq.diag[wave];
   f32x4_t am[NT];
 #pragma unroll
   for (int rt = 0; rt < NT; ++rt) {
     f32x4_t l;
     masked(rt, rt, l, am[rt]);
-    *reinterpret_cast<f32x4_t*>(&mine.diag[rt][c * Lds::kDRow + 4 * gq]) = l;
+    *reinterpret_cast<f32x4_t*>(&diag[rt][c * Lds::kDRow + 4 * gq]) = l;
   }
   auto own_lds = [&]() {  // the wave reads back only what it wrote
     ring_fence();
@@ -580,7 +675,7 @@ __global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
   own_lds();
   // the diagonal blocks' inverses, side by side: column c of block gq, D[i] = [i == c] + sum over m < i of -L[i][m] D[m]
   {
-    const float* const block = mine.diag[gq < NT ? gq : 0];
+    const float* const block = diag[gq < NT ? gq : 0];
     float dc[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -592,21 +687,23 @@ __global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
         for (int e = 0; e < 4; ++e)
           if (4 * m4 + e < i) acc = fmaf(lr[e], dc[4 * m4 + e], acc);
       }
+      if (i % 4 == 3) asm volatile("" : "+v"(acc) : : "memory");  // or all of the block is read into registers first
       dc[i] = acc;
     }
     own_lds();
     if (gq < NT) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mine.diag[gq][i * Lds::kDRow + c] = dc[i];
+      for (int i = 0; i < 16; ++i) diag[gq][i * Lds::kDRow + c] = dc[i];
     }
     own_lds();
   }
   uint32_t most = 0;  // bits of the largest |u|; infinity and NaN lie above every number
+  Parts4 u[NT][4];
 #pragma unroll
   for (int rt = 0; rt < NT; ++rt) {
     const int n0 = 16 * rt + 4 * gq;
     const f32x4_t bv = *reinterpret_cast<const f32x4_t*>(&mine.beta[n0]), ev = *reinterpret_cast<const f32x4_t*>(&mine.eg[n0]);
-    const f32x4_t inv = *reinterpret_cast<const f32x4_t*>(&mine.diag[rt][c * Lds::kDRow + 4 * gq]);
+    const f32x4_t inv = *reinterpret_cast<const f32x4_t*>(&diag[rt][c * Lds::kDRow + 4 * gq]);
     bool present[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) present[i] = mine.seen[n0 + i] != 0ull;
@@ -619,24 +716,33 @@ __global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
         qs[rt][e][i] *= ev[i];
       }
     if (rt + 1 < NT) load_v(rt + 1);
+    // the earlier tiles, two at a time: element j < 4 of an operand is of the first one's columns, the others of the second one's
 #pragma unroll
-    for (int ct = 0; ct < rt; ++ct) {
-      f32x4_t l, m;
-      masked(rt, ct, l, m);
+    for (int ct = 0; ct < rt; ct += 2) {
+      f32x4_t l[2] = {zero, zero}, m[2] = {zero, zero};
+      masked(rt, ct, l[0], m[0]);
+      if (ct + 1 < rt) masked(rt, ct + 1, l[1], m[1]);
+      const Parts4 l0 = parts_of(l[0]), l1 = parts_of(l[1]), m0 = parts_of(m[0]), m1 = parts_of(m[1]);
+      const Parts4 none = {};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = dn_mma(l, ks[ct][e], y[e]);
-        qs[rt][e] = dn_mma(m, ks[ct][e], qs[rt][e]);
-      }
+      for (int p = 0; p < kPartProducts; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bf16x8_t x = part8(u[ct][e], ct + 1 < rt ? u[ct + 1][e] : none, right_part(p));
+          y[e] = mfma16x16x32(part8(l0, l1, left_part(p)), x, y[e]);
+          qs[rt][e] = mfma16x16x32(part8(m0, m1, left_part(p)), x, qs[rt][e]);
+        }
     }
+    f32x4_t un[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) un[e] = dn_mma(inv, y[e], zero);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      ks[rt][e] = dn_mma(inv, y[e], zero);  // u, in the place of K S
+      qs[rt][e] = dn_mma(am[rt], un[e], qs[rt][e]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) most = max(most, f32_bits(ks[rt][e][i]) & 0x7fffffffu);
+      for (int i = 0; i < 4; ++i) most = max(most, f32_bits(un[e][i]) & 0x7fffffffu);
+      if (rt + 1 < NT) u[rt][e] = parts_of(un[e]);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) qs[rt][e] = dn_mma(am[rt], ks[rt][e], qs[rt][e]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = n0 + i;
@@ -648,7 +754,7 @@ __global__ __launch_bounds__(W* kWave) void k_tree_rule(TreeRuleArgs a) {
   odd |= __ballot(most >= 0x7f800000u) != 0ull;
   if (odd) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above, before those of the same places
-    tree_rule_again<DK, NT, W>(a, s, wave, state, row, head, col - 4 * c + lane);
+    tree_rule_again<DK, NT, W>(a, s, wave, state, row, kh, head, col - 4 * c + lane);
   }
 }
 
@@ -745,17 +851,24 @@ int tree_rule_waves(const TreeRuleArgs& a, int64_t rows, hipStream_t st) {
   return status_of(hipGetLastError());
 }
 
+// Four waves a workgroup: two lanes of 7 nodes 10.0 us, with eight 13.1; 48 of 16 53.1 / 55.4; 24 of 32 47.5 / 49.5. Above 32 nodes
+// LDS holds one workgroup a compute unit, and one of eight waves takes five thirds of the time of one of four (8 lanes of
+// 61: 256 of four 30.1, 128 of eight 41.6; 12: 384 of four 55.5, 192 of eight 46.5; 24 of 48: 768 of four 82.9, 384 of eight 94.7).
 template <int DK, int NT>
 int tree_rule_tiles(const TreeRuleArgs& a, int64_t rows, hipStream_t st) {
-  const int64_t units = (int64_t)a.rep * a.slabs;
-  if (units >= 8 && rows * a.qk_heads * units >= 8 * device_cu_count()) return tree_rule_waves<DK, NT, 8>(a, rows, st);
-  return tree_rule_waves<DK, NT, 2>(a, rows, st);
+  if constexpr (NT > 2) {
+    const int64_t units = (int64_t)a.rep * a.slabs, shared = rows * a.qk_heads, cus = device_cu_count();
+    auto rounds = [&](int64_t waves) { return (shared * ((units + waves - 1) / waves) + cus - 1) / cus; };
+    if (units >= 8 && 5 * rounds(8) < 3 * rounds(4)) return tree_rule_waves<DK, NT, 8>(a, rows, st);
+  }
+  return tree_rule_waves<DK, NT, 4>(a, rows, st);
 }
 
 template <int DK>
 int tree_rule_launch(const TreeRuleArgs& a, int64_t rows, hipStream_t st) {
   if (a.t <= 16) return tree_rule_tiles<DK, 1>(a, rows, st);
   if (a.t <= 32) return tree_rule_tiles<DK, 2>(a, rows, st);
+  if (a.t <= 48) return tree_rule_tiles<DK, 3>(a, rows, st);
   return tree_rule_tiles<DK, 4>(a, rows, st);
 }
 

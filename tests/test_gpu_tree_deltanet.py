@@ -31,7 +31,7 @@ SHAPES = [  # heads, q/k heads, k_dim, v_dim
 
 @pytest.mark.parametrize("heads,qk,dk,dv", SHAPES)
 @pytest.mark.parametrize("t,kinds", [(1, ["chain"]), (2, ["star", "empty"]), (7, ["random", "gaps", "forest"]), (16, ["deep", "random"]),
-                                     (17, ["gaps"]), (33, ["random", "chain"]), (61, ["random"]), (64, ["deep", "gaps"])])
+                                     (17, ["gaps"]), (33, ["random", "chain"]), (48, ["gaps", "random"]), (49, ["forest"]), (61, ["random"]), (64, ["deep", "gaps"])])
 def test_rule(dev, heads, qk, dk, dv, t, kinds) -> None:
     b = len(kinds)
     pool, slots, q, k, v, g, beta = _case(t + dk + heads, b + 2, heads, qk, dk, dv, b, t)
