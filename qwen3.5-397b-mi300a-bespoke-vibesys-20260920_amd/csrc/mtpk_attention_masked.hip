@@ -227,6 +227,10 @@ __device__ inline void load_lds(rsrc_t r, uint8_t* to, uint32_t off) {
 // their exponentials and sums stay inside fp32's and bf16's range as they are, and so the largest part of
 // the work between the two products falls away. A row whose sum all the same comes out below least_sum (its
 // keys all far below, or none: 0), or that holds a value that is not finite, is done again by masked_row_slow.
+// In a tree the maximum that a row's weights are taken against moves only when a score passes it by more than kRise: the weights
+// stay below 2^kRise, which fp32 sums and bf16 hold as well as those below 1, and the sums of a wave, which some of its 32
+// rows would have multiplied again in nearly every tile, in few.
+constexpr float kRise = 8.f;
 constexpr float kUnseen = -1e18f, kNoKey = -1e17f, kCapMost = 100.f;
 
 // The cap alone leaves every key at least 2^-100. A bias may take keys below 2^-126, where they are lost: up to 2^20
@@ -284,7 +288,7 @@ struct TileSoftmax {
         return (uint32_t)(16 * (i >> 3) + (i & 7) - lo) < (uint32_t)n;
     };
     auto past = [&]() { return __ballot(!(top <= a.cubic_max)) != 0ull; };
-    bool bent = CAP ? past() : a.cap2 > 0.f;  // past the cap's cubic part
+    bool bent = CAP ? past() : !TREE && a.cap2 > 0.f;  // past the cap's cubic part
     if (CAP && bent && !whole) {  // keys that no row sees have no part in the choice of the form
       begin();
 #pragma unroll
@@ -326,6 +330,16 @@ struct TileSoftmax {
       }
     }
     if (CAP) return 1.f;
+    if constexpr (TREE) {
+      const float now = halves_max(top * c0);
+      const bool up = now > r.m + kRise;
+      ms = up ? now : r.m;
+      if (__ballot(up) == 0ull) return 1.f;  // uniform
+      const float alpha = __builtin_amdgcn_exp2f(r.m - ms);
+      r.m = ms;
+      r.l *= alpha;
+      return alpha;
+    }
     ms = fmaxf(r.m, halves_max(top * c0));
     const float alpha = __builtin_amdgcn_exp2f(r.m - ms);
     r.m = ms;
@@ -1078,7 +1092,7 @@ __global__ __launch_bounds__(W* kWave, 1) void k_masked_few(MaskedArgs a) {
 // Merge of the key splits: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M = max_s m_s. W waves a
 // row: each weighs all splits at once (lane s split s), then takes every W-th split, four of them in
 // flight; the waves' sums are added in order.
-template <int HD, int W, bool TREE = false>
+template <int HD, int W>
 __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, int group_rows) {
   constexpr int NV = HD / kWave;
   typedef float vec_t __attribute__((ext_vector_type(NV)));
@@ -1126,7 +1140,88 @@ __global__ __launch_bounds__(256) void k_masked_merge(MaskedArgs a, int rows, in
     odd = fmaf(y, 0.f, odd);
     orow[e] = f32_to_bf16(grow ? y * sigmoid_of(grow[e]) : y);
   }
-  if (__ballot(odd != 0.f) != 0ull) masked_row_slow<HD, TREE>(a, b, hq, st, lane);
+  if (__ballot(odd != 0.f) != 0ull) masked_row_slow<HD>(a, b, hq, st, lane);
+}
+
+// The same of a tree's rows, workgroup (x, y) of node x of all lanes: everything that a row is made of is on its way at once,
+// the splits' sums before their weights are known (a split without keys has none written, and its garbage is left out). Up
+// to 8 splits with a wave a row, 4 heads to a workgroup, which weighs them without a word between lanes (24,576 rows of 2
+// splits of 256: 14.8 us, with the form above 19.7); beyond, a workgroup a row (2016 of 32 splits of 128: 8.7, 10.0).
+template <int HD, int W, int N>
+__global__ __launch_bounds__(256, N* HD > 2048 ? 4 : 6) void k_tree_merge(MaskedArgs a, int group_rows) {
+  constexpr int NV = HD / kWave;
+  typedef float vec_t __attribute__((ext_vector_type(NV)));
+  __shared__ vec_t red[W][kWave];
+  const int lane = threadIdx.x & (kWave - 1), part = uniform((int)threadIdx.x / kWave), wave = W == 1 ? 0 : part;
+  const int hq = W == 1 ? (int)blockIdx.y * 4 + part : (int)blockIdx.y, bs = (int)blockIdx.x;
+  if (hq >= a.heads) return;  // uniform over the wave (W == 1: no barrier below)
+  const int group = a.heads / a.kvh, b = bs / a.t, st = bs - b * a.t, kh = hq / group;
+  const int r = st * group + hq - kh * group, rg = r / group_rows, rl = r - rg * group_rows;
+  const int64_t base = (((int64_t)(b * a.kvh + kh) * a.row_groups + rg) * a.n_split) * group_rows + rl;
+  uint16_t* const orow = a.out + a.orow.at(b, hq, st) + NV * lane;
+  const uint16_t* const grow = a.gate ? a.gate + a.gr.at(b, hq, st) + NV * lane : nullptr;
+  uint16_t gate[NV] = {};
+  if (grow) {
+#pragma unroll
+    for (int e = 0; e < NV; ++e) gate[e] = grow[e];
+  }
+  vec_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int s = min(wave + W * i, a.n_split - 1);  // no branch around a load: past the last split, that one again
+    v[i] = *reinterpret_cast<const vec_t*>(a.part_o + (base + (int64_t)s * group_rows) * HD + NV * lane);
+  }
+  float w[N], sum = 0.f;
+  const float* const ml = a.part_ml + base * 2;
+  if constexpr (W == 1) {
+    float m[N], l[N], mx = kNoKey;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float2 x = *reinterpret_cast<const float2*>(ml + (int64_t)min(i, a.n_split - 1) * group_rows * 2);
+      m[i] = i < a.n_split ? x.x : -INFINITY;
+      l[i] = i < a.n_split ? x.y : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) mx = fmaxf(mx, m[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(m[i] - mx);
+      sum = fmaf(l[i], w[i], sum);
+      if (m[i] == -INFINITY) v[i] = vec_t{};
+    }
+  } else {
+    const bool live = lane < a.n_split;
+    const float2 x = *reinterpret_cast<const float2*>(ml + (int64_t)min(lane, a.n_split - 1) * group_rows * 2);
+    const float m = live ? x.x : -INFINITY, l = live ? x.y : 0.f;
+    const float mx = fmaxf(wave_max(m), kNoKey), wt = __builtin_amdgcn_exp2f(m - mx);
+    sum = wave_sum(l * wt);
+    const uint64_t held = __ballot(m != -INFINITY);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int s = wave + W * i;
+      w[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wt), s));
+      if (!(held >> s & 1ull)) v[i] = vec_t{};  // nor past the last split
+    }
+  }
+  vec_t acc = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc += v[i] * w[i];
+  if (W > 1) {
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) acc += red[i][lane];
+  }
+  const float inv = row_inverse(sum);
+  float odd = sum < least_sum(a) ? 1.f : 0.f;
+#pragma unroll
+  for (int e = 0; e < NV; ++e) {
+    const float y = acc[e] * inv;
+    odd = fmaf(y, 0.f, odd);
+    orow[e] = f32_to_bf16(grow ? y * sigmoid_of(gate[e]) : y);
+  }
+  if (__ballot(odd != 0.f) != 0ull) masked_row_slow<HD, true>(a, b, hq, st, lane);
 }
 
 namespace {
@@ -1184,10 +1279,33 @@ int masked_launch(const MaskedArgs& a, int64_t batch, hipStream_t st) {
   int rc = status_of(hipGetLastError());
   if (rc || a.n_split == 1) return rc;
   const int out_rows = (int)(batch * a.heads * a.t), group_rows = (int)masked_group_rows(rows);
-  if (a.n_split <= kMergeOne)
-    hipLaunchKernelGGL((k_masked_merge<HD, 1, TREE>), dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, a, out_rows, group_rows);
+  if constexpr (TREE) {
+    const unsigned nodes = (unsigned)(batch * a.t), heads = (unsigned)a.heads;
+    auto merge = [&](auto waves, auto n) {
+      const unsigned y = waves == 1 ? (heads + 3) / 4 : heads;
+      hipLaunchKernelGGL((k_tree_merge<HD, decltype(waves)::value, decltype(n)::value>), dim3(nodes, y), dim3(256), 0, st, a, group_rows);
+    };
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    constexpr std::integral_constant<int, 8> eight{};
+    constexpr std::integral_constant<int, 16> sixteen{};
+    if (a.n_split <= 2)
+      merge(one, two);
+    else if (a.n_split <= 4)
+      merge(one, four);
+    else if (a.n_split <= 8)
+      merge(one, eight);
+    else if (a.n_split <= 16)
+      merge(four, four);
+    else if (a.n_split <= 32)
+      merge(four, eight);
+    else
+      merge(four, sixteen);
+  } else if (a.n_split <= kMergeOne)
+    hipLaunchKernelGGL((k_masked_merge<HD, 1>), dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, a, out_rows, group_rows);
   else
-    hipLaunchKernelGGL((k_masked_merge<HD, 4, TREE>), dim3((unsigned)out_rows), dim3(256), 0, st, a, out_rows, group_rows);
+    hipLaunchKernelGGL((k_masked_merge<HD, 4>), dim3((unsigned)out_rows), dim3(256), 0, st, a, out_rows, group_rows);
   return status_of(hipGetLastError());
 }
 
@@ -1349,6 +1467,7 @@ int mtpk_paged_attention_tree(const uint16_t* q, const int64_t* q_strides, const
   if (!masked_operands(a, q, q_strides, gate, gate_strides, batch, t, heads, kv_heads, head_dim, k_pool, v_pool, pool_rows,
                        block_table, table_stride, base_pos, scale, n_split, workspace, workspace_bytes, out, out_strides))
     return MTPK_EINVAL;
+  if (heads > 65535) return MTPK_EINVAL;  // the merge's grid
   a.tree = {parents, parents_dtype, parents_strides[0], parents_strides[1]};
   const hipStream_t st = (hipStream_t)stream;
   switch (head_dim) {

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import attention
-from oracle import tree_ref
+from oracle import masked_attention_ref, tree_ref
 from tests import tree_inputs
 
 pytestmark = pytest.mark.gpu
@@ -83,10 +83,15 @@ def test_key_splits(dev) -> None:
 
 @pytest.mark.parametrize("heads,kvh,hd,t,base", [(8, 2, 64, 4, [40]), (16, 4, 128, 20, [100, 3]), (32, 2, 256, 6, [3000])])
 def test_a_chain_is_the_causal_order(dev, heads, kvh, hd, t, base) -> None:
+    """Both calls are within their bars of the same 64-bit values, so within two of them of each other: their sums run in
+    different orders."""
     q, k, v, table, b0 = case(t, len(base), t, heads, kvh, hd, base)
-    got = run(dev, q, k, v, table, b0, hd**-0.5, tree_inputs.batch(["chain"] * len(base), t))
+    got = check(dev, q, k, v, table, b0, hd**-0.5, tree_inputs.batch(["chain"] * len(base), t))
+    want, spread = masked_attention_ref.paged_attention_masked(q, k, v, table, b0, hd**-0.5)
+    assert float(((got - want).abs() / bars(want, spread)).max()) <= 1.0
     args = (q.to(dev), k.to(dev), attention.v_blocks(v).to(dev), table.to(dev), b0.to(dev), max(base) + t, hd**-0.5)
-    assert torch.equal(got, attention.paged_attention_masked(*args))
+    other = attention.paged_attention_masked(*args).double().cpu()
+    assert float(((got - other).abs() / bars(want, spread)).max()) <= 2.0
 
 
 @pytest.mark.parametrize("heads,kvh,hd,t,base", [(8, 2, 64, 4, [40]), (16, 4, 128, 20, [100, 3]), (32, 2, 256, 16, [3000, 64]),
