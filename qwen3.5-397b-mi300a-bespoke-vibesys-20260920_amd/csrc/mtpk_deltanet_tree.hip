@@ -17,14 +17,14 @@ constexpr int kTreeHeadMost = 256;  // widest head of the preparation
 //
 // As mtpk_deltanet_prep, but the columns before a node are its ancestors' (then the stored window's), which are the
 // highest bits of its ancestors. A wave takes one head unit (the q heads, the k heads, the v heads, and one more for g
-// and beta) of up to kPrepNodes nodes of a lane: lane l holds channels 2 l, 2 l + 1 (+ 128), and the columns of all
+// and beta) of up to R nodes of a lane: lane l holds channels 2 l, 2 l + 1 (+ 128), and the columns of all
 // nodes and taps are on their way at once.
 //
 // The convolution's output is a tensor of the model's type. Next to a rounding's border the order of the products decides
-// to which side a value goes, half a step of bf16 either way; bf16 rows are therefore summed in 64 bits (their products
-// are exact in 32), and the few outputs that 32 bits put within 2^-12 of a step of the border (1 in 2000) have their SiLU
-// done again in 64. Of f32 rows there is nothing to round, and the sums run as in mtpk_deltanet_prep.
-constexpr int kPrepNodes = 4;
+// to which side a value goes, half a step of bf16 either way: the few outputs of bf16 rows that lie nearer to one than 32
+// bits tell (1 in some 500) are done again in 64, from the products, which are exact. Of f32 rows there is nothing to round,
+// and the sums run as in mtpk_deltanet_prep.
+constexpr int kPrepThreads = 256;
 
 struct TreePrepArgs {
   const void* proj;  // [B * t, proj_stride]: qkv (C), z, b (vh), a (vh)
@@ -49,35 +49,45 @@ __device__ inline float tree_float(const void* p, int64_t i) {
     return static_cast<const float*>(p)[i];
 }
 
-// Channels ch, ch + 1 of element i; `two`: both exist. PAIR: a dword of two bf16.
+// Channels c, c + 1 of row `row` of the lane's rows in `r`, `stride` bytes apart; `two`: both exist. PAIR: a dword of two bf16.
 template <typename T, bool PAIR>
-__device__ inline float2 tree_pair(const void* p, int64_t i, bool two) {
+__device__ inline float2 tree_pair(rsrc_t r, int c, int row, int stride, bool two) {
+  const int off = c * (int)sizeof(T), at = row * stride;
   if constexpr (PAIR) {
-    const uint32_t d = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+    const uint32_t d = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, off, at, 0);
     return make_float2(bits_f32(d << 16), bits_f32(d & 0xffff0000u));
+  } else if constexpr (sizeof(T) == 2) {
+    const uint32_t d = (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, at, 0) & 0xffffu;
+    const uint32_t e = (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, two ? off + 2 : off, at, 0) & 0xffffu;
+    return make_float2(bits_f32(d << 16), two ? bits_f32(e << 16) : 0.f);
   } else {
-    return make_float2(tree_float<T>(p, i), two ? tree_float<T>(p, i + 1) : 0.f);
+    typedef uint32_t pair_t __attribute__((ext_vector_type(2)));
+    const pair_t d = __builtin_bit_cast(pair_t, __builtin_amdgcn_raw_buffer_load_b64(r, off, at, 0));
+    return make_float2(bits_f32(d[0]), two ? bits_f32(d[1]) : 0.f);
   }
 }
 
 __device__ inline float tree_silu(float x) { return x / (1.f + expf(-x)); }
 
-// SiLU of the exact sum x, rounded to bf16.
-__device__ inline float tree_silu_bf16(double x) {
-  float y = tree_silu((float)x);
-  const uint32_t away = (f32_bits(y) + 0x8010u) & 0xffffu;  // 16 on the border between two bf16 values
-  if (away <= 32u) y = (float)(x / (1.0 + exp(-x)));
-  return bf16_to_f32(f32_to_bf16(y));
+// The same within 8 units of the last place, in half of the instructions: e^-x as 2^p (1 + what p was rounded by), the
+// division by a reciprocal and a step towards the exact quotient.
+__device__ inline float tree_silu_near(float x) {
+  constexpr float kLog2eHi = 1.44269502f, kLog2eLo = 1.92596303e-8f;
+  const float p = -x * kLog2eHi, rest = fmaf(-x, kLog2eLo, fmaf(-x, kLog2eHi, -p)), e = __builtin_amdgcn_exp2f(p);
+  const float d = 1.f + fmaf(e, rest * 0.693147182f, e), r = __builtin_amdgcn_rcpf(d), y = x * r;
+  return d < INFINITY ? fmaf(fmaf(-d, y, x), r, y) : y;
 }
 
 // K: conv_k, or 0 for any. NI: 128-channel parts of a head.
-template <typename T, int K, bool PAIR, int NI>
-__global__ __launch_bounds__(kWave) void k_tree_prep(TreePrepArgs a) {
-  constexpr int R = kPrepNodes, KM = K ? K : kTreeConvMost + 1;
-  const int lane = threadIdx.x;
+template <typename T, int K, bool PAIR, int NI, int R>
+__global__ __launch_bounds__(kPrepThreads) void k_tree_prep(TreePrepArgs a) {
+  constexpr int KM = K ? K : kTreeConvMost + 1;
+  const int lane = threadIdx.x & (kWave - 1);
   const int conv_k = K ? K : a.conv_k, k1 = conv_k - 1;
   const int units = 2 * a.kh + a.vh + 1, groups = (a.t + R - 1) / R;
-  const int u = blockIdx.x % units, br = blockIdx.x / units, b = br / groups, s0 = (br - b * groups) * R;
+  const int64_t id = (int64_t)blockIdx.x * (kPrepThreads / kWave) + uniform((int)threadIdx.x / kWave);
+  if (id >= (int64_t)a.B * groups * units) return;
+  const int u = (int)(id % units), br = (int)(id / units), b = br / groups, s0 = (br - b * groups) * R;
   const int64_t row0 = (int64_t)b * a.t;
   const int C = 2 * a.kh * a.kd + a.vh * a.vd;
   const int parent = a.parents.at(b, lane, a.t);
@@ -142,6 +152,8 @@ __global__ __launch_bounds__(kWave) void k_tree_prep(TreePrepArgs a) {
   // tap j of node s0 + r: its ancestor conv_k - 1 - j generations up, or column `from` of the stored window
   float2 x[R][NI][KM];
   uint64_t way[R];
+  const int stride = (int)(a.proj_stride * (int)sizeof(T));
+  const rsrc_t rows = make_rsrc(static_cast<const T*>(a.proj) + row0 * a.proj_stride, (uint32_t)((a.t - 1) * stride + C * (int)sizeof(T)));
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     way[r] = s0 + r < a.t ? lane_bits(seen, s0 + r) : 0ull;
@@ -155,7 +167,7 @@ __global__ __launch_bounds__(kWave) void k_tree_prep(TreePrepArgs a) {
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         const int ch = 2 * lane + 128 * n, c = c0 + (ch < dim ? ch : 0);
-        x[r][n][j] = tree_pair<T, PAIR>(a.proj, (row0 + i) * a.proj_stride + c, ch + 1 < dim);
+        x[r][n][j] = tree_pair<T, PAIR>(rows, c, i, stride, ch + 1 < dim);
       }
     }
   }
@@ -163,6 +175,18 @@ __global__ __launch_bounds__(kWave) void k_tree_prep(TreePrepArgs a) {
   for (int r = 0; r < R; ++r) {
     if (s0 + r >= a.t) continue;
     const int above = __builtin_popcountll(way[r]);  // columns of the tree
+    // the columns before those are the stored window's last ones: tap j has column j + above - 1
+    if (above < conv_k) {  // uniform, and rare past the first generations
+#pragma unroll
+      for (int d = 0; d < KM; ++d) {
+        if (d != above) continue;
+#pragma unroll
+        for (int j = 0; j < KM; ++j)
+#pragma unroll
+          for (int n = 0; n < NI; ++n)
+            if (j + d < conv_k) x[r][n][j] = j + d > 0 ? stored[n][j + d - 1 < KM - 1 ? j + d - 1 : 0] : make_float2(0.f, 0.f);
+      }
+    }
     float2 y[NI];
     float ss = 0.f;
 #pragma unroll
@@ -171,26 +195,31 @@ __global__ __launch_bounds__(kWave) void k_tree_prep(TreePrepArgs a) {
       float f[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float acc = 0.f;
-        double exact = 0.;
+        float acc = 0.f, size = 0.f, prod[KM];
 #pragma unroll
         for (int j = 0; j < KM; ++j) {
           if (j >= conv_k) continue;
-          const int up = conv_k - 1 - j;  // generations
-          float col = e ? x[r][n][j].y : x[r][n][j].x;
-          if (up >= above) {  // uniform
-            col = 0.f;
-#pragma unroll
-            for (int i = 0; i < KM - 1; ++i)
-              if (i == k1 - 1 - (up - above)) col = e ? stored[n][i].y : stored[n][i].x;
-          }
-          const float prod = __fmul_rn(col, e ? w[n][j].y : w[n][j].x);
-          if constexpr (sizeof(T) == 2)
-            exact += (double)prod;
-          else
-            acc = j == 0 ? prod : __fadd_rn(acc, prod);
+          prod[j] = __fmul_rn(e ? x[r][n][j].y : x[r][n][j].x, e ? w[n][j].y : w[n][j].x);
+          acc = j == 0 ? prod[j] : __fadd_rn(acc, prod[j]);
+          size += fabsf(prod[j]);
         }
-        f[e] = ch + e < dim ? (sizeof(T) == 2 ? tree_silu_bf16(exact) : tree_silu(acc)) : 0.f;
+        if constexpr (sizeof(T) == 2) {
+          // An addition is off by 2^-24 of what it gives, which is at most the products' size, SiLU's slope is below 1.1, and
+          // its own error below 2^-22 of the value (2^-23 of the exponential, 2^-24 of the sum, the quotient and its step each).
+          float y = tree_silu_near(acc);
+          const float border = bits_f32((f32_bits(y) & 0xffff0000u) | 0x8000u);  // between two bf16 values
+          if (!(fabsf(y - border) > fmaf((float)k1 * 0x1.2p-24f, size, 0x1.4p-22f * fabsf(y)))) {
+            double exact = 0.;
+#pragma unroll
+            for (int j = 0; j < KM; ++j)
+              if (j < conv_k) exact += (double)prod[j];
+            y = (float)(exact / (1.0 + exp(-exact)));
+          }
+          f[e] = bf16_to_f32(f32_to_bf16(y));
+        } else {
+          f[e] = tree_silu(acc);
+        }
+        if (ch + e >= dim) f[e] = 0.f;
         ss += f[e] * f[e];
       }
       y[n] = make_float2(f[0], f[1]);
@@ -219,15 +248,27 @@ __global__ __launch_bounds__(kWave) void k_tree_prep(TreePrepArgs a) {
   }
 }
 
+// Nodes of a wave: the way to a node and the weights are the wave's, four nodes share them where there are waves enough. bf16, 96
+// head units, two / four: one lane of 7 nodes 4.2 / 5.9 us, 8 of 16 8.0 / 8.6, 48 of 4 10.6 / 10.3, 48 of 16 26.2 / 23.3 (eight 32).
+// Bound by its instructions, of which SiLU and its border are the most: 60.8 MB in 23.3 us.
+template <typename T, int K, bool PAIR, int NI, int R>
+int launch_tree_prep_nodes(const TreePrepArgs& a, hipStream_t st) {
+  const int64_t waves = (int64_t)a.B * ((a.t + R - 1) / R) * (2 * a.kh + a.vh + 1), n = (waves + 3) / 4;
+  if (n > kMaxGroups) return MTPK_EINVAL;
+  hipLaunchKernelGGL((k_tree_prep<T, K, PAIR, NI, R>), dim3((unsigned)n), dim3(kPrepThreads), 0, st, a);
+  return status_of(hipGetLastError());
+}
+
+template <typename T, int K, bool PAIR, int NI>
+int launch_tree_prep_heads(const TreePrepArgs& a, hipStream_t st) {
+  if (a.t <= 2) return launch_tree_prep_nodes<T, K, PAIR, NI, 2>(a, st);
+  if ((int64_t)a.B * a.t * (2 * a.kh + a.vh) >= 64 * (int64_t)device_cu_count()) return launch_tree_prep_nodes<T, K, PAIR, NI, 4>(a, st);
+  return launch_tree_prep_nodes<T, K, PAIR, NI, 2>(a, st);
+}
+
 template <typename T, int K, bool PAIR>
 int launch_tree_prep(const TreePrepArgs& a, hipStream_t st) {
-  const int64_t groups = (a.t + kPrepNodes - 1) / kPrepNodes, n = (int64_t)a.B * groups * (2 * a.kh + a.vh + 1);
-  if (n > 4 * kMaxGroups) return MTPK_EINVAL;  // one-wave workgroups
-  if (a.kd > 128 || a.vd > 128)
-    hipLaunchKernelGGL((k_tree_prep<T, K, PAIR, 2>), dim3((unsigned)n), dim3(kWave), 0, st, a);
-  else
-    hipLaunchKernelGGL((k_tree_prep<T, K, PAIR, 1>), dim3((unsigned)n), dim3(kWave), 0, st, a);
-  return status_of(hipGetLastError());
+  return a.kd > 128 || a.vd > 128 ? launch_tree_prep_heads<T, K, PAIR, 2>(a, st) : launch_tree_prep_heads<T, K, PAIR, 1>(a, st);
 }
 
 // ---------------------------------------------------------------- the rule, step by step
@@ -891,7 +932,8 @@ int mtpk_deltanet_prep_tree(const void* proj, int dtype, int64_t proj_stride, co
     return MTPK_EINVAL;
   if (k_dim < 1 || k_dim > kTreeHeadMost || v_dim < 1 || v_dim > kTreeHeadMost) return MTPK_EINVAL;
   const int64_t C = 2 * k_heads * k_dim + v_heads * v_dim;
-  if (proj_stride < C + v_heads * v_dim + 2 * v_heads) return MTPK_EINVAL;
+  // a lane's rows are one buffer of less than 2^31 bytes
+  if (proj_stride < C + v_heads * v_dim + 2 * v_heads || proj_stride >= (int64_t(1) << 31) / (4 * kTreeNodes)) return MTPK_EINVAL;
   if (batch == 0) return 0;
   if (!proj || !conv_state || !slot || !conv_w || !a_log || !dt_bias || !parents || !parents_strides || !q || !k || !v || !g || !beta)
     return MTPK_EINVAL;
@@ -899,7 +941,7 @@ int mtpk_deltanet_prep_tree(const void* proj, int dtype, int64_t proj_stride, co
                        {parents, parents_dtype, parents_strides[0], parents_strides[1]}, (int)batch, (int)t, (int)k_heads, (int)k_dim,
                        (int)v_heads, (int)v_dim, (int)conv_k, eps, q_scale, q, k, v, g, beta};
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == MTPK_F32) return launch_tree_prep<float, 0, false>(a, st);
+  if (dtype == MTPK_F32) return conv_k == 4 ? launch_tree_prep<float, 4, false>(a, st) : launch_tree_prep<float, 0, false>(a, st);
   auto at = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const bool pair = conv_k == 4 && proj_stride % 2 == 0 && k_dim % 2 == 0 && v_dim % 2 == 0 && at(proj, 4) && at(conv_state, 4) &&
                     at(conv_w, 16) && at(q, 8) && at(k, 8) && at(v, 8);
