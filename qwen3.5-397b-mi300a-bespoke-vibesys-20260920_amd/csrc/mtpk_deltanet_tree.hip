@@ -941,7 +941,7 @@ int mtpk_deltanet_prep_tree(const void* proj, int dtype, int64_t proj_stride, co
                        {parents, parents_dtype, parents_strides[0], parents_strides[1]}, (int)batch, (int)t, (int)k_heads, (int)k_dim,
                        (int)v_heads, (int)v_dim, (int)conv_k, eps, q_scale, q, k, v, g, beta};
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == MTPK_F32) return conv_k == 4 ? launch_tree_prep<float, 4, false>(a, st) : launch_tree_prep<float, 0, false>(a, st);
+  if (dtype == MTPK_F32) return launch_tree_prep<float, 0, false>(a, st);
   auto at = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
   const bool pair = conv_k == 4 && proj_stride % 2 == 0 && k_dim % 2 == 0 && v_dim % 2 == 0 && at(proj, 4) && at(conv_state, 4) &&
                     at(conv_w, 16) && at(q, 8) && at(k, 8) && at(v, 8);
