@@ -392,6 +392,42 @@ def _verify_rows(model, m, buf: MTPVerifyBuffers, ctx_len: int) -> None:
         model.hidden_cache[slots] = torch.where(active[:, None], seed, model.hidden_cache[slots])
 
 
+def verify_tree(model, lanes, tokens: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, budget: torch.Tensor,
+                stops: torch.Tensor, ctx_len: int, *, mtp=None, active: torch.Tensor | None = None,
+                block_table: torch.Tensor | None = None) -> TreeAccept:
+    """One verify round over trees of drafts, `verify_round_step` for drafts that branch: the forward of every node
+    (`Model.forward_rows(parents=)`), the acceptance of one path per lane (`tree_accept`), and the commit along it of the cache
+    rows, the DeltaNet states (`Model.commit_path`), the MTP cache and the hidden seed. The slots are then where the accepted
+    tokens, one after another, would have left them; `bonus` is each lane's next token, at `next_pos`.
+
+    `tokens` int64 `[B, t]`, t up to 64, node 0 the lane's last committed token at `pos` `[B]`; `parents` `[B, t]` as in
+    `attention.paged_attention_tree`; `budget`, `stops` as in `tree_accept`; `ctx_len` a host bound on `max(pos) + t`. The lanes'
+    blocks must hold `pos + t` positions (`BlockTables.grow_many`). `mtp` defaults to the model's attached head. Rows with
+    `active` False touch no lane state. No host read: the call can be captured."""
+    lanes = model.lane_index(lanes)
+    b, t = tokens.shape
+    m = model.mtp if mtp is None else mtp
+    act = torch.ones(b, dtype=torch.bool, device=tokens.device) if active is None else active
+    table = model.blocks.table[lanes] if block_table is None else block_table
+    res = model.forward_rows(tokens, lanes, pos, ctx_len, block_table=table, active=act, final_norm=True, parents=parents)
+    best = model.next_tokens(res.normed.reshape(b * t, -1)).view(b, t)
+    out = tree_accept(best, tokens, parents, act, pos, budget, stops)
+    model.commit_path(res, lanes, pos, out.path, out.lengths, block_table=table, active=act)
+    at = torch.arange(b, device=tokens.device)[:, None]
+    hidden, ids = res.hidden[at, out.path], tokens[at, out.path]
+    if m is not None:
+        grid = pos[:, None] + torch.arange(t, device=tokens.device)
+        previous = torch.cat([model.hidden_cache[lanes][:, None], hidden[:, :-1]], dim=1)
+        rows = None if vm.kv_write_in_kernel(model) else vm.table_rows(table, grid, model.cfg.block_size)
+        mtp_mod.cache_target_rows(model, m, ids, previous, grid, rows, out.keep, block_table=table, base_pos=pos)
+    if tokens.is_cuda:
+        copy_rows(res.hidden.reshape(b * t, -1), out.hidden_src, model.hidden_cache, torch.where(act, lanes, -1))
+    else:
+        seed = res.hidden.reshape(b * t, -1)[out.hidden_src]
+        model.hidden_cache[lanes] = torch.where(act[:, None], seed, model.hidden_cache[lanes])
+    return out
+
+
 def copy_rows(src: torch.Tensor, src_idx: torch.Tensor, dst: torch.Tensor, dst_idx: torch.Tensor) -> None:
     """`dst[dst_idx[j]] = src[src_idx[j]]` on device 2-D tensors of one dtype and row width (rows
     at any stride), skipping every j whose index lies outside its table: `mtpk_copy_rows`."""

@@ -231,6 +231,20 @@ def causal_conv_rows(window: torch.Tensor, weight: torch.Tensor, t: int) -> torc
     return F.silu(acc)
 
 
+def tree_windows(stored: torch.Tensor, raw: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
+    """The convolution's columns of every node of trees `parents` `[B, t]`, oldest first, `[B, t, C, conv_k]`: its own of
+    `raw` `[B, C, t]`, its nearest ancestors', and where its way is shorter the last ones of `stored` `[B, C, conv_k - 1]`."""
+    b, _, t = raw.shape
+    lane = torch.arange(b, device=raw.device)
+    after: list[torch.Tensor] = [stored]
+    out = []
+    for s in range(t):
+        above = torch.stack(after, 1)[lane, parents[:, s].long().clamp(-1, s - 1) + 1]
+        out.append(torch.cat([above, raw[:, :, s : s + 1]], dim=-1))
+        after.append(out[-1][..., 1:])
+    return torch.stack(out, 1)
+
+
 def delta_rule_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                     g: torch.Tensor, beta: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """One gated delta-rule step for every (slot, head) (`model.py:651-697`):
@@ -245,9 +259,48 @@ def delta_rule_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     return s, out
 
 
+def tree_ancestors(parents: torch.Tensor) -> torch.Tensor:
+    """bool `[B, t, t]`: whether node j is node i or one of its ancestors, in the trees `parents` `[B, t]` of
+    `attention.paged_attention_tree`; False rows for absent nodes. No host read."""
+    b, t = parents.shape
+    rows: list[torch.Tensor] = []
+    for i in range(t):
+        p = parents[:, i].long()
+        ok = (p >= -1) & (p < i)
+        above = torch.zeros(b, t, dtype=torch.bool, device=parents.device)
+        if i:
+            up = p.clamp(0, i - 1)
+            lane = torch.arange(b, device=parents.device)
+            above = torch.stack(rows, 1)[lane, up] & (p >= 0)[:, None]
+            ok = ok & ((p < 0) | above.any(1))
+        above = above & ok[:, None]
+        above[:, i] = ok
+        rows.append(above)
+    return torch.stack(rows, 1)
+
+
+def tree_depths(parents: torch.Tensor) -> torch.Tensor:
+    """int64 `[B, t]`: how many ancestors each node has (0 for an absent one): its position is the lane's base plus that.
+    Found by doubling the ways up, without a host read."""
+    b, t = parents.shape
+    node = torch.arange(t, device=parents.device)
+    p = parents.long()
+    ok = (p >= -1) & (p < node)
+    lost = t + 1  # where absent nodes and what hangs below them end up; t is the context
+    up = torch.where(ok, torch.where(p < 0, t, p), lost)
+    up = torch.cat([up, torch.full((b, 2), lost, device=p.device)], 1)
+    up[:, t] = t
+    n = torch.ones_like(up)
+    n[:, t:] = 0
+    for _ in range((t - 1).bit_length() + 1):
+        n = n + n.gather(1, up)
+        up = up.gather(1, up)
+    return torch.where(up[:, :t] == t, n[:, :t] - 1, 0)
+
+
 def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                     block_table: torch.Tensor, base_pos: torch.Tensor, ctx_blocks: int,
-                    block_size: int, scale: float) -> torch.Tensor:
+                    block_size: int, scale: float, parents: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of `t` new query rows per lane over the paged cache
     (`verify_attention_paged`, `model.py:1120-1205`). `q` `[B, heads, t, hd]`; the pools (K
     `[rows, kv_heads, hd]`, V `[rows / block, kv_heads, hd, block]`, see `attention.v_blocks`)
@@ -255,8 +308,9 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     `base_pos[b] + s` and sees every cached position up to its own. `ctx_blocks` bounds the
     gather (a host value, at least every lane's block count). fp32 math, q's dtype out. bf16
     device tensors with 16-row blocks and head_dim 64/128/256 go to the HIP kernel
-    (`attention.paged_attention`: bf16 MFMA, bf16 probabilities, fp32 softmax)."""
-    if attention.supported(q, block_size):
+    (`attention.paged_attention`: bf16 MFMA, bf16 probabilities, fp32 softmax). With `parents` `[B, t]` the rows are a tree's
+    nodes (`attention.paged_attention_tree`, which is the device form): row s sees the context and its ancestors' rows."""
+    if parents is None and attention.supported(q, block_size):
         return attention.paged_attention(q, k_pool, v_pool, block_table, base_pos, ctx_blocks * block_size,
                                          scale)
     b, heads, t, hd = q.shape
@@ -271,9 +325,17 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     qg = q.float().reshape(b, kvh, group * t, hd)
     scores = torch.matmul(qg, keys) * scale  # [B, kvh, group*t, S]
     qpos = base_pos.long()[:, None] + torch.arange(t, device=q.device)[None, :]  # [B, t]
-    live = torch.arange(s_len, device=q.device)[None, None, :] <= qpos[:, :, None]  # [B, t, S]
+    at = torch.arange(s_len, device=q.device)[None, None, :]
+    live = at <= qpos[:, :, None]  # [B, t, S]
+    if parents is not None:
+        above = tree_ancestors(parents)
+        node = at - base_pos.long()[:, None, None]
+        live = above.gather(2, node.clamp(0, t - 1).expand(b, t, s_len)) & (node < t)
+        live = torch.where(node < 0, above.any(2, keepdim=True), live)
     live = live[:, None, None].expand(b, 1, group, t, s_len).reshape(b, 1, group * t, s_len)
     probs = scores.masked_fill(~live, float("-inf")).softmax(-1)
+    if parents is not None:  # absent nodes' rows
+        probs = probs.masked_fill(~live.any(-1, keepdim=True), 0.0)
     out = torch.matmul(probs, vals)  # [B, kvh, group*t, hd]
     return out.reshape(b, heads, t, hd).to(q.dtype)
 
@@ -312,7 +374,7 @@ def split_kv(kv: torch.Tensor, kv_heads: int, head_dim: int) -> tuple[torch.Tens
 def gated_attention(model: "Model", w: dict, pool: dict, h: torch.Tensor, base_pos: torch.Tensor,
                     write_rows: torch.Tensor, block_table: torch.Tensor, ctx_blocks: int,
                     keep: torch.Tensor | None = None,
-                    positions: torch.Tensor | None = None) -> torch.Tensor:
+                    positions: torch.Tensor | None = None, parents: torch.Tensor | None = None) -> torch.Tensor:
     """Gated GQA attention of `t` rows per lane (`h` `[B, t, hidden]`, normed): q/gate
     projection, q/k RMSNorm, partial RoPE at `base_pos + s`, this round's K/V written at
     `write_rows` `[B, t]` of `pool`, causal paged attention, `o_proj(out * sigmoid(gate))`
@@ -322,7 +384,8 @@ def gated_attention(model: "Model", w: dict, pool: dict, h: torch.Tensor, base_p
     `[B, t]` bool (optional) masks the K/V writes: rows with False write nothing (on the torch
     path they write into row 0, which lies in the reserved block 0 that no lane owns).
     `positions` `[B, t]` (optional) is `base_pos[:, None] + arange(t)` precomputed. A layer with
-    `qkv_proj` (`fuse_qkv`) projects q, gate, k and v with one GEMM."""
+    `qkv_proj` (`fuse_qkv`) projects q, gate, k and v with one GEMM. `parents` `[B, t]`: the rows are the nodes of a tree
+    (`attention.paged_attention_tree`), `positions` their own (`base_pos + depth`); they are written side by side all the same."""
     c = model.cfg
     b, t, _ = h.shape
     if "qkv_proj" in w:
@@ -359,11 +422,14 @@ def gated_attention(model: "Model", w: dict, pool: dict, h: torch.Tensor, base_p
         attention.write_v(pool["v"], rows, v.reshape(-1, c.kv_heads, c.head_dim))
     if attention.supported(q, c.block_size):
         # q read in its [B, t, heads, hd] layout, the sigmoid gate applied in the epilogue
-        out = attention.paged_attention_gated(q, pool["k"], pool["v"], block_table, base_pos,
-                                              ctx_blocks * c.block_size, c.head_dim ** -0.5, gate)
+        args = (q, pool["k"], pool["v"], block_table, base_pos, ctx_blocks * c.block_size, c.head_dim ** -0.5)
+        if parents is not None:
+            out = attention.paged_attention_tree(*args, parents, gate=gate)
+        else:
+            out = attention.paged_attention_gated(*args, gate)
         return linear(out.reshape(b, t, -1), w["o_proj"])
     out = paged_attention(q.transpose(1, 2), pool["k"], pool["v"], block_table, base_pos, ctx_blocks,
-                          c.block_size, c.head_dim ** -0.5)
+                          c.block_size, c.head_dim ** -0.5, parents)
     out = out.transpose(1, 2).reshape(b, t, -1)
     return F.linear(out * torch.sigmoid(gate.reshape(b, t, -1)), w["o_proj"])
 
@@ -842,12 +908,12 @@ class Model:
 
     def attention_rows(self, w: dict, pool: dict, h: torch.Tensor, lanes: torch.Tensor,
                        base_pos: torch.Tensor, ctx_len: int, block_table: torch.Tensor | None = None,
-                       keep: torch.Tensor | None = None,
-                       positions: torch.Tensor | None = None) -> torch.Tensor:
+                       keep: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                       parents: torch.Tensor | None = None) -> torch.Tensor:
         """Gated GQA attention for `t` rows per lane at positions `base_pos + s` (`attn_verify`,
         `model.py:3519-3577`) over `block_table` `[B, blocks]` (default: the lanes' own tables),
         K/V writes masked by `keep` `[B, t]`. `ctx_len` is a host bound on `base_pos + t`;
-        `positions` (optional) the `[B, t]` positions precomputed."""
+        `positions` (optional) the `[B, t]` positions precomputed; `parents` as in `gated_attention`."""
         c = self.cfg
         t = h.shape[1]
         table = self.blocks.table[lanes] if block_table is None else block_table
@@ -856,12 +922,13 @@ class Model:
             pos = base_pos.long()[:, None] + torch.arange(t, device=h.device)[None, :]
             rows = table_rows(table, pos, c.block_size)
         ctx_blocks = (ctx_len + c.block_size - 1) // c.block_size
-        return gated_attention(self, w, pool, h, base_pos, rows, table, ctx_blocks, keep, positions)
+        return gated_attention(self, w, pool, h, base_pos, rows, table, ctx_blocks, keep, positions, parents)
 
-    def deltanet_verify(self, w: dict, pool: dict, h: torch.Tensor,
-                        lanes: torch.Tensor) -> tuple[torch.Tensor, DeltaNetRows]:
+    def deltanet_verify(self, w: dict, pool: dict, h: torch.Tensor, lanes: torch.Tensor,
+                        parents: torch.Tensor | None = None) -> tuple[torch.Tensor, DeltaNetRows]:
         """Gated DeltaNet over `t` rows per lane from the committed state, which is read and
-        not written (`deltanet_verify`, `model.py:3738-3905`)."""
+        not written (`deltanet_verify`, `model.py:3738-3905`). With `parents` `[B, t]` the rows are a tree's nodes, each
+        of which follows its own ancestors (`deltanet.prep_tree`, `deltanet.delta_rule_tree`)."""
         c = self.cfg
         b, t, _ = h.shape
         proj = F.linear(h, w["in_proj_all"])
@@ -869,14 +936,22 @@ class Model:
         raw = qkv.transpose(1, 2)  # [B, C, t]
         if h.device.type == "cuda":
             # conv, SiLU, split, q/k norms, g and beta in one launch; then the recurrence
-            q, k, v, g, beta = deltanet.prep(proj, pool["conv"], lanes, w["conv"], w["A_log"],
-                                             w["dt_bias"], c.k_heads, c.k_dim, c.v_heads, c.v_dim)
-            out = deltanet.delta_rule(pool["rec"], lanes, q, k, v, g, beta)  # [B, t, vh, vd] fp32
+            args = (proj, pool["conv"], lanes, w["conv"], w["A_log"], w["dt_bias"], c.k_heads, c.k_dim, c.v_heads, c.v_dim)
+            if parents is not None:
+                q, k, v, g, beta = deltanet.prep_tree(*args, parents)
+                out = deltanet.delta_rule_tree(pool["rec"], lanes, q, k, v, g, beta, parents)
+            else:
+                q, k, v, g, beta = deltanet.prep(*args)
+                out = deltanet.delta_rule(pool["rec"], lanes, q, k, v, g, beta)  # [B, t, vh, vd] fp32
             normed = gated_rmsnorm(out, z.reshape(b, t, c.v_heads, c.v_dim), w["dn_norm"], c.eps, h.dtype)
             mixer = linear(normed.reshape(b, t, -1), w["out_proj"])
             return mixer, DeltaNetRows(raw, q, k, v, g, beta, proj)
-        window = torch.cat([pool["conv"][lanes], raw], dim=-1)
-        mixed = causal_conv_rows(window, w["conv"], t).to(h.dtype).transpose(1, 2)  # [B, t, C]
+        if parents is None:
+            window = torch.cat([pool["conv"][lanes], raw], dim=-1)
+            mixed = causal_conv_rows(window, w["conv"], t).to(h.dtype).transpose(1, 2)  # [B, t, C]
+        else:
+            windows = tree_windows(pool["conv"][lanes], raw, parents)  # [B, t, C, conv_k]
+            mixed = causal_conv_rows(windows.flatten(0, 1), w["conv"], 1)[..., 0].to(h.dtype).view(b, t, -1)
         kd = c.k_heads * c.k_dim
         q = mixed[..., :kd].reshape(b, t, c.k_heads, c.k_dim).float()
         k = mixed[..., kd : 2 * kd].reshape(b, t, c.k_heads, c.k_dim).float()
@@ -889,10 +964,17 @@ class Model:
         qe, ke = q.repeat_interleave(rep, dim=2), k.repeat_interleave(rep, dim=2)
         state = pool["rec"][lanes]
         outs = []
+        after = [state]  # a tree's states: the stored one, then after each node
         for s in range(t):
+            if parents is not None:  # the state after the node's parent
+                state = torch.stack(after, 1)[torch.arange(b), parents[:, s].long().clamp(-1, s - 1) + 1]
             state, o = delta_rule_step(state, qe[:, s], ke[:, s], v[:, s], g[:, s], beta[:, s])
             outs.append(o)
+            after.append(state)
         out = torch.stack(outs, dim=1)  # [B, t, vh, vd] fp32
+        if parents is not None:
+            present = tree_ancestors(parents).any(2)
+            out = out * present[..., None, None]
         normed = gated_rmsnorm(out, z.reshape(b, t, c.v_heads, c.v_dim), w["dn_norm"], c.eps, h.dtype)
         mixer = F.linear(normed.reshape(b, t, -1), w["out_proj"])
         return mixer, DeltaNetRows(raw.contiguous(), q, k, v, g, beta)
@@ -940,13 +1022,38 @@ class Model:
         pool["conv"][lanes[sel]] = conv[sel]
         pool["rec"][lanes[sel]] = state[sel]
 
+    def commit_path(self, res: "VerifyOut", lanes, base_pos: torch.Tensor, path: torch.Tensor, lengths: torch.Tensor, *,
+                    block_table: torch.Tensor | None = None, active: torch.Tensor | None = None) -> None:
+        """`commit` after a tree's forward (`forward_rows(parents=)`): the accepted path's cache rows move together in every
+        attention layer (`attention.keep_path`), and every DeltaNet layer's state advances along it (`deltanet.commit_path`).
+        `path` int64 `[B, t]` and `lengths` `[B]` from `graph_mtp.tree_accept`; rows with `active` False touch nothing."""
+        c = self.cfg
+        lanes = self.lane_index(lanes)
+        table = self.blocks.table[lanes] if block_table is None else block_table
+        kept = lengths if active is None else torch.where(active, lengths, torch.zeros_like(lengths))
+        pools = [p[name] for ty, p in zip(c.layer_types, self.pool) if ty == ATTN for name in ("k", "v")]
+        if pools:
+            attention.keep_path(pools, table, base_pos.to(self.device, torch.long), path, kept)
+        for i, rows in res.dn_rows.items():
+            pool = self.pool[i]
+            if self.device.type == "cuda" and rows.proj is not None:
+                slots = lanes if active is None else torch.where(active, lanes, torch.full_like(lanes, -1))
+                deltanet.commit_path(pool["rec"], pool["conv"], slots, rows.k, rows.v, rows.g, rows.beta, path, kept,
+                                     rows.proj, c.conv_dim)
+                continue
+            on = path.long()  # the path's rows in order, then the chain's commit
+            take = lambda x: x.gather(1, on.view(*on.shape, *[1] * (x.dim() - 2)).expand_as(x))  # noqa: E731, B023
+            chain = DeltaNetRows(rows.raw_qkv.gather(2, on[:, None].expand_as(rows.raw_qkv)), take(rows.q), take(rows.k),
+                                 take(rows.v), take(rows.g), take(rows.beta))
+            self.deltanet_commit(pool, chain, lanes, lengths, None, active)
+
     # ------------------------------------------------------------ forward
 
     def forward_rows(self, ids: torch.Tensor, lanes, base_pos: torch.Tensor, ctx_len: int, *,
                      block_table: torch.Tensor | None = None,
                      active: torch.Tensor | None = None,
                      positions: torch.Tensor | None = None,
-                     final_norm: bool = False) -> VerifyOut:
+                     final_norm: bool = False, parents: torch.Tensor | None = None) -> VerifyOut:
         """The wide forward over fed tokens `ids` `[B, t]` at positions `base_pos[b] + s`
         (`verify_and_commit`'s layer loop, `mtp.py:767-772`). Writes the rows' K/V; DeltaNet
         state is left for `commit`. `ctx_len` is a host bound on `max(base_pos) + t`.
@@ -956,10 +1063,22 @@ class Model:
         (padding) read their slot's state but write no K/V. `positions` (optional) is
         `base_pos[:, None] + arange(t)` precomputed (a round buffer's `pos_grid`). With
         `final_norm`, `res.normed` also holds the final-normed rows (the last residual add and
-        the norm in one launch)."""
+        the norm in one launch).
+
+        `parents` int32 or int64 `[B, t]`: `ids` are the nodes of a tree of drafts per lane
+        (`attention.paged_attention_tree`), node 0 the lane's own token. Node s is rotated at `base_pos[b]` plus its depth, its
+        K/V row lies at `base_pos[b] + s`, and `commit_path` takes the accepted ones from there. Absent nodes' rows are of no use."""
         c = self.cfg
         lanes = self.lane_index(lanes)
         base_pos = base_pos.to(self.device, torch.long)
+        if parents is not None:
+            parents = parents.to(self.device)
+            if parents.shape != ids.shape or not 1 <= ids.shape[1] <= 64:
+                raise ValueError(f"parents must be {tuple(ids.shape)} of 1 to 64 nodes, got {tuple(parents.shape)}")
+            if parents.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f"parents must be int32 or int64, got {parents.dtype}")
+            if positions is None:
+                positions = base_pos[:, None] + tree_depths(parents)
         keep = None if active is None else active[:, None].expand(ids.shape[0], ids.shape[1])
         x = self.embed[ids.to(self.device)]
         res = VerifyOut(x)
@@ -969,9 +1088,9 @@ class Model:
             w, pool = self.layers[i], self.pool[i]
             if ty == ATTN:
                 mixer = self.attention_rows(w, pool, h, lanes, base_pos, ctx_len, block_table, keep,
-                                            positions)
+                                            positions, parents)
             else:
-                mixer, rows = self.deltanet_verify(w, pool, h, lanes)
+                mixer, rows = self.deltanet_verify(w, pool, h, lanes, parents)
                 res.dn_rows[i] = rows
             x, hm = add_rmsnorm(x, mixer, w["post_norm"], c.eps)
             # the MoE output joins the residual stream in front of the next norm (the next
