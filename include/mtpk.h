@@ -717,7 +717,7 @@ int mtpk_copy_blocks(void* const* pools, const int64_t* block_bytes, int n_pools
  * fp32, probabilities bf16, the output (times sigmoid(gate) when gate is given) rounded once. What a node does not see may
  * hold anything. n_split from mtpk_attention_tree_splits (0: a shape that is not taken; max_ctx a bound on base_pos + t), at
  * most 64; n_split > 1 needs mtpk_attention_tree_workspace_bytes of workspace (16-byte aligned). Limits as
- * mtpk_paged_attention_masked's. */
+ * mtpk_paged_attention_masked's, and heads <= 65535. */
 int mtpk_attention_tree_splits(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_ctx);
 int64_t mtpk_attention_tree_workspace_bytes(int64_t batch, int64_t t, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                             int n_split);
@@ -730,7 +730,8 @@ int mtpk_paged_attention_tree(const uint16_t* q, const int64_t* q_strides, const
 
 /* mtpk_deltanet_prep for a tree's rows: the convolution's columns before a node are its ancestors', then the stored
  * window's. Same operands and outputs; k_dim, v_dim <= 256, conv_k 2..9. bf16 rows' convolution is rounded to bf16 as its
- * exact value is, next to a border too (mtpk_deltanet_prep: as its fp32 value is). A slot outside the pool reads a zero window. */
+ * exact value is, next to a border too (mtpk_deltanet_prep: as its fp32 value is). A slot outside the pool reads a zero window.
+ * proj_stride < 2^23 elements. */
 int mtpk_deltanet_prep_tree(const void* proj, int dtype, int64_t proj_stride, const void* conv_state, const int64_t* slot,
                             int64_t slots_total, const void* conv_w, const float* a_log, const float* dt_bias, const void* parents,
                             int parents_dtype, const int64_t* parents_strides, int64_t batch, int64_t t, int64_t k_heads,
@@ -770,7 +771,8 @@ int mtpk_tree_accept(const int64_t* step_argmax, int64_t sa_stride, const int64_
 
 /* The accepted rows together: cache row base_pos[b] + path[b * t + i] becomes row base_pos[b] + i, for i < lengths[b],
  * in each of n_pools pools (host arrays: addresses, 16-byte aligned; channels = kv_heads * head_dim; element bytes, 2 or 4;
- * transposed 0: a K pool [n_blocks * 16, channels], its rows a multiple of 16 bytes, 1: a V pool [n_blocks, channels, 16]).
+ * transposed 0: a K pool [n_blocks * 16, channels], its rows a multiple of 16 bytes, 1: a V pool [n_blocks, channels, 16];
+ * no two of them share memory). The blocks that a lane's rows from base_pos[b] on lie in are its own, no other lane's of the call.
  * A path rises (int64 [batch, t], t <= 64); an entry outside [0, t) ends it, and a row whose position lies outside the
  * lane's table or whose block lies outside the pools is left. */
 int mtpk_keep_path(void* const* pools, const int64_t* channels, const int* element_bytes, const int* transposed, int n_pools,

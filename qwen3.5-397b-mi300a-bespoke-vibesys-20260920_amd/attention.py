@@ -303,6 +303,7 @@ def keep_path(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: to
 
     `path` int32 or int64 `[B, t]`, t up to 64, rises in its first `lengths[b]` entries (`graph_mtp.tree_accept`); an entry
     that is no node of `[0, t)` ends it. Rows outside the lane's table, and blocks outside the pools, are left.
+    No two pools share memory, and the blocks of a lane's rows from `base_pos[b]` on are no other lane's of the call.
     CPU pools take the torch spelling."""
     if pools and not pools[0].is_cuda:
         _keep_path_torch(pools, block_table, base_pos, path, lengths)
@@ -315,6 +316,9 @@ def keep_path(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: to
 def _keep_path_torch(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: torch.Tensor, path: torch.Tensor,
                      lengths: torch.Tensor) -> None:
     n_blocks = _pool_blocks(pools, BLOCK)
+    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in pools)
+    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+        raise ValueError("pools must not share memory")
     if path.dim() != 2 or not 1 <= path.shape[1] <= 64:
         raise ValueError(f"path must be [B, 1 to 64], got {tuple(path.shape)}")
     b, t = path.shape

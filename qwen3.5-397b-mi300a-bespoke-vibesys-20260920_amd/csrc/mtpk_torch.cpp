@@ -570,7 +570,7 @@ void keep_path(const std::vector<Tensor>& pools, const Tensor& block_table, cons
   check(lib.keep_path(at.data(), channels.data(), size.data(), transposed.data(), (int)pools.size(), n, table.data_ptr<int32_t>(),
                       table.size(1), base.data_ptr<int64_t>(), path.data_ptr<int64_t>(), lengths.data_ptr<int64_t>(), b, t,
                       (void*)stream),
-        "mtpk_keep_path (elements of 2 or 4 bytes, K rows of a multiple of 16 bytes, pools on 16 bytes)");
+        "mtpk_keep_path (elements of 2 or 4 bytes, K rows of a multiple of 16 bytes, pools on 16 bytes, no two of one memory)");
 }
 
 template <typename F>

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(TreeAcceptArgs a) {
   for (int i = 0; i < a.n_stops; ++i) stop |= node && a.stops[(int64_t)b * a.n_stops + i] == best;
   const uint64_t stops = __ballot(stop);
   int at = 0, n = 0, mine = 0;
-  while (n < budget - 1 && !(stops >> at & 1ull)) {
+  while (n + 1 < budget && !(stops >> at & 1ull)) {
     const uint64_t fits = __ballot(parent == at && token == lane_value(best, at));  // a parent comes before its children
     if (fits == 0ull) break;
     at = __builtin_ctzll(fits);
@@ -177,6 +177,12 @@ int mtpk_keep_path(void* const* pools, const int64_t* channels, const int* eleme
     if (!pools[i] || !aligned16(pools[i]) || channels[i] < 1 || channels[i] > (1 << 20)) return MTPK_EINVAL;
     if (element_bytes[i] != 2 && element_bytes[i] != 4) return MTPK_EINVAL;
     if (!transposed[i] && channels[i] * element_bytes[i] % 16) return MTPK_EINVAL;
+    // no two may share memory: each moves its rows in an order of its own
+    const uintptr_t at = reinterpret_cast<uintptr_t>(pools[i]), bytes = (uintptr_t)(n_blocks * kKeepBlock * channels[i] * element_bytes[i]);
+    for (int j = 0; j < i; ++j) {
+      const uintptr_t other = reinterpret_cast<uintptr_t>(pools[j]);
+      if (at < other + (uintptr_t)(n_blocks * kKeepBlock * channels[j] * element_bytes[j]) && other < at + bytes) return MTPK_EINVAL;
+    }
   }
   if (batch == 0 || t == 1) return 0;  // a path of one node is where it belongs
   if (!block_table || !base_pos || !path || !lengths) return MTPK_EINVAL;

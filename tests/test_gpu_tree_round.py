@@ -147,3 +147,20 @@ def test_in_a_graph(dev) -> None:
         want = step(eager)
         assert all(torch.equal(getattr(got, n), getattr(want, n)) for n in got.__dataclass_fields__)
         assert all(torch.equal(x, y) for x, y in zip(mine, eager))
+
+
+def test_pools_that_share_memory_are_refused(dev) -> None:
+    rows, table, b0, path, lengths = keep_case(1, 2, 8, 2, 64, [3, 9], torch.bfloat16)
+    k, v = pools_of(rows, dev)
+    args = (table.to(dev), b0.to(dev), path.to(dev), lengths.to(dev))
+    for pools in ([k, v, k], [k, k.view(-1, 2, 64, 16)]):
+        with pytest.raises(ValueError, match="no two of one memory"):
+            attention.keep_path(pools, *args)
+    assert torch.equal(k.cpu(), rows[0])
+
+
+def test_the_lowest_budget_accepts_nothing(dev) -> None:
+    best, tokens, tree, active, pos, budget, stops = (x.to(dev) for x in accept_case(5, 9, 2, words=1))
+    budget[:] = -(2**63) + 70
+    got = graph_mtp.tree_accept(best, tokens, tree, active, pos, budget, stops)
+    assert got.accept_len.tolist() == [0] * 5 and not got.live.any()
