@@ -400,7 +400,7 @@ def verify_tree(model, lanes, tokens: torch.Tensor, parents: torch.Tensor, pos: 
     rows, the DeltaNet states (`Model.commit_path`), the MTP cache and the hidden seed. The slots are then where the accepted
     tokens, one after another, would have left them; `bonus` is each lane's next token, at `next_pos`.
 
-    `tokens` int64 `[B, t]`, t up to 64, node 0 the lane's last committed token at `pos` `[B]`; `parents` `[B, t]` as in
+    `lanes` distinct; `tokens` int64 `[B, t]`, t up to 64, node 0 the lane's last committed token at `pos` `[B]`; `parents` `[B, t]` as in
     `attention.paged_attention_tree`; `budget`, `stops` as in `tree_accept`; `ctx_len` a host bound on `max(pos) + t`. The lanes'
     blocks must hold `pos + t` positions (`BlockTables.grow_many`). `mtp` defaults to the model's attached head. Rows with
     `active` False touch no lane state. No host read: the call can be captured."""
@@ -414,7 +414,7 @@ def verify_tree(model, lanes, tokens: torch.Tensor, parents: torch.Tensor, pos: 
     out = tree_accept(best, tokens, parents, act, pos, budget, stops)
     model.commit_path(res, lanes, pos, out.path, out.lengths, block_table=table, active=act)
     at = torch.arange(b, device=tokens.device)[:, None]
-    hidden, ids = res.hidden[at, out.path], tokens[at, out.path]
+    hidden, ids = res.hidden[at, out.path], tokens[at, out.path].clamp(0, model.cfg.vocab - 1)  # an inactive lane's may be anything
     if m is not None:
         grid = pos[:, None] + torch.arange(t, device=tokens.device)
         previous = torch.cat([model.hidden_cache[lanes][:, None], hidden[:, :-1]], dim=1)

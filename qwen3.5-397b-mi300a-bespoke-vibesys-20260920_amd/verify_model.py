@@ -1067,7 +1067,8 @@ class Model:
 
         `parents` int32 or int64 `[B, t]`: `ids` are the nodes of a tree of drafts per lane
         (`attention.paged_attention_tree`), node 0 the lane's own token. Node s is rotated at `base_pos[b]` plus its depth, its
-        K/V row lies at `base_pos[b] + s`, and `commit_path` takes the accepted ones from there. Absent nodes' rows are of no use."""
+        K/V row lies at `base_pos[b] + s`, and `commit_path` takes the accepted ones from there. Absent nodes' ids may be anything,
+        their rows are of no use."""
         c = self.cfg
         lanes = self.lane_index(lanes)
         base_pos = base_pos.to(self.device, torch.long)
@@ -1079,6 +1080,7 @@ class Model:
                 raise ValueError(f"parents must be int32 or int64, got {parents.dtype}")
             if positions is None:
                 positions = base_pos[:, None] + tree_depths(parents)
+            ids = ids.clamp(0, c.vocab - 1)  # absent nodes' ids
         keep = None if active is None else active[:, None].expand(ids.shape[0], ids.shape[1])
         x = self.embed[ids.to(self.device)]
         res = VerifyOut(x)

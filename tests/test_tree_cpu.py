@@ -113,6 +113,32 @@ def test_inactive_rows_touch_nothing() -> None:
     assert all(torch.equal(x, y) for x, y in zip(before, mh.slot_state(model, 1, 16), strict=True))
 
 
+@pytest.mark.parametrize("pad,like", [(-100, 0), (2**40, vm.tiny_cfg().vocab - 1)])
+def test_padded_trees_may_hold_any_ids(pad, like) -> None:
+    """Trees of different sizes in one batch: absent nodes and an inactive lane may hold ids that are no ids. They count as the
+    nearest id, so the batch is the same to the last bit (another id there changes which rows an expert's product sums together)."""
+    outs, states = [], []
+    for fill in (pad, like):
+        model = mh.build(lanes=3)
+        for lane, p in enumerate(mh.prompts(3)):
+            model.prefill(lane, p)
+        tokens = mh.prompts(3, 6, seed=4)
+        tokens[0][4:], tokens[2][:] = [fill] * 2, [fill] * 6
+        parents = [[-1, 0, 0, 1, -2, 4], [-1, 0, 1, 1, 0, 4], [-1, 0, 1, 2, 3, 4]]
+        out = tree_round.run(model, [0, 1, 2], tokens, parents, [16] * 3, 22, active=[True, True, False])
+        outs.append([out.path[:2], out.accept_len[:2], out.bonus[:2]])
+        states.append([x for j in range(3) for x in mh.slot_state(model, j, 16 + (int(out.lengths[j]) if j < 2 else 0))])
+    for x, y in zip(outs[0] + states[0], outs[1] + states[1], strict=True):
+        assert torch.equal(x, y)
+
+
+def test_a_budget_of_the_lowest_value_accepts_nothing() -> None:
+    b = torch.tensor([[1, 2]])
+    got = graph_mtp.tree_accept(b, torch.tensor([[0, 1]]), torch.tensor([[-1, 0]]), torch.tensor([True]), torch.tensor([3]),
+                                torch.tensor([-(2**63) + 9]), torch.full((1, 1), -1))
+    assert got.accept_len.tolist() == [0] and got.live.tolist() == [False]
+
+
 def test_the_model_refuses_trees_of_other_sizes() -> None:
     model = mh.build()
     with pytest.raises(ValueError, match="parents must be"):
@@ -129,7 +155,8 @@ def test_kept_rows_refusals() -> None:
     path, n = torch.zeros(1, 4, dtype=torch.long), torch.ones(1, dtype=torch.long)
     for bad in (([], table, base, path, n), ([k], table, base, path[0], n), ([k], table, base, torch.zeros(1, 65, dtype=torch.long), n),
                 ([k], table, base, path.float(), n), ([k], table, base, path, n.repeat(2)), ([k[:31]], table, base, path, n),
-                ([k, torch.zeros(3, 2, 8, 16)], table, base, path, n)):
+                ([k, torch.zeros(3, 2, 8, 16)], table, base, path, n), ([k, k], table, base, path, n),
+                ([k, k.view(2, 2, 8, 16)], table, base, path, n)):
         with pytest.raises(ValueError):
             attention.keep_path(*bad)
 
