@@ -530,10 +530,10 @@ std::vector<Tensor> tree_accept(const Tensor& argmax_in, const Tensor& tokens_in
   const Tensor best = argmax_in.stride(1) == 1 ? argmax_in : argmax_in.contiguous(),
                tokens = tokens_in.stride(1) == 1 ? tokens_in : tokens_in.contiguous();
   const Tensor active = active_in.contiguous(), pos = pos_in.contiguous(), budget = budget_in.contiguous(), stops = stops_in.contiguous();
-  const auto i64 = best.options(), flags = best.options().dtype(at::kBool);
-  const Tensor path = at::empty({b, t}, i64), keep = at::empty({b, t}, flags), live = at::empty({b}, flags);
-  std::vector<Tensor> n;  // accept_len, lengths, bonus, next_pos, budget_left, hidden_src
-  for (int i = 0; i < 6; ++i) n.push_back(at::empty({b}, i64));
+  // the outputs lie in two allocations: the call takes 7.8 us of the host, with nine 9.5
+  const std::vector<Tensor> n = at::empty({b * (t + 6)}, best.options()).unsafe_split_with_sizes({b, b, b, b, b, b, b * t});
+  const std::vector<Tensor> flags = at::empty({b * (t + 1)}, best.options().dtype(at::kBool)).unsafe_split_with_sizes({b, b * t});
+  const Tensor path = n[6].view({b, t}), keep = flags[1].view({b, t}), live = flags[0];
   auto at64 = [](const Tensor& x) { return x.data_ptr<int64_t>(); };
   check(lib.tree_accept(at64(best), best.stride(0), at64(tokens), tokens.stride(0), tree.p, tree.dtype, tree.s,
                         (const uint8_t*)active.data_ptr(), at64(pos), at64(budget), at64(stops), stops.size(1), b, t, at64(path),

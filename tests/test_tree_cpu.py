@@ -3,9 +3,12 @@ and the refusals that need no device."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
+import _mtpk
 import attention
 import deltanet
 import graph_mtp
@@ -174,3 +177,96 @@ def test_device_operators_refuse_cpu_tensors() -> None:
     with pytest.raises(ValueError):
         deltanet.commit_path(state, f(1, 256, 3), base, f(1, 2, 1, 64), f(1, 2, 2, 64), f(1, 2, 2), f(1, 2, 2), tree.long(), base,
                              f(1, 2, 260), 256)
+
+
+# ---------------------------------------------------------------- the C entry points: refused before anything is launched
+
+P = 1 << 20  # an address that no refused call follows
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _mtpk.LIB_PATH.exists():
+        import __graft_entry__
+
+        __graft_entry__.build()
+    return _mtpk.lib()
+
+
+def array(kind, values) -> tuple:
+    held = (kind * len(values))(*values)
+    return ctypes.addressof(held), held
+
+
+def refuse(entry, good: dict, bad: list[dict]) -> None:
+    for change in bad:
+        assert change.keys() <= good.keys()
+        assert entry(*{**good, **change}.values(), None) == _mtpk.EINVAL, change
+
+
+PAIR, PAIR_HELD = array(ctypes.c_int64, (4, 1))
+QS, QS_HELD = array(ctypes.c_int64, (1024, 64, 256))
+
+
+def test_attention_entry_refuses(lib) -> None:
+    good = {"q": P, "qs": QS, "gate": None, "gs": QS, "b": 2, "t": 4, "heads": 4, "kvh": 2, "hd": 64, "k": P, "v": P, "rows": 160, "table": P,
+            "stride": 5, "base": P, "scale": 0.1, "parents": P, "pdt": _mtpk.I32, "ps": PAIR, "n": 1, "ws": None, "wsb": 0, "out": P, "os": QS}
+    refuse(lib.mtpk_paged_attention_tree, good, [
+        *({n: None} for n in ("q", "qs", "k", "v", "table", "base", "parents", "ps", "out", "os")), {"gate": P, "gs": None}, {"t": 0}, {"t": 65},
+        {"pdt": _mtpk.BF16}, {"b": -1}, {"heads": 3}, {"heads": 0}, {"kvh": 0}, {"hd": 96}, {"rows": 150}, {"rows": 0}, {"stride": 0}, {"scale": 0.0},
+        {"scale": float("nan")}, {"n": 0}, {"n": 65}, {"n": 2}, {"heads": 65536, "kvh": 1}, {"q": P + 2},
+    ])  # fmt: skip
+    assert lib.mtpk_attention_tree_splits(2, 65, 8, 2, 64, 100) == 0
+    assert lib.mtpk_attention_tree_splits(2, 4, 8, 2, 64, 0) == 1
+    assert lib.mtpk_attention_tree_workspace_bytes(2, 65, 8, 2, 64, 4) == 0
+
+
+def test_delta_net_entries_refuse(lib) -> None:
+    good = {"proj": P, "dt": _mtpk.BF16, "stride": 200, "conv": P, "slot": P, "slots": 3, "w": P, "a_log": P, "bias": P, "parents": P,
+            "pdt": _mtpk.I64, "ps": PAIR, "b": 2, "t": 4, "kh": 1, "kd": 16, "vh": 2, "vd": 16, "taps": 4, "eps": 1e-6, "scale": 0.25, "q": P,
+            "k": P, "v": P, "g": P, "beta": P}
+    refuse(lib.mtpk_deltanet_prep_tree, good, [
+        *({n: None} for n in ("proj", "conv", "slot", "w", "a_log", "bias", "parents", "ps", "q", "k", "v", "g", "beta")), {"dt": _mtpk.I32},
+        {"pdt": _mtpk.F32}, {"t": 0}, {"t": 65}, {"b": -1}, {"b": 1 << 31}, {"kd": 257}, {"kd": 0}, {"vd": 300}, {"kh": 0}, {"vh": 65536}, {"taps": 1},
+        {"taps": 10}, {"slots": 0}, {"stride": 99}, {"stride": 1 << 23},
+    ])  # fmt: skip
+    good = {"state": P, "slots": 3, "slot": P, "rows": 2, "t": 4, "heads": 4, "qk": 2, "kd": 16, "vd": 8, "q": P, "k": P, "v": P, "g": P, "beta": P,
+            "parents": P, "pdt": _mtpk.I32, "ps": PAIR, "out": P}
+    shapes = [{"t": 0}, {"t": 65}, {"rows": -1}, {"heads": 3}, {"heads": 0}, {"qk": 0}, {"kd": 48}, {"vd": 0}, {"vd": 4097}, {"slots": 0},
+              {"slots": 1 << 40}, {"rows": 1 << 40}]
+    refuse(lib.mtpk_delta_rule_tree, good, [
+        *shapes, *({n: None} for n in ("state", "q", "k", "v", "g", "beta", "parents", "ps", "out")), {"pdt": 9}, {"slot": None, "rows": 4},
+    ])  # fmt: skip
+    good = {"state": P, "slots": 3, "slot": P, "rows": 2, "t": 4, "heads": 4, "qk": 2, "kd": 16, "vd": 8, "k": P, "v": P, "g": P, "beta": P,
+            "path": P, "lengths": P, "conv": P, "cdt": _mtpk.F32, "cslots": 3, "proj": P, "stride": 64, "channels": 64, "k1": 3}
+    refuse(lib.mtpk_deltanet_commit_path, good, [
+        *shapes, *({n: None} for n in ("state", "slot", "k", "v", "g", "beta", "path", "lengths", "conv", "proj")), {"cdt": _mtpk.I64}, {"cslots": 0},
+        {"stride": 63}, {"channels": 0}, {"k1": 0}, {"k1": 9},
+    ])  # fmt: skip
+
+
+def test_acceptance_and_move_entries_refuse(lib) -> None:
+    outs = ("path", "n", "lengths", "keep", "bonus", "next", "left", "live", "src")
+    good = {"best": P, "bs": 4, "tokens": P, "ts": 4, "parents": P, "pdt": _mtpk.I32, "ps": PAIR, "active": P, "pos": P, "budget": P, "stops": P,
+            "n_stops": 2, "b": 2, "t": 4, **dict.fromkeys(outs, P)}
+    refuse(lib.mtpk_tree_accept, good, [
+        *({n: None} for n in ("best", "tokens", "parents", "ps", "active", "pos", "budget", "stops", *outs)), {"t": 0}, {"t": 65}, {"b": -1},
+        {"b": 1 << 40}, {"n_stops": -1}, {"pdt": _mtpk.F32},
+    ])  # fmt: skip
+
+    def pools(ps=(P, P + (1 << 20)), channels=(16, 16), size=(2, 2), transposed=(0, 1)) -> tuple[dict, list]:
+        made = {"pools": array(ctypes.c_void_p, ps), "channels": array(ctypes.c_int64, channels), "size": array(ctypes.c_int, size),
+                "transposed": array(ctypes.c_int, transposed)}
+        return {n: x[0] for n, x in made.items()}, [x[1] for x in made.values()]
+
+    first, held = pools()
+    good = {**first, "n": 2, "blocks": 8, "table": P, "stride": 2, "base": P, "path": P, "lengths": P, "b": 2, "t": 4}
+    refuse(lib.mtpk_keep_path, good, [
+        *({n: None} for n in ("pools", "channels", "size", "transposed", "table", "base", "path", "lengths")), {"n": 0}, {"blocks": 0}, {"stride": 0},
+        {"stride": 1 << 27}, {"t": 0}, {"t": 65}, {"b": -1},
+    ])  # fmt: skip
+    for change in ({"ps": (P, P)}, {"ps": (P, P + 4080)}, {"ps": (P + 4080, P)}, {"ps": (P, P + (1 << 20) + 8)}, {"ps": (P, 0)}, {"channels": (4, 16)},
+                   {"channels": (16, 0)}, {"size": (2, 8)}):
+        made, held2 = pools(**change)
+        refuse(lib.mtpk_keep_path, good, [made])
+    assert held and held2
