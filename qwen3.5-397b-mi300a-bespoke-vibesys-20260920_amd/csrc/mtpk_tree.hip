@@ -9,7 +9,7 @@ namespace mtpk {
 // Greedy acceptance. From node 0, the lane's own token, on to the first child whose token is the model's next token
 // after the node, as long as there is one, the node's next token is no stop and the budget lasts. One wave a lane of the
 // round, a node to each of its lanes: a step is one ballot. All latency: the loads of the tree's three rows, the
-// stop ids and the lane's numbers are on their way together.
+// stop ids and the lane's numbers are on their way together (3.1 us alone, 48 lanes of 61 nodes 4.7).
 struct TreeAcceptArgs {
   const int64_t* best;  // [B, t]: the model's next token after each node
   int64_t best_stride;
@@ -69,7 +69,8 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(TreeAcceptArgs a) {
 // The accepted rows together: cache row base + path[i] to base + i for i below the lane's length, in the K and V pools
 // of all layers at once. A path rises, so a row is read before a later one takes its place, and never written before it
 // is read, if each thread moves its share of the rows in order. Of K that is 16 bytes of every row; of V, which lies
-// transposed in its block, one channel's line of the block's positions.
+// transposed in its block, one channel's line of the block's positions. A chain of latencies, base and path, table, rows, store:
+// 30 pools of one lane 3.9 us, of 48 lanes with up to 8 rows 10.6.
 constexpr int kKeepPools = 64;  // pools a launch takes
 constexpr int kKeepAhead = 8;   // rows on their way at once
 constexpr int kKeepBlock = 16;  // rows of a cache block
