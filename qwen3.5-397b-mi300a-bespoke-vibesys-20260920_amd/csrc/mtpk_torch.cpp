@@ -327,6 +327,25 @@ void copy_blocks(const std::vector<Tensor>& pools, const Tensor& src_in, const T
         "mtpk_copy_blocks (blocks of a multiple of 16 bytes, pools on 16 bytes)");
 }
 
+// A call's outputs in one allocation, each from 16 bytes on: an allocation of its own takes the host about 1.1 us.
+std::vector<Tensor> together(const at::TensorOptions& options, std::initializer_list<at::IntArrayRef> shapes) {
+  const int64_t unit = 16 / (int64_t)options.dtype().itemsize();
+  int64_t total = 0;
+  for (const at::IntArrayRef& s : shapes) total += (c10::multiply_integers(s) + unit - 1) / unit * unit;
+  const Tensor all = at::empty({total}, options);
+  const at::AutoDispatchBelowADInplaceOrView plain;  // outputs of a call, not views of a tensor that anyone else holds
+  std::vector<Tensor> out;
+  out.reserve(shapes.size());
+  int64_t at = 0;
+  for (const at::IntArrayRef& s : shapes) {
+    int64_t strides[4], step = 1;
+    for (size_t i = s.size(); i-- > 0; step *= s[i]) strides[i] = step;
+    out.push_back(all.as_strided(s, at::IntArrayRef(strides, s.size()), at));
+    at += (step + unit - 1) / unit * unit;
+  }
+  return out;
+}
+
 // A tree's parents, read where they lie.
 struct Tree {
   const void* p;
@@ -434,15 +453,15 @@ std::vector<Tensor> prep_tree(const Tensor& proj_in, const Tensor& conv_state, c
   const c10::DeviceGuard guard(device);
   const Tensor slots = as_long(slots_in, "slots", {b}, device);
   const Tensor a_log = as_float(a_log_in, "a_log", {v_heads}, device), dt_bias = as_float(dt_bias_in, "dt_bias", {v_heads}, device);
-  const auto f32 = proj.options().dtype(at::kFloat);
-  const Tensor q = at::empty({b, t, k_heads, k_dim}, f32), k = at::empty({b, t, k_heads, k_dim}, f32),
-               v = at::empty({b, t, v_heads, v_dim}, f32), g = at::empty({b, t, v_heads}, f32), beta = at::empty({b, t, v_heads}, f32);
+  const int64_t qk_shape[4] = {b, t, k_heads, k_dim}, v_shape[4] = {b, t, v_heads, v_dim}, g_shape[3] = {b, t, v_heads};
+  const std::vector<Tensor> out = together(proj.options().dtype(at::kFloat), {qk_shape, qk_shape, v_shape, g_shape, g_shape});
+  const Tensor &q = out[0], &k = out[1], &v = out[2], &g = out[3], &beta = out[4];
   check(lib.prep_tree(proj.data_ptr(), float_code(proj), stride, conv_state.data_ptr(), slots.data_ptr<int64_t>(), conv_state.size(0),
                       conv_w.data_ptr(), a_log.data_ptr<float>(), dt_bias.data_ptr<float>(), tree.p, tree.dtype, tree.s, b, t, k_heads,
                       k_dim, v_heads, v_dim, conv_w.size(1), (float)eps, (float)(1.0 / std::sqrt((double)k_dim)), q.data_ptr<float>(),
                       k.data_ptr<float>(), v.data_ptr<float>(), g.data_ptr<float>(), beta.data_ptr<float>(), (void*)stream),
         "mtpk_deltanet_prep_tree");
-  return {q, k, v, g, beta};
+  return out;
 }
 
 // The delta rule's operands of a call's rows: fp32, contiguous.
@@ -530,10 +549,10 @@ std::vector<Tensor> tree_accept(const Tensor& argmax_in, const Tensor& tokens_in
   const Tensor best = argmax_in.stride(1) == 1 ? argmax_in : argmax_in.contiguous(),
                tokens = tokens_in.stride(1) == 1 ? tokens_in : tokens_in.contiguous();
   const Tensor active = active_in.contiguous(), pos = pos_in.contiguous(), budget = budget_in.contiguous(), stops = stops_in.contiguous();
-  // the outputs lie in two allocations: the call takes 7.8 us of the host, with nine 9.5
-  const std::vector<Tensor> n = at::empty({b * (t + 6)}, best.options()).unsafe_split_with_sizes({b, b, b, b, b, b, b * t});
-  const std::vector<Tensor> flags = at::empty({b * (t + 1)}, best.options().dtype(at::kBool)).unsafe_split_with_sizes({b, b * t});
-  const Tensor path = n[6].view({b, t}), keep = flags[1].view({b, t}), live = flags[0];
+  const int64_t lanes[1] = {b}, rows[2] = {b, t};
+  const std::vector<Tensor> n = together(best.options(), {lanes, lanes, lanes, lanes, lanes, lanes, rows});
+  const std::vector<Tensor> flags = together(best.options().dtype(at::kBool), {lanes, rows});
+  const Tensor &path = n[6], &keep = flags[1], &live = flags[0];
   auto at64 = [](const Tensor& x) { return x.data_ptr<int64_t>(); };
   check(lib.tree_accept(at64(best), best.stride(0), at64(tokens), tokens.stride(0), tree.p, tree.dtype, tree.s,
                         (const uint8_t*)active.data_ptr(), at64(pos), at64(budget), at64(stops), stops.size(1), b, t, at64(path),
