@@ -713,7 +713,7 @@ int mtpk_copy_blocks(void* const* pools, const int64_t* block_bytes, int n_pools
  * zeros. No reference counterpart (its drafts are chains).
  *
  * Attention: mtpk_paged_attention_gated's operands. Node s of lane b has its key and value at cache position
- * base_pos[b] + s; it sees every position below base_pos[b], and of the nodes itself and its ancestors. Sums and statistics
+ * base_pos[b] + s (base_pos[b] >= 0); it sees every position below base_pos[b], and of the nodes itself and its ancestors. Sums and statistics
  * fp32, probabilities bf16, the output (times sigmoid(gate) when gate is given) rounded once. What a node does not see may
  * hold anything. n_split from mtpk_attention_tree_splits (0: a shape that is not taken; max_ctx a bound on base_pos + t), at
  * most 64; n_split > 1 needs mtpk_attention_tree_workspace_bytes of workspace (16-byte aligned). Limits as

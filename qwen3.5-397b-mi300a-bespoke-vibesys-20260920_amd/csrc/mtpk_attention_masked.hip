@@ -1467,7 +1467,8 @@ int mtpk_paged_attention_tree(const uint16_t* q, const int64_t* q_strides, const
   if (!masked_operands(a, q, q_strides, gate, gate_strides, batch, t, heads, kv_heads, head_dim, k_pool, v_pool, pool_rows,
                        block_table, table_stride, base_pos, scale, n_split, workspace, workspace_bytes, out, out_strides))
     return MTPK_EINVAL;
-  if (heads > 65535) return MTPK_EINVAL;  // the merge's grid
+  // the merge's grid
+  if (heads > 65535 || (n_split > 1 && batch * t * (n_split <= 8 ? (heads + 3) / 4 : heads) > kMaxGroups)) return MTPK_EINVAL;
   a.tree = {parents, parents_dtype, parents_strides[0], parents_strides[1]};
   const hipStream_t st = (hipStream_t)stream;
   switch (head_dim) {

@@ -215,6 +215,7 @@ def test_attention_entry_refuses(lib) -> None:
         *({n: None} for n in ("q", "qs", "k", "v", "table", "base", "parents", "ps", "out", "os")), {"gate": P, "gs": None}, {"t": 0}, {"t": 65},
         {"pdt": _mtpk.BF16}, {"b": -1}, {"heads": 3}, {"heads": 0}, {"kvh": 0}, {"hd": 96}, {"rows": 150}, {"rows": 0}, {"stride": 0}, {"scale": 0.0},
         {"scale": float("nan")}, {"n": 0}, {"n": 65}, {"n": 2}, {"heads": 65536, "kvh": 1}, {"q": P + 2},
+        *({"b": (1 << 19) - 1, "t": 64, "heads": 1, "kvh": 1, "n": n, "ws": P, "wsb": 1 << 50} for n in (2, 8, 9, 64)),  # the merge's grid
     ])  # fmt: skip
     assert lib.mtpk_attention_tree_splits(2, 65, 8, 2, 64, 100) == 0
     assert lib.mtpk_attention_tree_splits(2, 4, 8, 2, 64, 0) == 1
