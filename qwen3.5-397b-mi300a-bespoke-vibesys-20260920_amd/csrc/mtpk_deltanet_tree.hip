@@ -889,6 +889,7 @@ bool tree_rule_shape(int64_t rows, int64_t t, int64_t heads, int64_t qk_heads, i
 template <int DK, int NT, int W>
 int tree_rule_waves(const TreeRuleArgs& a, int64_t rows, hipStream_t st) {
   const int64_t grid = rows * a.qk_heads * ((a.rep * a.slabs + W - 1) / W);
+  if (grid > 4 * kMaxGroups / W) return MTPK_EINVAL;  // of 64 W threads: fewer than 2^32 in all
   hipLaunchKernelGGL((k_tree_rule<DK, NT, W>), dim3((unsigned)grid), dim3(W * kWave), 0, st, a);
   return status_of(hipGetLastError());
 }
@@ -961,7 +962,7 @@ int mtpk_delta_rule_tree(const float* state, int64_t slots_total, const int64_t*
   const hipStream_t st = (hipStream_t)stream;
   const int rep = (int)(heads / qk_heads);
   const int64_t slabs = (v_dim + kWave - 1) / kWave, grid = rows * heads * slabs;
-  if (grid > 4 * kMaxGroups) return MTPK_EINVAL;
+  if (grid > 4 * kMaxGroups) return MTPK_EINVAL;  // workgroups of one wave, step by step; all at once they are counted again
   if (v_dim % 4 == 0 && aligned16(state) && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out)) {
     const TreeRuleArgs a{state, slots_total, slot, (int)t, (int)heads, (int)qk_heads, rep, (int)v_dim, (int)slabs, q, k, v, g, beta, tree, out};
     switch (k_dim) {
