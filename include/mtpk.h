@@ -758,12 +758,12 @@ int mtpk_deltanet_commit_path(float* state, int64_t slots_total, const int64_t* 
 
 /* Greedy acceptance of a path (mtpk_greedy_accept for a tree): from node 0, the lane's own token, to the lowest child
  * whose token is step_argmax of the node it hangs below, and so on while there is one, that argmax is none of the lane's
- * stop ids and fewer than budget - 1 drafts are accepted. step_argmax, tokens int64 [batch, t] (row strides given, unit
- * column stride); stops int64 [batch, n_stops], -1 padded. Outputs, contiguous: path int64 [batch, t] (node 0, then the
- * accepted ones; the last repeated behind them), accept_len int64 [batch] (accepted drafts), lengths (accept_len + 1, 1
- * on inactive lanes), keep u8 [batch, t] (active and i <= accept_len), bonus (step_argmax of the last accepted node),
- * next_pos = pos + accept_len + 1, budget_left = budget - accept_len - 1, live u8 (bonus is no stop and budget_left > 0),
- * hidden_src = b * t + the last accepted node. */
+ * stop ids and fewer than budget - 1 drafts are accepted. Below an absent node 0 there is nothing to accept.
+ * step_argmax, tokens int64 [batch, t] (row strides given, unit column stride); stops int64 [batch, n_stops], -1 padded.
+ * Outputs, contiguous: path int64 [batch, t] (node 0, then the accepted ones; the last repeated behind them), accept_len
+ * int64 [batch] (accepted drafts), lengths (accept_len + 1, 1 on inactive lanes), keep u8 [batch, t] (active and
+ * i <= accept_len), bonus (step_argmax of the last accepted node), next_pos = pos + accept_len + 1, budget_left = budget -
+ * accept_len - 1, live u8 (bonus is no stop and budget_left > 0), hidden_src = b * t + the last accepted node. */
 int mtpk_tree_accept(const int64_t* step_argmax, int64_t sa_stride, const int64_t* tokens, int64_t tokens_stride,
                      const void* parents, int parents_dtype, const int64_t* parents_strides, const uint8_t* active,
                      const int64_t* pos, const int64_t* budget, const int64_t* stops, int64_t n_stops, int64_t batch, int64_t t,

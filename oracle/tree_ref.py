@@ -117,9 +117,9 @@ def accept(best, tokens, parents, active, pos, budget, stops) -> dict[str, list]
     names = ("path", "accept_len", "lengths", "keep", "bonus", "next_pos", "budget_left", "live", "hidden_src")
     out: dict[str, list] = {n: [] for n in names}
     for j, row in enumerate(best):
-        t, way = len(row), [0]
+        t, way, present = len(row), [0], ways(parents[j])
         while len(way) < budget[j] and row[way[-1]] not in stops[j]:
-            below = [s for s in range(way[-1] + 1, t) if parents[j][s] == way[-1] and tokens[j][s] == row[way[-1]]]
+            below = [s for s in range(way[-1] + 1, t) if parents[j][s] == way[-1] and present[s] and tokens[j][s] == row[way[-1]]]
             if not below:
                 break
             way.append(below[0])

@@ -41,8 +41,9 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(TreeAcceptArgs a) {
   bool stop = false;
   for (int i = 0; i < a.n_stops; ++i) stop |= node && a.stops[(int64_t)b * a.n_stops + i] == best;
   const uint64_t stops = __ballot(stop);
+  const bool rooted = __builtin_amdgcn_readlane(parent, 0) == -1;  // else node 0, and so all that hangs below it, is absent
   int at = 0, n = 0, mine = 0;
-  while (n + 1 < budget && !(stops >> at & 1ull)) {
+  while (rooted && n + 1 < budget && !(stops >> at & 1ull)) {
     const uint64_t fits = __ballot(parent == at && token == lane_value(best, at));  // a parent comes before its children
     if (fits == 0ull) break;
     at = __builtin_ctzll(fits);

@@ -228,7 +228,7 @@ def tree_accept(step_argmax: torch.Tensor, tokens: torch.Tensor, parents: torch.
                 pos: torch.Tensor, budget: torch.Tensor, stops: torch.Tensor) -> TreeAccept:
     """`greedy_accept` for trees of up to 64 drafts (`mtpk_tree_accept`): from node 0, the lane's own token, on to the lowest
     child whose token is `step_argmax` of the node it hangs below, while there is one, that argmax is no stop id and the
-    budget lasts. step_argmax, tokens int64 `[B, t]`; parents `[B, t]` as in `attention.paged_attention_tree`; active bool
+    budget lasts; nothing is accepted below a node 0 that is absent. step_argmax, tokens int64 `[B, t]`; parents `[B, t]` as in `attention.paged_attention_tree`; active bool
     `[B]`; pos, budget int64 `[B]`; stops int64 `[B, S]`, -1 padded. CPU tensors take the torch spelling."""
     if not step_argmax.is_cuda:
         return tree_accept_torch(step_argmax, tokens, parents, active, pos, budget, stops)
@@ -242,7 +242,7 @@ def tree_accept_torch(step_argmax: torch.Tensor, tokens: torch.Tensor, parents: 
     b, t = step_argmax.shape
     lane, node = torch.arange(b, device=pos.device), torch.arange(t, device=pos.device)
     at, n = torch.zeros_like(pos), torch.zeros_like(pos)
-    going = torch.ones_like(active)
+    going = parents[:, 0] == -1  # else node 0, and so all that hangs below it, is absent
     path = [at]
     for i in range(1, t):
         best = step_argmax[lane, at]
@@ -400,7 +400,7 @@ def verify_tree(model, lanes, tokens: torch.Tensor, parents: torch.Tensor, pos: 
     rows, the DeltaNet states (`Model.commit_path`), the MTP cache and the hidden seed. The slots are then where the accepted
     tokens, one after another, would have left them; `bonus` is each lane's next token, at `next_pos`.
 
-    `lanes` distinct; `tokens` int64 `[B, t]`, t up to 64, node 0 the lane's last committed token at `pos` `[B]`; `parents` `[B, t]` as in
+    `lanes` distinct; `tokens` int64 `[B, t]`, t up to 64, node 0, with parent -1, the lane's last committed token at `pos` `[B]`; `parents` `[B, t]` as in
     `attention.paged_attention_tree`; `budget`, `stops` as in `tree_accept`; `ctx_len` a host bound on `max(pos) + t`. The lanes'
     blocks must hold `pos + t` positions (`BlockTables.grow_many`). `mtp` defaults to the model's attached head. Rows with
     `active` False touch no lane state. No host read: the call can be captured."""
