@@ -296,17 +296,17 @@ def copy_blocks(pools: list[torch.Tensor], src, dst, block: int = BLOCK) -> None
 
 
 def keep_path(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: torch.Tensor, path: torch.Tensor,
-              lengths: torch.Tensor) -> None:
+              lengths: torch.Tensor, block: int = BLOCK) -> None:
     """The accepted rows of verified trees, moved together: of lane b, cache position `base_pos[b] + path[b, i]` becomes
     position `base_pos[b] + i` for `i < lengths[b]`, in every pool in one launch (`mtpk_keep_path`): K pools `[rows, kv_heads,
-    hd]` and V pools `[rows / 16, kv_heads, hd, 16]` of one cache's layers, read through the lanes' `block_table` `[B, blocks]`.
+    hd]` and V pools `[rows / block, kv_heads, hd, block]` of one cache's layers, read through the lanes' `block_table` `[B, blocks]`.
 
     `path` int32 or int64 `[B, t]`, t up to 64, rises in its first `lengths[b]` entries (`graph_mtp.tree_accept`); an entry
     that is no node of `[0, t)` ends it. Rows outside the lane's table, and blocks outside the pools, are left.
     No two pools share memory, and the blocks of a lane's rows from `base_pos[b]` on are no other lane's of the call.
-    CPU pools take the torch spelling."""
-    if pools and not pools[0].is_cuda:
-        _keep_path_torch(pools, block_table, base_pos, path, lengths)
+    CPU pools, and blocks of other than 16 rows, take the torch spelling, which reads nothing on the host either."""
+    if pools and not (pools[0].is_cuda and block == BLOCK):
+        _keep_path_torch(pools, block_table, base_pos, path, lengths, block)
         return
     if not pools:
         raise ValueError("keep_path takes at least one pool")
@@ -314,8 +314,8 @@ def keep_path(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: to
 
 
 def _keep_path_torch(pools: list[torch.Tensor], block_table: torch.Tensor, base_pos: torch.Tensor, path: torch.Tensor,
-                     lengths: torch.Tensor) -> None:
-    n_blocks = _pool_blocks(pools, BLOCK)
+                     lengths: torch.Tensor, block: int) -> None:
+    n_blocks, device = _pool_blocks(pools, block), pools[0].device
     spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in pools)
     if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
         raise ValueError("pools must not share memory")
@@ -325,20 +325,26 @@ def _keep_path_torch(pools: list[torch.Tensor], block_table: torch.Tensor, base_
     if block_table.dim() != 2 or block_table.shape[0] != b or tuple(base_pos.shape) != (b,) or tuple(lengths.shape) != (b,):
         raise ValueError(f"block_table must be [{b}, blocks], base_pos and lengths [{b}]")
     for name, x in (("block_table", block_table), ("base_pos", base_pos), ("path", path), ("lengths", lengths)):
-        if x.dtype not in (torch.int32, torch.int64) or x.is_cuda:
+        if x.dtype not in (torch.int32, torch.int64) or x.device != device:
             raise ValueError(f"{name} must be int32 or int64 beside the pools, got {x.dtype} on {x.device}")
-    node = torch.arange(t)
+    if b == 0 or block_table.shape[1] == 0:
+        return
+    node = torch.arange(t, device=device)
     path, base, table = path.long(), base_pos.long()[:, None], block_table.long()
     on = ((path >= 0) & (path < t)).int().cumprod(1).bool() & (node < lengths[:, None])
     src, dst = (base + x for x in (path, node.expand(b, t)))
-    end = table.shape[1] * BLOCK
+    end = table.shape[1] * block
     on &= (src >= 0) & (src < end) & (dst >= 0) & (dst < end)
-    at = [(table.gather(1, x.clamp(0, end - 1) // BLOCK), x % BLOCK) for x in (src, dst)]
+    at = [(table.gather(1, x.clamp(0, end - 1) // block), x % block) for x in (src, dst)]
     for blocks, _ in at:
         on &= (blocks >= 0) & (blocks < n_blocks)
-    (sb, sr), (db, dr) = ((blocks[on], rows[on]) for blocks, rows in at)
+    # A row that stays goes along as the first that moves, which is then written twice alike; where none does, as a move in place.
+    on = on.reshape(-1)
+    take = torch.where(on, torch.arange(b * t, device=device), on.int().argmax())
+    (sb, sr), (db, dr) = ((blocks.clamp(0, n_blocks - 1).reshape(-1)[take], rows.reshape(-1)[take]) for blocks, rows in at)
+    db, dr = (torch.where(on.any(), d, s) for d, s in ((db, sb), (dr, sr)))
     for p in pools:
         if p.dim() == 3:
-            p[db * BLOCK + dr] = p[sb * BLOCK + sr]
+            p[db * block + dr] = p[sb * block + sr]
         else:
             p[db, :, :, dr] = p[sb, :, :, sr]

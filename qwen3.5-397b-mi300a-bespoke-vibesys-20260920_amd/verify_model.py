@@ -1033,7 +1033,7 @@ class Model:
         kept = lengths if active is None else torch.where(active, lengths, torch.zeros_like(lengths))
         pools = [p[name] for ty, p in zip(c.layer_types, self.pool) if ty == ATTN for name in ("k", "v")]
         if pools:
-            attention.keep_path(pools, table, base_pos.to(self.device, torch.long), path, kept)
+            attention.keep_path(pools, table, base_pos.to(self.device, torch.long), path, kept, c.block_size)
         for i, rows in res.dn_rows.items():
             pool = self.pool[i]
             if self.device.type == "cuda" and rows.proj is not None:
