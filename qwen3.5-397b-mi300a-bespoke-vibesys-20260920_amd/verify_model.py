@@ -964,13 +964,14 @@ class Model:
         qe, ke = q.repeat_interleave(rep, dim=2), k.repeat_interleave(rep, dim=2)
         state = pool["rec"][lanes]
         outs = []
-        after = [state]  # a tree's states: the stored one, then after each node
+        after = [] if parents is None else [state]  # a tree's states: the stored one, then after each node
         for s in range(t):
             if parents is not None:  # the state after the node's parent
                 state = torch.stack(after, 1)[torch.arange(b), parents[:, s].long().clamp(-1, s - 1) + 1]
             state, o = delta_rule_step(state, qe[:, s], ke[:, s], v[:, s], g[:, s], beta[:, s])
             outs.append(o)
-            after.append(state)
+            if parents is not None:
+                after.append(state)
         out = torch.stack(outs, dim=1)  # [B, t, vh, vd] fp32
         if parents is not None:
             present = tree_ancestors(parents).any(2)
