@@ -1027,7 +1027,8 @@ class Model:
                     block_table: torch.Tensor | None = None, active: torch.Tensor | None = None) -> None:
         """`commit` after a tree's forward (`forward_rows(parents=)`): the accepted path's cache rows move together in every
         attention layer (`attention.keep_path`), and every DeltaNet layer's state advances along it (`deltanet.commit_path`).
-        `path` int64 `[B, t]` and `lengths` `[B]` from `graph_mtp.tree_accept`; rows with `active` False touch nothing."""
+        `path` int64 `[B, t]` and `lengths` `[B]` from `graph_mtp.tree_accept` (an entry that is no node ends a path); rows with
+        `active` False touch nothing."""
         c = self.cfg
         lanes = self.lane_index(lanes)
         table = self.blocks.table[lanes] if block_table is None else block_table
@@ -1042,11 +1043,13 @@ class Model:
                 deltanet.commit_path(pool["rec"], pool["conv"], slots, rows.k, rows.v, rows.g, rows.beta, path, kept,
                                      rows.proj, c.conv_dim)
                 continue
-            on = path.long()  # the path's rows in order, then the chain's commit
+            t = path.shape[1]  # the path's rows up to its end in order, then the chain's commit
+            n = ((path >= 0) & (path < t)).int().cumprod(1).sum(1).minimum(lengths).clamp(min=0)
+            on = path.long().clamp(0, t - 1)
             take = lambda x: x.gather(1, on.view(*on.shape, *[1] * (x.dim() - 2)).expand_as(x))  # noqa: E731, B023
             chain = DeltaNetRows(rows.raw_qkv.gather(2, on[:, None].expand_as(rows.raw_qkv)), take(rows.q), take(rows.k),
                                  take(rows.v), take(rows.g), take(rows.beta))
-            self.deltanet_commit(pool, chain, lanes, lengths, None, active)
+            self.deltanet_commit(pool, chain, lanes, n, None, active)
 
     # ------------------------------------------------------------ forward
 
