@@ -741,7 +741,9 @@ int mtpk_deltanet_prep_tree(const void* proj, int dtype, int64_t proj_stride, co
 /* mtpk_delta_rule's verify mode for a tree: node s runs one step on its parent's state (-1: its slot's stored one),
  * out [rows, t, heads, v_dim] holds every node's output; the stored states are read alone. slot may be NULL (row j: slot j);
  * rows of a slot outside the pool give zeros. A launch of 2^32 threads or more is refused: with slabs = ceil(v_dim / 64),
- * rows * qk_heads * ceil(heads / qk_heads * slabs / 4) must be below 2^24, and rows * heads * slabs at most 2^26 - 4. */
+ * rows * qk_heads * ceil(heads / qk_heads * slabs / 4) must be below 2^24, and rows * heads * slabs at most 2^26 - 4.
+ * Made for the layer's inputs: of a present node |k|^2 at most 1.01, g <= 0, beta in [0, 1], all of them finite. Others are
+ * taken too, but each (row, head) that holds one does its columns node by node from memory, 8 to 30 times slower. */
 int mtpk_delta_rule_tree(const float* state, int64_t slots_total, const int64_t* slot, int64_t rows, int64_t t, int64_t heads,
                          int64_t qk_heads, int64_t k_dim, int64_t v_dim, const float* q, const float* k, const float* v,
                          const float* g, const float* beta, const void* parents, int parents_dtype, const int64_t* parents_strides,

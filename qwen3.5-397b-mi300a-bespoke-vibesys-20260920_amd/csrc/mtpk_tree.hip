@@ -71,7 +71,7 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(TreeAcceptArgs a) {
 // of all layers at once. A path rises, so a row is read before a later one takes its place, and never written before it
 // is read, if each thread moves its share of the rows in order. Of K that is 16 bytes of every row; of V, which lies
 // transposed in its block, one channel's line of the block's positions. A chain of latencies, base and path, table, rows, store:
-// 30 pools of one lane 3.9 us, of 48 lanes with up to 8 rows 10.6.
+// 30 pools of one lane 3.9 us. Of 48 lanes with up to 8 rows 10.6: V goes two bytes at a time, out of a line of 32 for each row.
 constexpr int kKeepPools = 64;  // pools a launch takes
 constexpr int kKeepAhead = 8;   // rows on their way at once
 constexpr int kKeepBlock = 16;  // rows of a cache block

@@ -194,7 +194,8 @@ def delta_rule_tree(state: torch.Tensor, slots: torch.Tensor | None, q: torch.Te
     """`delta_rule`'s verify mode for trees of up to 64 drafts (`mtpk_delta_rule_tree`): node s of row j takes its step from
     the state after its parent `parents[j, s]` (-1: the slot's stored state), so its output is that of a chain of its
     ancestors and itself. `parents` `[B, t]` as in `attention.paged_attention_tree`; absent nodes give zeros. The states are
-    read and not written (`commit_path` advances them). Returns f32 `[B, t, heads, v_dim]`."""
+    read and not written (`commit_path` advances them). Returns f32 `[B, t, heads, v_dim]`. Inputs that `prep_tree` does not make
+    (`|k|^2` above 1.01, `g` above 0, `beta` outside [0, 1], values that are not finite) are taken, but 8 to 30 times slower."""
     return _mtpk.native().delta_rule_tree(state, slots, q, k, v, g, beta, parents, _mtpk.stream_for(state))
 
 
